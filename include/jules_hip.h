@@ -351,6 +351,132 @@ int jules_hip_cross_entropy(const float* logits, const int32_t* targets,
                             void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* ---- residual addition + root-mean-square norm -----------------------------
+ * h = x + residual,  y = h / sqrt(mean(h^2) + epsilon) * weight,  row by row of
+ * [M, N].  No counterpart in the reference: the norm between the products of a
+ * quantised decoder, next to jules_hip_layernorm.
+ * x_dtype, residual_dtype: JH_F32 or JH_BF16, each by itself; weight fp32 [N].
+ * residual NULL: h = x (residual_dtype is not looked at).  residual_out: NULL,
+ * or [M, N] of residual_dtype that receives h rounded to it; it may be
+ * `residual`.  The norm is of h in fp32, before that rounding.
+ * out_dtype JH_F32 or JH_BF16: out [M, N] receives y; it may be x where the
+ *   types are the same; scale must be NULL.
+ * out_dtype JH_I8: out int8 [M, N] receives rint(y / s) (ties to even) in
+ *   -127 .. 127 and scale fp32 [M] receives s = max|y| / 127 of each row: the A
+ *   and scale_A of jules_hip_matmul_w8a8.  A row of zeros gives scale 0 and
+ *   codes 0.  A row with a NaN or an infinity, or where x + residual or h *
+ *   weight passes fp32, gives scale NaN and codes 0, so that every product of
+ *   the row is NaN.
+ * Sums of squares are held in 64 bits.  Deterministic.  epsilon >= 0; with 0 a
+ * row of zeros is NaN in fp32 and bf16, and the factor of one whose root mean
+ * square is below 2^-127 passes fp32.  Pointers aligned to their elements.
+ */
+int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const void* x,
+                          const void* residual, const float* weight, void* residual_out,
+                          void* out, float* scale, int M, int N, float epsilon, void* stream);
+
+/* ---- rotary positions --------------------------------------------------------
+ * Rotates pairs of elements of x [B, H, S, D] by the angle a(p, b, s) =
+ * positions[pair_axis[p]][b][s] * inv_freq[p], p = 0 .. R/2 - 1:
+ *   (u, w) -> (u cos a - w sin a, u sin a + w cos a)
+ * pairing 0: u, w = elements p and p + R/2; pairing 1: elements 2p and 2p + 1.
+ * Elements R .. D - 1 are copied.  inverse = 1 rotates by -a: the gradient of x
+ * from that of out.  No counterpart in the reference: the positions of
+ * jules_hip_flash_attn_fwd's or jules_hip_kv4_attention's queries and keys.
+ * x_dtype, out_dtype: JH_F32 or JH_BF16, each by itself; arithmetic in fp32,
+ * angles in fp64 (less than 10^-6 off at any int32 position).
+ * x_strides, out_strides: host arrays of 3, the elements between two batches,
+ * heads and tokens; the D elements of a head lie side by side.  x may have
+ * strides of 0; out's must keep its elements apart (JH_ERR_ARG otherwise).  out
+ * may be x with the same strides and dtype; other overlaps are not allowed.
+ * positions int32 [axes, B, S], any sign; inv_freq fp64 [R/2]; pair_axis int32
+ * [R/2] or NULL (axis 0); a pair whose axis is outside [0, axes) gives NaN.
+ * 2 <= R <= D, R even, D <= 1024, 1 <= axes <= 16, B * S <= 2^28, H <= 65535.
+ */
+int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const void* x,
+                     const int64_t* x_strides, void* out, const int64_t* out_strides,
+                     const int32_t* positions, const double* inv_freq, const int32_t* pair_axis,
+                     int axes, int B, int H, int S, int D, int R, void* stream);
+
+/* ---- key/value cache held in 4 bits -------------------------------------------
+ * A paged cache, next to jules_hip_flash_attn_fwd (which takes whole [B,H,S,D]
+ * tensors).  No counterpart in the reference.  A row is the D values of one token and key/value
+ * head, held as a scale s and a minimum m (bf16 each) and D codes of 4 bits;
+ * code c stands for m + s c.  Device arrays, pages of page_size tokens:
+ *   k       [num_pages][heads][page_size][D/2] bytes; of 8 neighbouring elements
+ *           e = 0..7 the four bytes hold (e0, e2), (e4, e6), (e1, e3), (e5, e7),
+ *           the first of each two in the low 4 bits
+ *   v       [num_pages][heads][page_size/4][D/4][8] bytes; of 4 neighbouring
+ *           tokens and elements the eight bytes hold (e0, e1), (e2, e3) of the
+ *           first token, then of the others
+ *   k_meta, v_meta  [num_pages][heads][page_size][2] bf16: s, m
+ * k and v 16-byte, k_meta and v_meta 16-byte aligned.  head_dim 64 or 128 (others
+ * JH_ERR_UNSUPPORTED), page_size 16, 32, 64, 128 or 256; heads <=
+ * 65535; num_pages >= 1.
+ *
+ * A batch's new tokens, the same four arguments in the three calls:
+ *   table   int32 [batch, max_pages]: the pages of each sequence in order
+ *   lens    int32 [batch]: tokens of each sequence, the new ones among them
+ *   cu_q    int32 [batch + 1] or NULL: rows cu_q[b] .. cu_q[b+1] - 1 of the packed
+ *           arrays belong to sequence b, ascending, and are its last ones; rows
+ *           outside cu_q[0] .. cu_q[batch] - 1 are not touched.  NULL: max_q rows
+ *           each, tokens = batch * max_q.
+ *   max_q   the largest number of new tokens of a sequence.  With cu_q it is a
+ *           hint: a wrong one costs time, not results.
+ * These arrays are on the device, so their contents are not checked by a status;
+ * whatever they hold, nothing outside the arrays is read or written.  Page
+ * numbers outside [0, num_pages) and positions past max_pages * page_size are no pages:
+ * a row appended there is dropped, a row read there is NaN, and so is the
+ * attention of a token that sees such a position.  Pages of two sequences may be
+ * the same (a shared beginning), but not where both append.
+ *
+ * jules_hip_kv4_append: writes the new rows.  dtype JH_F32 or JH_BF16, k and v
+ *   [tokens, heads, D] with strides in elements between tokens and heads (the D
+ *   elements side by side); s = bf16((max - min) / 15), m = bf16(min), c =
+ *   clamp(rint((x - m) / s), 0, 15), 0 where s is 0.  A row with a NaN or an
+ *   infinity, or a range past fp32 or a minimum past bf16, is held as NaN throughout.
+ *   A row before position 0 is dropped.
+ * jules_hip_kv4_read: the new rows as values m + s c into dense k and v
+ *   [tokens, heads, D] of dtype, 16-byte aligned; 0 for a row before position 0.
+ * jules_hip_kv4_attention: o = softmax(scale * q K^T) V for the new tokens, each
+ *   over its sequence's keys up to its own position.  q bf16 [tokens, heads_q, D]
+ *   by strides (multiples of 8 elements, q 16-byte aligned), heads_q a multiple
+ *   of the cache's heads (head i reads head i / (heads_q / heads)); out bf16
+ *   [tokens, heads_q, D] dense, 16-byte aligned; lse NULL or fp32 [tokens, heads_q]:
+ *   natural-log log-sum-exp of the scaled scores.  A token that sees no key gets 0
+ *   and lse -infinity.  A key row held as NaN makes the rows that see it NaN.
+ *   scale finite and > 0.  max_len: the largest of lens, a hint like max_q.
+ *   tokens * heads_q <= 2^30.
+ *   workspace: jules_hip_kv4_attention_workspace_size(...) bytes for the same
+ *   arguments, 16-byte aligned, no initialisation, overwritten by every call;
+ *   calls that overlap in time need separate ones (0 bytes: NULL will do).
+ *   fp32 accumulation and softmax; probabilities times the value's scale are
+ *   rounded to bf16.  Deterministic.  The calls may be captured in a graph.
+ */
+typedef struct jh_kv4_cache {
+    void* k;
+    void* v;
+    void* k_meta;
+    void* v_meta;
+    int32_t num_pages, page_size, heads, head_dim;
+} jh_kv4_cache;
+
+int jules_hip_kv4_append(int dtype, const jh_kv4_cache* cache, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                         int64_t v_head_stride, const int32_t* table, int max_pages,
+                         const int32_t* lens, const int32_t* cu_q, int batch, int tokens, int max_q,
+                         void* stream);
+int jules_hip_kv4_read(int dtype, const jh_kv4_cache* cache, void* k, void* v, const int32_t* table,
+                       int max_pages, const int32_t* lens, const int32_t* cu_q, int batch, int tokens,
+                       int max_q, void* stream);
+size_t jules_hip_kv4_attention_workspace_size(int batch, int tokens, int heads_q, int heads, int head_dim,
+                                              int max_q, int max_len);
+int jules_hip_kv4_attention(float scale, const jh_kv4_cache* cache, const void* q, int64_t q_token_stride,
+                            int64_t q_head_stride, void* out, float* lse, int heads_q,
+                            const int32_t* table, int max_pages, const int32_t* lens,
+                            const int32_t* cu_q, int batch, int tokens, int max_q, int max_len,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- 2-layer MLP forward ---------------------------------------------------
  * output [M,N2] = relu(X W1 + b1) W2 + b2, fp32 row-major; X [M,K1],
  * W1 [K1,N1], b1 [N1], W2 [N1,N2], b2 [N2].

@@ -28,6 +28,11 @@ class JhTensor(ctypes.Structure):
                 ("rank", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
+class JhKV4Cache(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_meta", _vp), ("v_meta", _vp), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
 KERNEL_FN = ctypes.CFUNCTYPE(_int, _int, ctypes.POINTER(JhTensor), _int, ctypes.POINTER(JhTensor),
                              ctypes.c_char_p, _vp)
 
@@ -65,6 +70,16 @@ SIGNATURES = {
     "jules_hip_layernorm": (_int, [_vp, _vp, _vp, _vp, _int, _int, _f32, _vp]),
     "jules_hip_cross_entropy_workspace_size": (_size, [_int]),
     "jules_hip_cross_entropy": (_int, [_vp, _vp, _vp, _vp, _int, _int, _vp, _size, _vp]),
+    "jules_hip_add_rmsnorm": (_int, [_int, _int, _int] + [_vp] * 6 + [_int, _int, _f32, _vp]),
+    "jules_hip_rotary": (_int, [_int] * 4 + [_vp, ctypes.POINTER(_i64), _vp, ctypes.POINTER(_i64)] + [_vp] * 3 +
+                         [_int] * 6 + [_vp]),
+    "jules_hip_kv4_append": (_int, [_int, ctypes.POINTER(JhKV4Cache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _int,
+                                    _vp, _vp, _int, _int, _int, _vp]),
+    "jules_hip_kv4_read": (_int, [_int, ctypes.POINTER(JhKV4Cache), _vp, _vp, _vp, _int, _vp, _vp, _int, _int, _int,
+                                  _vp]),
+    "jules_hip_kv4_attention_workspace_size": (_size, [_int] * 7),
+    "jules_hip_kv4_attention": (_int, [_f32, ctypes.POINTER(JhKV4Cache), _vp, _i64, _i64, _vp, _vp, _int, _vp, _int,
+                                       _vp, _vp] + [_int] * 4 + [_vp, _size, _vp]),
     "jules_hip_mlp_forward_workspace_size": (_size, [_int, _int, _int, _int]),
     "jules_hip_mlp_forward": (_int, [_vp] * 6 + [_int] * 4 + [_vp, _size, _vp]),
     "jules_hip_mlp_workspace_size": (_size, [_int, _int, _int, _int]),

@@ -15,6 +15,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <string>
+#include <utility>
 
 #include "jules_hip.h"
 #include "launch.hpp"
@@ -461,6 +462,192 @@ int jules_hip_cross_entropy(const float* logits, const int32_t* targets, float* 
                                               static_cast<float*>(workspace), M, N,
                                               static_cast<hipStream_t>(stream)),
                      "cross_entropy launch");
+}
+
+int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const void* x, const void* residual,
+                          const float* weight, void* residual_out, void* out, float* scale, int M, int N,
+                          float epsilon, void* stream) {
+    const auto real = [](int t) { return t == JH_F32 || t == JH_BF16; };
+    if (!real(x_dtype) || (residual && !real(residual_dtype)) || (!real(out_dtype) && out_dtype != JH_I8))
+        return fail(JH_ERR_DTYPE, "add_rmsnorm: dtypes %d %d %d", x_dtype, residual_dtype, out_dtype);
+    const int st = row_shape("add_rmsnorm", M, N);
+    if (st != JH_OK) return st;
+    if (!(std::isfinite(epsilon) && epsilon >= 0.0f)) return fail(JH_ERR_ARG, "add_rmsnorm: epsilon %g", epsilon);
+    if (residual_out && !residual) return fail(JH_ERR_ARG, "add_rmsnorm: residual_out without residual");
+    if (scale && out_dtype != JH_I8) return fail(JH_ERR_ARG, "add_rmsnorm: scale is of int8 rows only");
+    if (M == 0 || N == 0) return JH_OK;
+    if (!x || !weight || !out || (out_dtype == JH_I8 && !scale))
+        return fail(JH_ERR_NULL, "add_rmsnorm: null x, weight, out or scale");
+    const auto size = [](int t) { return t == JH_F32 ? 4 : t == JH_BF16 ? 2 : 1; };
+    if (!aligned(x, size(x_dtype)) || !aligned(weight, 4) || !aligned(out, size(out_dtype)) || !aligned(scale, 4) ||
+        (residual && (!aligned(residual, size(residual_dtype)) || !aligned(residual_out, size(residual_dtype)))))
+        return fail(JH_ERR_ALIGN, "add_rmsnorm: pointers must be aligned to their elements");
+    return check_hip(jh::launch_add_rmsnorm(x_dtype, residual_dtype, out_dtype, x, residual, weight, residual_out, out,
+                                            scale, M, N, epsilon, static_cast<hipStream_t>(stream)),
+                     "add_rmsnorm launch");
+}
+
+// Whether the elements of a [sizes] array with these strides, rows of D side by
+// side, lie apart: each axis steps past everything the smaller ones span.
+static bool apart(const int64_t* strides, const int* sizes, int D) {
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (strides[order[j]] < strides[order[i]]) std::swap(order[i], order[j]);
+    int64_t span = D;
+    for (const int i : order) {
+        if (sizes[i] <= 1) continue;
+        if (strides[i] < span) return false;
+        span += strides[i] * (sizes[i] - 1);
+    }
+    return true;
+}
+
+int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const void* x, const int64_t* x_strides,
+                     void* out, const int64_t* out_strides, const int32_t* positions, const double* inv_freq,
+                     const int32_t* pair_axis, int axes, int B, int H, int S, int D, int R, void* stream) {
+    const auto real = [](int t) { return t == JH_F32 || t == JH_BF16; };
+    if (!real(x_dtype) || !real(out_dtype)) return fail(JH_ERR_DTYPE, "rotary: dtypes %d %d", x_dtype, out_dtype);
+    if ((pairing != 0 && pairing != 1) || (inverse != 0 && inverse != 1))
+        return fail(JH_ERR_ARG, "rotary: pairing %d, inverse %d (0 or 1)", pairing, inverse);
+    if (B < 0 || H < 0 || S < 0 || H > 65535 || (int64_t)B * S > (int64_t(1) << 28))
+        return fail(JH_ERR_SHAPE, "rotary: B=%d H=%d S=%d", B, H, S);
+    if (D < 2 || D > 1024 || R < 2 || R > D || R % 2)
+        return fail(JH_ERR_SHAPE, "rotary: D=%d R=%d (2 <= R <= D <= 1024, R even)", D, R);
+    if (axes < 1 || axes > 16) return fail(JH_ERR_SHAPE, "rotary: axes %d (1..16)", axes);
+    if (B == 0 || H == 0 || S == 0) return JH_OK;
+    if (!x || !out || !x_strides || !out_strides || !positions || !inv_freq)
+        return fail(JH_ERR_NULL, "rotary: null x, out, strides, positions or inv_freq");
+    if (!aligned(x, x_dtype == JH_F32 ? 4 : 2) || !aligned(out, out_dtype == JH_F32 ? 4 : 2) || !aligned(positions, 4) ||
+        !aligned(inv_freq, 8) || !aligned(pair_axis, 4))
+        return fail(JH_ERR_ALIGN, "rotary: pointers must be aligned to their elements");
+    const int sizes[3] = {B, H, S};
+    for (int i = 0; i < 3; ++i)
+        if (x_strides[i] < 0 || out_strides[i] < 0 || x_strides[i] > kMaxElems || out_strides[i] > kMaxElems)
+            return fail(JH_ERR_ARG, "rotary: strides must be 0 .. 2^40");
+    if (!apart(out_strides, sizes, D)) return fail(JH_ERR_ARG, "rotary: elements of out overlap");
+    if (x == out) {
+        bool same = x_dtype == out_dtype;
+        for (int i = 0; i < 3; ++i) same = same && (sizes[i] <= 1 || x_strides[i] == out_strides[i]);
+        if (!same) return fail(JH_ERR_ARG, "rotary: in place needs the same strides and dtype");
+    }
+    return check_hip(jh::launch_rotary(x_dtype, out_dtype, pairing == 0, inverse != 0, x, x_strides, out, out_strides,
+                                       positions, inv_freq, pair_axis, axes, B, H, S, D, R,
+                                       static_cast<hipStream_t>(stream)),
+                     "rotary launch");
+}
+
+// checks shared by the calls on the 4-bit cache; *done: nothing to compute
+static int kv4_check(const char* who, const jh_kv4_cache* c, const int32_t* table, int max_pages, const int32_t* lens,
+                     const int32_t* cu_q, int batch, int tokens, int max_q, jh::KV4View* view, jh::KV4Batch* b,
+                     bool* done) {
+    *done = false;
+    if (!c) return fail(JH_ERR_NULL, "%s: null cache", who);
+    if (batch < 0 || tokens < 0 || max_q < 0 || max_pages < 0 || c->num_pages < 1)
+        return fail(JH_ERR_SHAPE, "%s: batch=%d tokens=%d max_q=%d max_pages=%d num_pages=%d", who, batch, tokens, max_q,
+                    max_pages, c->num_pages);
+    if (c->heads < 1 || c->heads > 65535) return fail(JH_ERR_SHAPE, "%s: %d heads (1..65535)", who, c->heads);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(JH_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", who, c->head_dim);
+    int shift = 4;
+    while (shift < 8 && c->page_size != 1 << shift) ++shift;
+    if (c->page_size != 1 << shift)
+        return fail(JH_ERR_UNSUPPORTED, "%s: page_size %d (16, 32, 64, 128 or 256)", who, c->page_size);
+    if ((int64_t)c->num_pages * c->heads * c->page_size > kMaxElems / c->head_dim)
+        return fail(JH_ERR_SHAPE, "%s: cache too large", who);
+    if (!cu_q && (int64_t)batch * max_q != tokens)
+        return fail(JH_ERR_SHAPE, "%s: %d tokens, batch %d of %d each", who, tokens, batch, max_q);
+    if (batch == 0 || tokens == 0) {
+        *done = true;
+        return JH_OK;
+    }
+    if (!lens || (!table && max_pages > 0)) return fail(JH_ERR_NULL, "%s: null table or lens", who);
+    if (!c->k || !c->v || !c->k_meta || !c->v_meta)
+        return fail(JH_ERR_NULL, "%s: null cache array", who);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_meta, 16) || !aligned(c->v_meta, 16))
+        return fail(JH_ERR_ALIGN, "%s: cache arrays must be 16-byte aligned", who);
+    if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(cu_q, 4))
+        return fail(JH_ERR_ALIGN, "%s: table, lens and cu_q must be 4-byte aligned", who);
+    *view = {static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), static_cast<uint32_t*>(c->k_meta),
+             static_cast<uint32_t*>(c->v_meta), c->num_pages, c->page_size, shift, c->heads, c->head_dim};
+    *b = {table, lens, cu_q, max_pages, batch, tokens, max_q};
+    return JH_OK;
+}
+
+static bool row_strides(int64_t token, int64_t head) {
+    return token >= 0 && head >= 0 && token <= kMaxElems && head <= kMaxElems;
+}
+
+int jules_hip_kv4_append(int dtype, const jh_kv4_cache* cache, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                         const int32_t* table, int max_pages, const int32_t* lens, const int32_t* cu_q, int batch,
+                         int tokens, int max_q, void* stream) {
+    if (dtype != JH_F32 && dtype != JH_BF16) return fail(JH_ERR_DTYPE, "kv4_append: dtype %d", dtype);
+    jh::KV4View view;
+    jh::KV4Batch b;
+    bool done;
+    const int st = kv4_check("kv4_append", cache, table, max_pages, lens, cu_q, batch, tokens, max_q, &view, &b, &done);
+    if (st != JH_OK || done) return st;
+    if (!k || !v) return fail(JH_ERR_NULL, "kv4_append: null k or v");
+    const size_t size = dtype == JH_F32 ? 4 : 2;
+    if (!aligned(k, size) || !aligned(v, size)) return fail(JH_ERR_ALIGN, "kv4_append: alignment of k or v");
+    if (!row_strides(k_token_stride, k_head_stride) || !row_strides(v_token_stride, v_head_stride))
+        return fail(JH_ERR_ARG, "kv4_append: strides must be 0 .. 2^40");
+    return check_hip(jh::launch_kv4_append(dtype, view, b, k, k_token_stride, k_head_stride, v, v_token_stride,
+                                           v_head_stride, static_cast<hipStream_t>(stream)),
+                     "kv4_append launch");
+}
+
+int jules_hip_kv4_read(int dtype, const jh_kv4_cache* cache, void* k, void* v, const int32_t* table, int max_pages,
+                       const int32_t* lens, const int32_t* cu_q, int batch, int tokens, int max_q, void* stream) {
+    if (dtype != JH_F32 && dtype != JH_BF16) return fail(JH_ERR_DTYPE, "kv4_read: dtype %d", dtype);
+    jh::KV4View view;
+    jh::KV4Batch b;
+    bool done;
+    const int st = kv4_check("kv4_read", cache, table, max_pages, lens, cu_q, batch, tokens, max_q, &view, &b, &done);
+    if (st != JH_OK || done) return st;
+    if (!k || !v) return fail(JH_ERR_NULL, "kv4_read: null k or v");
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(JH_ERR_ALIGN, "kv4_read: k and v must be 16-byte aligned");
+    return check_hip(jh::launch_kv4_read(dtype, view, b, k, v, static_cast<hipStream_t>(stream)), "kv4_read launch");
+}
+
+size_t jules_hip_kv4_attention_workspace_size(int batch, int tokens, int heads_q, int heads, int head_dim, int max_q,
+                                              int max_len) {
+    if (batch < 1 || tokens < 1 || heads < 1 || heads_q < heads || heads_q % heads || max_q < 0 || max_len < 0 ||
+        (head_dim != 64 && head_dim != 128) || (int64_t)tokens * heads_q > int64_t(1) << 30)
+        return 0;
+    return jh::kv4_attn_workspace_size(batch, tokens, heads_q, heads, head_dim, max_q, max_len);
+}
+
+int jules_hip_kv4_attention(float scale, const jh_kv4_cache* cache, const void* q, int64_t q_token_stride,
+                            int64_t q_head_stride, void* out, float* lse, int heads_q, const int32_t* table,
+                            int max_pages, const int32_t* lens, const int32_t* cu_q, int batch, int tokens, int max_q,
+                            int max_len, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!(std::isfinite(scale) && scale > 0.0f)) return fail(JH_ERR_ARG, "kv4_attention: scale %g", scale);
+    jh::KV4View view;
+    jh::KV4Batch b;
+    bool done;
+    const int st =
+        kv4_check("kv4_attention", cache, table, max_pages, lens, cu_q, batch, tokens, max_q, &view, &b, &done);
+    if (st != JH_OK) return st;
+    if (heads_q < 1 || heads_q % cache->heads)
+        return fail(JH_ERR_SHAPE, "kv4_attention: %d query heads, %d key heads", heads_q, cache->heads);
+    if (max_len < 0 || (int64_t)tokens * heads_q > int64_t(1) << 30)
+        return fail(JH_ERR_SHAPE, "kv4_attention: max_len %d, %d tokens of %d heads", max_len, tokens, heads_q);
+    if (done) return JH_OK;
+    if (!q || !out) return fail(JH_ERR_NULL, "kv4_attention: null q or out");
+    if (!row_strides(q_token_stride, q_head_stride)) return fail(JH_ERR_ARG, "kv4_attention: strides must be 0 .. 2^40");
+    if (!aligned(q, 16) || (tokens > 1 && q_token_stride % 8) || (heads_q > 1 && q_head_stride % 8) ||
+        !aligned(out, 16) || !aligned(lse, 4))
+        return fail(JH_ERR_ALIGN, "kv4_attention: q and out 16-byte aligned, strides of q multiples of 8");
+    const size_t need = jh::kv4_attn_workspace_size(batch, tokens, heads_q, cache->heads, cache->head_dim, max_q, max_len);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(JH_ERR_WORKSPACE, "kv4_attention: workspace %zu bytes, need %zu", workspace_bytes, need);
+    if (!aligned(workspace, 16)) return fail(JH_ERR_ALIGN, "kv4_attention: workspace alignment");
+    return check_hip(jh::launch_kv4_attn(scale, view, b, static_cast<const uint16_t*>(q), q_token_stride, q_head_stride,
+                                         static_cast<uint16_t*>(out), lse, heads_q, max_len, workspace,
+                                         static_cast<hipStream_t>(stream)),
+                     "kv4_attention launch");
 }
 
 size_t jules_hip_mlp_forward_workspace_size(int M, int K1, int N1, int N2) {

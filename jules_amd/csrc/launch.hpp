@@ -170,4 +170,34 @@ size_t static_scratch_bytes();
 size_t static_scratch_partial_bytes();  // the partial-tile part; the counters follow it
 hipError_t static_scratch(void** ptr);
 
+// h = x + r; r_out = h (null: not kept); out = rows of the norm, int8 with a
+// scale a row where out_dtype is JH_I8 (rmsnorm.hip).  r may be null.
+hipError_t launch_add_rmsnorm(int x_dtype, int r_dtype, int out_dtype, const void* x, const void* r, const float* w,
+                              void* r_out, void* out, float* scale, int M, int N, float eps, hipStream_t s);
+// strides of batch, head and token, in elements (rotary.hip)
+hipError_t launch_rotary(int x_dtype, int out_dtype, bool half, bool inverse, const void* x, const int64_t* xs,
+                         void* out, const int64_t* os, const int32_t* pos, const double* freq, const int32_t* axis,
+                         int axes, int B, int H, int S, int D, int R, hipStream_t s);
+
+// the 4-bit key/value cache (layout: kv4.hpp)
+struct KV4View {
+    uint8_t *k, *v;
+    uint32_t *k_meta, *v_meta;
+    int num_pages, page_size, page_shift, heads, D;  // page_size = 1 << page_shift
+};
+// new tokens of a batch of sequences: rows cu_q[b] .. cu_q[b + 1] - 1 of packed
+// arrays of `tokens` rows are the last ones of sequence b of lens[b] tokens
+struct KV4Batch {
+    const int32_t *table, *lens, *cu_q;  // table [batch][max_pages]; cu_q null: max_q rows each
+    int max_pages, batch, tokens, max_q;
+};
+// rows of k and v by token and head strides, in elements (kv4_cache.hip)
+hipError_t launch_kv4_append(int dtype, const KV4View& c, const KV4Batch& b, const void* k, int64_t k_token,
+                             int64_t k_head, const void* v, int64_t v_token, int64_t v_head, hipStream_t s);
+hipError_t launch_kv4_read(int dtype, const KV4View& c, const KV4Batch& b, void* k, void* v, hipStream_t s);
+// attention over the cache (kv4_attn.hip); ws: kv4_attn_workspace_size bytes
+size_t kv4_attn_workspace_size(int batch, int tokens, int heads_q, int heads_kv, int D, int max_q, int max_len);
+hipError_t launch_kv4_attn(float scale, const KV4View& c, const KV4Batch& b, const uint16_t* q, int64_t q_token,
+                           int64_t q_head, uint16_t* o, float* lse, int heads_q, int max_len, void* ws, hipStream_t s);
+
 }  // namespace jh

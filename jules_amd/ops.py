@@ -10,13 +10,16 @@ stream only; all arithmetic happens in libjules_hip.so.  Names follow the
 reference's jules::kernel functions (include/jules/Kernel/FusedKernels.h,
 FlashAttention.h).
 """
+import ctypes
+
 import numpy as np
 
 import torch
 
-from ._lib import ACT, BF16, F32, check, lib
+from ._lib import ACT, BF16, F32, I8, JhKV4Cache, check, lib
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
+_REAL = (torch.float32, torch.bfloat16)
 
 
 def _stream(t):
@@ -331,6 +334,280 @@ def layernorm(x, gamma, beta, eps=1e-5, out=None):
     check(lib().jules_hip_layernorm(_ptr(out), _ptr(x), _ptr(gamma), _ptr(beta), M, N,
                                     float(eps), _stream(x)))
     return out
+
+
+def _call(t, fn, *args):
+    """check(fn(*args, stream)) on t's device and torch's current stream there,
+    whichever device is the current one."""
+    index = t.get_device()
+    if torch._C._cuda_getDevice() == index:
+        check(fn(*args, _stream(t)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, _stream(t)))
+
+
+def _add_rmsnorm(x, residual, weight, eps, out, out_types, scale, residual_out):
+    _need(x, "x", _REAL)
+    M, N = _rows(x)
+    _need(weight, "weight", (torch.float32,), numel=N)
+    if residual is not None:
+        _need(residual, "residual", _REAL, shape=x.shape)
+        if residual_out is not None:
+            _need(residual_out, "residual_out", (residual.dtype,), shape=x.shape)
+    elif residual_out is not None:
+        raise ValueError("residual_out without residual")
+    if out is not None:
+        _need(out, "out", out_types, shape=x.shape)
+    if scale is not None:
+        _need(scale, "scale", (torch.float32,), numel=M)
+    _on_device(x=x, residual=residual, weight=weight, out=out, scale=scale, residual_out=residual_out)
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty_like(residual)
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_types[0], device=x.device)
+    if out.dtype == torch.int8 and scale is None:
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call(x, lib().jules_hip_add_rmsnorm, _DT[x.dtype], F32 if residual is None else _DT[residual.dtype],
+          I8 if out.dtype == torch.int8 else _DT[out.dtype], _ptr(x), _ptr(residual), _ptr(weight), _ptr(residual_out),
+          _ptr(out), _ptr(scale), M, N, float(eps))
+    return out, scale, residual_out
+
+
+def add_rmsnorm(x, residual, weight, eps=1e-5, out=None, residual_out=None):
+    """h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight over the last
+    dimension (jules_hip_add_rmsnorm; no counterpart in the reference).  x and
+    residual fp32 or bf16, each by itself, residual or None; weight fp32.
+    Returns (y, h): y of x's dtype (or of out's, fp32 or bf16), h of the
+    residual's dtype, None without one.  residual_out may be residual."""
+    y, _, h = _add_rmsnorm(x, residual, weight, eps, out, (x.dtype, *_REAL) if isinstance(x, torch.Tensor) else _REAL,
+                           None, residual_out)
+    return y, h
+
+
+def add_rmsnorm_int8(x, residual, weight, eps=1e-5, out=None, scale=None, residual_out=None):
+    """add_rmsnorm with int8 rows and a scale for each: returns (q, scale, h)
+    with y = q * scale to half a step, q and scale being the A and scale_a of
+    matmul_w8a8."""
+    return _add_rmsnorm(x, residual, weight, eps, out, (torch.int8,), scale, residual_out)
+
+
+def rotary_frequencies(rotary_dim, sections=None, base=10000.0, device="cuda"):
+    """(inv_freq fp64 [rotary_dim/2], pair_axis int32 or None) of rotary:
+    inv_freq[p] = base^(-2p / rotary_dim).  sections: numbers of pairs of each
+    axis, in order (they sum to rotary_dim/2); None for a single axis."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} must be even and at least 2")
+    pairs = rotary_dim // 2
+    p = torch.arange(pairs, dtype=torch.float64)
+    inv_freq = torch.pow(torch.tensor(float(base), dtype=torch.float64), -p / pairs).to(device)
+    if sections is None:
+        return inv_freq, None
+    if any(n < 0 for n in sections) or sum(sections) != pairs:
+        raise ValueError(f"sections {tuple(sections)} must sum to {pairs}")
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(list(sections)))
+    return inv_freq, axis.to(torch.int32).to(device)
+
+
+_PAIRING = {"half": 0, "adjacent": 1}
+
+
+def _strides3(t, rank):
+    # batch, head, token of [B,H,S,D]; [H,S,D] is one batch
+    return t.stride()[:3] if rank == 4 else (0, t.stride(0), t.stride(1))
+
+
+def rotary(x, positions, inv_freq, pair_axis=None, pairing="half", inverse=False, dtype=None, out=None):
+    """Rotary positions of one or several axes (jules_hip_rotary; no counterpart
+    in the reference) on x [B,H,S,D] or [H,S,D], fp32 or bf16, of any strides
+    whose last is 1 (a transposed [tokens, heads, D], heads of a fused
+    projection).  positions int32 [axes, B, S], [axes, S] for [H,S,D]; a single
+    axis may be left out.  inv_freq fp64 [R/2], pair_axis int32 [R/2] or None:
+    rotary_frequencies.  pairing "half": elements p and p + R/2, "adjacent": 2p
+    and 2p + 1.  inverse: the other way, which takes the gradient of the output
+    to that of x.  out: of x's shape, any such strides (x itself: in place); if
+    None, dense of `dtype` (x's)."""
+    if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
+        raise ValueError("x must be a tensor of 3 or 4 dimensions")
+    rank = x.dim()
+    for t, n in ((x, "x"), (out, "out")):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
+            raise ValueError(f"{n}: fp32 or bf16 tensor expected")
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{n}: the last stride must be 1")
+    B, H, S, D = x.shape if rank == 4 else (1, *x.shape)
+    where = (B, S) if rank == 4 else (S,)
+    if not isinstance(positions, torch.Tensor) or positions.dim() not in (len(where), len(where) + 1):
+        raise ValueError("positions must be a tensor [axes, *tokens] or [*tokens]")
+    axes = 1 if positions.dim() == len(where) else positions.shape[0]
+    _need(positions, "positions", (torch.int32,), numel=axes * B * S)
+    if tuple(positions.shape[-len(where):]) != where:
+        raise ValueError(f"positions: shape {tuple(positions.shape)}, expected [axes, *{where}]")
+    _need(inv_freq, "inv_freq", (torch.float64,))
+    R = 2 * inv_freq.numel()
+    if R < 2 or R > D:
+        raise ValueError(f"inv_freq: {R // 2} pairs for {D} elements")
+    if pair_axis is not None:
+        _need(pair_axis, "pair_axis", (torch.int32,), numel=R // 2)
+    if pairing not in _PAIRING:
+        raise ValueError(f"pairing {pairing!r} not in {tuple(_PAIRING)}")
+    if out is not None:
+        if out.shape != x.shape:
+            raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(x.shape)}")
+        if dtype is not None and out.dtype != dtype:
+            raise ValueError(f"out: dtype {out.dtype}, expected {dtype}")
+    elif dtype is not None and dtype not in _DT:
+        raise ValueError(f"dtype {dtype} not in {tuple(_DT)}")
+    _on_device(x=x, positions=positions, inv_freq=inv_freq, pair_axis=pair_axis, out=out)
+    if out is None:
+        out = torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
+    i64x3 = ctypes.c_int64 * 3
+    _call(x, lib().jules_hip_rotary, _DT[x.dtype], _DT[out.dtype], _PAIRING[pairing], int(bool(inverse)), _ptr(x),
+          i64x3(*_strides3(x, rank)), _ptr(out), i64x3(*_strides3(out, rank)), _ptr(positions), _ptr(inv_freq),
+          _ptr(pair_axis), axes, B, H, S, D, R)
+    return out
+
+
+class KV4Cache:
+    """A paged key/value cache held in 4 bits (jh_kv4_cache; layout in
+    include/jules_hip.h): k uint8 [pages, heads, page_size, D/2], v uint8
+    [pages, heads, page_size/4, 2*D], k_meta and v_meta bf16 [pages, heads,
+    page_size, 2] with each row's scale and minimum."""
+
+    def __init__(self, k, v, k_meta, v_meta):
+        _rank(k, "k", 4)
+        _need(k, "k", (torch.uint8,))
+        pages, heads, page_size, half = k.shape
+        _need(v, "v", (torch.uint8,), shape=(pages, heads, page_size // 4, 4 * half))
+        for t, n in ((k_meta, "k_meta"), (v_meta, "v_meta")):
+            _need(t, n, (torch.bfloat16,), shape=(pages, heads, page_size, 2))
+        self.k, self.v, self.k_meta, self.v_meta = k, v, k_meta, v_meta
+        self.pages, self.heads, self.page_size, self.head_dim = pages, heads, page_size, 2 * half
+        self._c = JhKV4Cache(_ptr(k), _ptr(v), _ptr(k_meta), _ptr(v_meta), pages, page_size, heads, 2 * half)
+
+    @classmethod
+    def empty(cls, pages, heads, head_dim, page_size=64, device="cuda"):
+        """A pool of `pages` pages; what they hold is not set."""
+        return cls(torch.empty(pages, heads, page_size, head_dim // 2, dtype=torch.uint8, device=device),
+                   torch.empty(pages, heads, page_size // 4, 2 * head_dim, dtype=torch.uint8, device=device),
+                   *(torch.empty(pages, heads, page_size, 2, dtype=torch.bfloat16, device=device) for _ in "kv"))
+
+    def _ref(self):
+        return ctypes.byref(self._c)
+
+
+def _kv4_batch(cache, table, lens, cu_q, max_q, tokens):
+    """Checks of what the calls on a KV4Cache share; returns (batch, max_q)."""
+    if not isinstance(cache, KV4Cache):
+        raise TypeError("cache must be a KV4Cache")
+    _rank(table, "table", 2)
+    _need(table, "table", (torch.int32,))
+    batch = table.shape[0]
+    _need(lens, "lens", (torch.int32,), numel=batch)
+    if cu_q is None:
+        each = tokens // batch if batch else 0
+        if each * batch != tokens or max_q not in (None, each):
+            raise ValueError(f"{tokens} tokens for {batch} sequences, max_q {max_q}: unequal numbers need cu_q")
+        return batch, each
+    _need(cu_q, "cu_q", (torch.int32,), numel=batch + 1)
+    return batch, tokens if max_q is None else int(max_q)
+
+
+def _kv4_rows(t, name, dtypes, tail):
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise ValueError(f"{name} must have 3 dimensions")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: dtype {t.dtype} not in {dtypes}")
+    if t.shape[1:] != tail:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [tokens, {tail[0]}, {tail[1]}]")
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last stride must be 1")
+
+
+def kv4_append(cache, k, v, table, lens, cu_q=None, max_q=None):
+    """Writes new rows into the cache (jules_hip_kv4_append; no counterpart in
+    the reference): k, v [tokens, heads, D], fp32 or bf16, of any strides whose
+    last is 1.  table int32 [batch, max_pages]: the pages of each sequence;
+    lens int32 [batch]: tokens of each, the new ones among them; rows cu_q[b]
+    .. cu_q[b+1] - 1 are the last ones of sequence b (None: the same number
+    each).  max_q: the largest number of new rows, where the caller knows it."""
+    tail = (cache.heads, cache.head_dim) if isinstance(cache, KV4Cache) else (0, 0)
+    if tail != (0, 0):
+        _kv4_rows(k, "k", _REAL, tail)
+        _kv4_rows(v, "v", (k.dtype,), tail)
+        if v.shape != k.shape:
+            raise ValueError(f"v: shape {tuple(v.shape)}, expected {tuple(k.shape)}")
+    tokens = k.shape[0]
+    batch, max_q = _kv4_batch(cache, table, lens, cu_q, max_q, tokens)
+    _on_device(k=k, v=v, cache=cache.k, v_cache=cache.v, k_meta=cache.k_meta, v_meta=cache.v_meta, table=table,
+               lens=lens, cu_q=cu_q)
+    _call(k, lib().jules_hip_kv4_append, _DT[k.dtype], cache._ref(), _ptr(k), k.stride(0), k.stride(1), _ptr(v),
+          v.stride(0), v.stride(1), _ptr(table), table.shape[1], _ptr(lens), _ptr(cu_q), batch, tokens, max_q)
+
+
+def kv4_read(cache, table, lens, tokens, cu_q=None, max_q=None, dtype=torch.bfloat16, k=None, v=None):
+    """The rows that kv4_append with the same arguments writes, as values
+    (jules_hip_kv4_read): (k, v) [tokens, heads, D] of dtype.  With lens and
+    cu_q of whole sequences it lays a cache out for flash_attention."""
+    batch, max_q = _kv4_batch(cache, table, lens, cu_q, max_q, tokens)
+    shape = (tokens, cache.heads, cache.head_dim)
+    if dtype not in _DT:
+        raise ValueError(f"dtype {dtype} not in {tuple(_DT)}")
+    for t, n in ((k, "k"), (v, "v")):
+        if t is not None:
+            _need(t, n, (dtype,), shape=shape)
+    _on_device(cache=cache.k, v_cache=cache.v, k_meta=cache.k_meta, v_meta=cache.v_meta, table=table, lens=lens,
+               cu_q=cu_q, k=k, v=v)
+    k = torch.empty(shape, dtype=dtype, device=lens.device) if k is None else k
+    v = torch.empty(shape, dtype=dtype, device=lens.device) if v is None else v
+    _call(lens, lib().jules_hip_kv4_read, _DT[dtype], cache._ref(), _ptr(k), _ptr(v), _ptr(table), table.shape[1],
+          _ptr(lens), _ptr(cu_q), batch, tokens, max_q)
+    return k, v
+
+
+def kv4_attention(q, cache, table, lens, cu_q=None, max_q=None, max_len=None, scale=None, out=None, lse=None,
+                  return_lse=False, workspace=None):
+    """Attention of new tokens over the cache (jules_hip_kv4_attention; no
+    counterpart in the reference): q bf16 [tokens, heads_q, D], heads_q a
+    multiple of the cache's heads, each token over its sequence's keys up to
+    its own position; table, lens, cu_q and max_q as in kv4_append, which comes
+    before.  max_len: the largest of lens, where the caller knows it (None: what
+    the table has room for).  scale defaults to 1/sqrtf(D).  Returns out
+    [tokens, heads_q, D], or (out, lse [tokens, heads_q]) with return_lse."""
+    if isinstance(cache, KV4Cache):
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+            raise ValueError("q must have 3 dimensions")
+        if q.shape[1] < 1 or q.shape[1] % cache.heads:
+            raise ValueError(f"q: {q.shape[1]} heads, the cache has {cache.heads}")
+        _kv4_rows(q, "q", (torch.bfloat16,), (q.shape[1], cache.head_dim))
+    tokens, heads_q = q.shape[:2]
+    batch, max_q = _kv4_batch(cache, table, lens, cu_q, max_q, tokens)
+    if out is not None:
+        _need(out, "out", (torch.bfloat16,), shape=q.shape)
+    if lse is not None:
+        _need(lse, "lse", (torch.float32,), numel=tokens * heads_q)
+    ws_bytes = 0 if workspace is None else _workspace(workspace, "workspace")
+    _on_device(q=q, cache=cache.k, v_cache=cache.v, k_meta=cache.k_meta, v_meta=cache.v_meta, table=table, lens=lens,
+               cu_q=cu_q, out=out, lse=lse, workspace=workspace)
+    if max_len is None:
+        max_len = min(table.shape[1] * cache.page_size, 2**31 - 1)
+    if scale is None:
+        scale = default_scale(cache.head_dim)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if lse is None and return_lse:
+        lse = torch.empty((tokens, heads_q), dtype=torch.float32, device=q.device)
+    if workspace is None:
+        ws_bytes = lib().jules_hip_kv4_attention_workspace_size(batch, tokens, heads_q, cache.heads, cache.head_dim,
+                                                                max_q, max_len)
+        if ws_bytes:
+            workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
+    _call(q, lib().jules_hip_kv4_attention, float(scale), cache._ref(), _ptr(q), q.stride(0), q.stride(1), _ptr(out),
+          _ptr(lse), heads_q, _ptr(table), table.shape[1], _ptr(lens), _ptr(cu_q), batch, tokens, max_q, int(max_len),
+          _ptr(workspace), ws_bytes)
+    return (out, lse) if return_lse else out
 
 
 def cross_entropy_workspace(M, device):
