@@ -415,7 +415,8 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  * 65535; num_pages >= 1.
  *
  * A batch's new tokens, the same four arguments in the three calls:
- *   table   int32 [batch, max_pages]: the pages of each sequence in order
+ *   table   int32 [batch, max_pages], max_pages >= 1: the pages of each sequence in
+ *           order
  *   lens    int32 [batch]: tokens of each sequence, the new ones among them
  *   cu_q    int32 [batch + 1] or NULL: rows cu_q[b] .. cu_q[b+1] - 1 of the packed
  *           arrays belong to sequence b, ascending, and are its last ones; rows

@@ -561,7 +561,8 @@ static int kv4_check(const char* who, const jh_kv4_cache* c, const int32_t* tabl
         *done = true;
         return JH_OK;
     }
-    if (!lens || (!table && max_pages > 0)) return fail(JH_ERR_NULL, "%s: null table or lens", who);
+    if (max_pages < 1) return fail(JH_ERR_SHAPE, "%s: a table of %d pages a sequence", who, max_pages);
+    if (!lens || !table) return fail(JH_ERR_NULL, "%s: null table or lens", who);
     if (!c->k || !c->v || !c->k_meta || !c->v_meta)
         return fail(JH_ERR_NULL, "%s: null cache array", who);
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_meta, 16) || !aligned(c->v_meta, 16))

@@ -22,6 +22,12 @@
 
 namespace jh {
 
+// One number of a call's table, lens or cu_q, the same address in all lanes, by a
+// scalar load: it takes no place among the vector loads in flight.
+__device__ __forceinline__ int kv4_scalar(const int32_t* p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
+}
+
 // row index of token `off` of a page and head
 __device__ __forceinline__ int64_t kv4_row(const KV4View& c, int page, int head, int off) {
     return ((int64_t)page * c.heads + head) * c.page_size + off;
@@ -30,18 +36,18 @@ __device__ __forceinline__ int64_t kv4_row(const KV4View& c, int page, int head,
 // first packed row of sequence `seq`, and how many are its; never past the
 // arrays, whatever cu_q holds
 __device__ __forceinline__ int kv4_first(const KV4Batch& b, int seq) {
-    return b.cu_q ? min(max(b.cu_q[seq], 0), b.tokens) : seq * b.max_q;
+    return b.cu_q ? min(max(kv4_scalar(b.cu_q + seq), 0), b.tokens) : seq * b.max_q;
 }
 __device__ __forceinline__ int kv4_count(const KV4Batch& b, int seq) {
     if (!b.cu_q) return b.max_q;
-    return max(0, min(max(b.cu_q[seq + 1], 0), b.tokens) - kv4_first(b, seq));
+    return max(0, min(max(kv4_scalar(b.cu_q + seq + 1), 0), b.tokens) - kv4_first(b, seq));
 }
 
-// the page that holds position `at` of a sequence, or -1 where its row of the
-// table has none of the pool's
+// the page that holds position `at` >= 0 of a sequence, or -1 where its row of
+// the table has none of the pool's
 __device__ __forceinline__ int kv4_page(const KV4View& c, const KV4Batch& b, int seq, int at) {
     const int i = at >> c.page_shift;
-    if (at < 0 || i >= b.max_pages) return -1;
+    if (i >= b.max_pages) return -1;
     const int p = b.table[(int64_t)seq * b.max_pages + i];
     return p >= 0 && p < c.num_pages ? p : -1;
 }

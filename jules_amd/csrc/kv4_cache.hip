@@ -78,7 +78,7 @@ __global__ __launch_bounds__(THREADS) void kv4_append_kernel(KV4View c, KV4Batch
     constexpr int LANES = D / 8, TOKENS = THREADS / LANES;
     const int h = blockIdx.y, lane = threadIdx.x % LANES;
     for (int seq = blockIdx.z; seq < b.batch; seq += gridDim.z) {
-        const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = b.lens[seq];
+        const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
         for (int64_t i0 = (int64_t)blockIdx.x * TOKENS; i0 < n; i0 += (int64_t)gridDim.x * TOKENS) {
             const int i = (int)i0 + (int)threadIdx.x / LANES;
             if (i >= n) continue;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(THREADS) void kv4_read_kernel(KV4View c, KV4Batch b
     constexpr int LANES = D / 8, TOKENS = THREADS / LANES;
     const int h = blockIdx.y, lane = threadIdx.x % LANES;
     for (int seq = blockIdx.z; seq < b.batch; seq += gridDim.z) {
-        const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = b.lens[seq];
+        const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
         for (int64_t i0 = (int64_t)blockIdx.x * TOKENS; i0 < n; i0 += (int64_t)gridDim.x * TOKENS) {
             const int i = (int)i0 + (int)threadIdx.x / LANES;
             if (i >= n) continue;
