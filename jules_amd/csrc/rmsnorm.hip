@@ -58,20 +58,23 @@ __device__ __forceinline__ void store8(uint16_t* p, const f32x8_t& r) {
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(uint16_t* p, float v) { *p = (uint16_t)pack_bf16x2(v, 0.0f); }
 
-// sum and largest of the group's values, the same order for every row
+// sum and largest of the group's values, the same order for every row.  The waves'
+// parts alternate between two places, so that one barrier a row is enough: a wave
+// that writes a place again has passed the barrier after which it was read.
 struct RowStats {
     double sum;
     float top;
 };
 template <int G>
-__device__ __forceinline__ RowStats reduce_row(RowStats a) {
+__device__ __forceinline__ RowStats reduce_row(RowStats a, int turn) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         a.sum += __shfl_xor(a.sum, o);
         a.top = fmaxf(a.top, __shfl_xor(a.top, o));
     }
     if constexpr (G > 64) {
-        __shared__ RowStats part[G / 64];
+        __shared__ RowStats parts[2][G / 64];
+        RowStats* part = parts[turn & 1];
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
         __syncthreads();
         a = part[0];
@@ -206,14 +209,26 @@ __device__ __forceinline__ void count(RowStats* s, const f32x8_t& h, const f32x8
     }
 }
 
-// G threads a row, NP pieces of 8 neighbouring elements a thread; a block
-// holds 256 / G rows, or one row of more threads
+// G threads a row, NP pieces of 8 neighbouring elements a thread; a block holds
+// 256 / G rows, or one row of more threads, and goes on to others with the weight
+// in its registers
 template <typename XT, typename RT, bool RES, int G, int NP>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void add_rmsnorm_kernel(NormArgs a) {
     constexpr int ROWS = G < 256 ? 256 / G : 1;
     const int tid = G < 256 ? threadIdx.x % G : threadIdx.x;
+    constexpr bool KEEP = G * NP < 4096;  // 1024 threads with 4 pieces have no registers for it
+    f32x8_t w[KEEP ? NP : 1];
+    const auto weight = [&](int t) {
+        const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+        return n > 0 ? read_weight(a.w, j, n) : f32x8_t{};
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int t = 0; t < NP; ++t) w[t] = weight(t);
+    }
+    int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + (G < 256 ? threadIdx.x / G : 0); row < a.M;
-         row += (int64_t)gridDim.x * ROWS) {
+         row += (int64_t)gridDim.x * ROWS, ++turn) {
         const int64_t at = row * a.N;
         f32x8_t h[NP];
         RowStats s{0.0, 0.0f};
@@ -223,19 +238,16 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_rmsnorm_kernel(NormArgs
             if (n > 0) h[t] = read_piece<XT, RT, RES>(a, at + j, n);
         }
 #pragma unroll
-        for (int t = 0; t < NP; ++t) {
-            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n > 0) count(&s, h[t], read_weight(a.w, j, n));
-        }
-        s = reduce_row<G>(s);
+        for (int t = 0; t < NP; ++t)
+            if (8 * (tid + G * t) < a.N) count(&s, h[t], KEEP ? w[KEEP ? t : 0] : weight(t));
+        s = reduce_row<G>(s, turn);
         const RowFactors f = row_factors(s, a.N, a.eps);
         if (a.out_dtype == JH_I8 && tid == 0) a.scale[row] = f.scale;
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
             const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n > 0) write_piece<RT, RES>(a, f, at + j, h[t], read_weight(a.w, j, n), n);
+            if (n > 0) write_piece<RT, RES>(a, f, at + j, h[t], KEEP ? w[KEEP ? t : 0] : weight(t), n);
         }
-        if constexpr (G > 64) __syncthreads();  // the row's numbers are read before the next row's are written
     }
 }
 
@@ -243,14 +255,15 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_rmsnorm_kernel(NormArgs
 // written by the same thread, so r' may be r or x here too.
 template <typename XT, typename RT, bool RES>
 __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs a) {
-    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x, ++turn) {
         const int64_t at = row * a.N;
         RowStats s{0.0, 0.0f};
         for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) {
             const int n = (int)min((int64_t)8, a.N - j);
             count(&s, read_piece<XT, RT, RES>(a, at + j, n), read_weight(a.w, (int)j, n));
         }
-        s = reduce_row<1024>(s);
+        s = reduce_row<1024>(s, turn);
         const RowFactors f = row_factors(s, a.N, a.eps);
         if (a.out_dtype == JH_I8 && threadIdx.x == 0) a.scale[row] = f.scale;
         for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) {
@@ -258,24 +271,40 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_long_kernel(NormArgs a) {
             const f32x8_t h = read_piece<XT, RT, RES>(a, at + j, n);
             write_piece<RT, RES>(a, f, at + j, h, read_weight(a.w, (int)j, n), n);
         }
-        __syncthreads();
     }
 }
 
+template <typename XT, typename RT, bool RES, int G, int NP>
+void launch(const NormArgs& a, int blocks, hipStream_t s) {
+    constexpr int ROWS = G < 256 ? 256 / G : 1;
+    const int64_t rows = ((int64_t)a.M + ROWS - 1) / ROWS;
+    add_rmsnorm_kernel<XT, RT, RES, G, NP><<<(unsigned)std::min((int64_t)blocks, rows), G < 256 ? 256 : G, 0, s>>>(a);
+}
+
+// Few threads with many elements each keep the most rows in flight: 8192 rows of
+// 8192 bf16 take 90 us (5.2 TB/s) with 256 threads of 32 elements, 165 us with
+// 1024 of 8, of which a CU holds one row at a time.  Up to two rows a CU 1024
+// threads are the faster, a row being done sooner (8 rows: 5.6 us).  Four blocks a
+// CU, as many as are resident, read the weight once each; a block a row: 98 us.
+// Rows of odd width, at 4-byte addresses: 4.1 TB/s (1999 of 5001 fp32, 39 us).
 template <typename XT, typename RT, bool RES>
 hipError_t launch(const NormArgs& a, hipStream_t s) {
-    const int64_t wide = (int64_t)1 << 21;  // blocks: below 2^32 threads at 1024 a block
-    const auto grid = [&](int rows) { return (unsigned)std::min(wide, ((int64_t)a.M + rows - 1) / rows); };
     if (a.N <= 512)
-        add_rmsnorm_kernel<XT, RT, RES, 64, 1><<<grid(4), 256, 0, s>>>(a);
+        launch<XT, RT, RES, 64, 1>(a, 8192, s);
     else if (a.N <= 2048)
-        add_rmsnorm_kernel<XT, RT, RES, 256, 1><<<grid(1), 256, 0, s>>>(a);
+        launch<XT, RT, RES, 256, 1>(a, 2048, s);
+    else if (a.M <= 512 && a.N <= 8192)
+        launch<XT, RT, RES, 1024, 1>(a, 512, s);
+    else if (a.N <= 4096)
+        launch<XT, RT, RES, 256, 2>(a, 1024, s);
     else if (a.N <= 8192)
-        add_rmsnorm_kernel<XT, RT, RES, 1024, 1><<<grid(1), 1024, 0, s>>>(a);
+        launch<XT, RT, RES, 256, 4>(a, 1024, s);
+    else if (a.N <= 16384)
+        launch<XT, RT, RES, 512, 4>(a, 512, s);
     else if (a.N <= 32768)
-        add_rmsnorm_kernel<XT, RT, RES, 1024, 4><<<grid(1), 1024, 0, s>>>(a);
+        launch<XT, RT, RES, 1024, 4>(a, 512, s);
     else
-        add_rmsnorm_long_kernel<XT, RT, RES><<<grid(1), 1024, 0, s>>>(a);
+        add_rmsnorm_long_kernel<XT, RT, RES><<<(unsigned)std::min(a.M, 2048), 1024, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -336,6 +336,19 @@ def layernorm(x, gamma, beta, eps=1e-5, out=None):
     return out
 
 
+def _one_device(names, *tensors):
+    """_on_device without a dictionary where all is well: for calls short enough
+    that its cost shows."""
+    index = tensors[0].get_device()
+    if index >= 0:
+        for t in tensors:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return
+    _on_device(**dict(zip(names, tensors)))
+
+
 def _call(t, fn, *args):
     """check(fn(*args, stream)) on t's device and torch's current stream there,
     whichever device is the current one."""
@@ -361,16 +374,17 @@ def _add_rmsnorm(x, residual, weight, eps, out, out_types, scale, residual_out):
         _need(out, "out", out_types, shape=x.shape)
     if scale is not None:
         _need(scale, "scale", (torch.float32,), numel=M)
-    _on_device(x=x, residual=residual, weight=weight, out=out, scale=scale, residual_out=residual_out)
+    _one_device(("x", "weight", "residual", "out", "scale", "residual_out"), x, weight, residual, out, scale, residual_out)
     if residual is not None and residual_out is None:
         residual_out = torch.empty_like(residual)
     if out is None:
-        out = torch.empty(x.shape, dtype=out_types[0], device=x.device)
-    if out.dtype == torch.int8 and scale is None:
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        out = torch.empty_like(x, dtype=out_types[0])
+    int8 = out.dtype == torch.int8
+    if int8 and scale is None:
+        scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _call(x, lib().jules_hip_add_rmsnorm, _DT[x.dtype], F32 if residual is None else _DT[residual.dtype],
-          I8 if out.dtype == torch.int8 else _DT[out.dtype], _ptr(x), _ptr(residual), _ptr(weight), _ptr(residual_out),
-          _ptr(out), _ptr(scale), M, N, float(eps))
+          I8 if int8 else _DT[out.dtype], x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(residual_out),
+          out.data_ptr(), _ptr(scale), M, N, float(eps))
     return out, scale, residual_out
 
 
@@ -412,9 +426,17 @@ def rotary_frequencies(rotary_dim, sections=None, base=10000.0, device="cuda"):
 _PAIRING = {"half": 0, "adjacent": 1}
 
 
-def _strides3(t, rank):
-    # batch, head, token of [B,H,S,D]; [H,S,D] is one batch
-    return t.stride()[:3] if rank == 4 else (0, t.stride(0), t.stride(1))
+_I64x3 = ctypes.c_int64 * 3
+
+
+def _rotary_strides(t, name):
+    """Strides of batch, head and token of [B,H,S,D], or of [H,S,D], which is one batch."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
+        raise ValueError(f"{name}: fp32 or bf16 tensor expected")
+    *outer, last = t.stride()
+    if last != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the last stride must be 1")
+    return _I64x3(*outer) if len(outer) == 3 else _I64x3(0, *outer)
 
 
 def rotary(x, positions, inv_freq, pair_axis=None, pairing="half", inverse=False, dtype=None, out=None):
@@ -429,21 +451,14 @@ def rotary(x, positions, inv_freq, pair_axis=None, pairing="half", inverse=False
     None, dense of `dtype` (x's)."""
     if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
         raise ValueError("x must be a tensor of 3 or 4 dimensions")
-    rank = x.dim()
-    for t, n in ((x, "x"), (out, "out")):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
-            raise ValueError(f"{n}: fp32 or bf16 tensor expected")
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            raise ValueError(f"{n}: the last stride must be 1")
-    B, H, S, D = x.shape if rank == 4 else (1, *x.shape)
-    where = (B, S) if rank == 4 else (S,)
+    strides = _rotary_strides(x, "x")
+    B, H, S, D = x.shape if x.dim() == 4 else (1, *x.shape)
+    where = (S,) if x.dim() == 3 else (B, S)
     if not isinstance(positions, torch.Tensor) or positions.dim() not in (len(where), len(where) + 1):
         raise ValueError("positions must be a tensor [axes, *tokens] or [*tokens]")
     axes = 1 if positions.dim() == len(where) else positions.shape[0]
     _need(positions, "positions", (torch.int32,), numel=axes * B * S)
-    if tuple(positions.shape[-len(where):]) != where:
+    if positions.shape[-len(where):] != where:
         raise ValueError(f"positions: shape {tuple(positions.shape)}, expected [axes, *{where}]")
     _need(inv_freq, "inv_freq", (torch.float64,))
     R = 2 * inv_freq.numel()
@@ -453,20 +468,23 @@ def rotary(x, positions, inv_freq, pair_axis=None, pairing="half", inverse=False
         _need(pair_axis, "pair_axis", (torch.int32,), numel=R // 2)
     if pairing not in _PAIRING:
         raise ValueError(f"pairing {pairing!r} not in {tuple(_PAIRING)}")
+    if dtype is None:
+        dtype = x.dtype if out is None else out.dtype
+    elif dtype not in _DT:
+        raise ValueError(f"dtype {dtype} not in {tuple(_DT)}")
     if out is not None:
+        out_strides = _rotary_strides(out, "out")
         if out.shape != x.shape:
             raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(x.shape)}")
-        if dtype is not None and out.dtype != dtype:
+        if out.dtype != dtype:
             raise ValueError(f"out: dtype {out.dtype}, expected {dtype}")
-    elif dtype is not None and dtype not in _DT:
-        raise ValueError(f"dtype {dtype} not in {tuple(_DT)}")
-    _on_device(x=x, positions=positions, inv_freq=inv_freq, pair_axis=pair_axis, out=out)
+    _one_device(("x", "positions", "inv_freq", "pair_axis", "out"), x, positions, inv_freq, pair_axis, out)
     if out is None:
-        out = torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
-    i64x3 = ctypes.c_int64 * 3
-    _call(x, lib().jules_hip_rotary, _DT[x.dtype], _DT[out.dtype], _PAIRING[pairing], int(bool(inverse)), _ptr(x),
-          i64x3(*_strides3(x, rank)), _ptr(out), i64x3(*_strides3(out, rank)), _ptr(positions), _ptr(inv_freq),
-          _ptr(pair_axis), axes, B, H, S, D, R)
+        out = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+        out_strides = _I64x3(H * S * D, S * D, D)
+    _call(x, lib().jules_hip_rotary, _DT[x.dtype], _DT[dtype], _PAIRING[pairing], int(bool(inverse)), x.data_ptr(),
+          strides, out.data_ptr(), out_strides, positions.data_ptr(), inv_freq.data_ptr(), _ptr(pair_axis), axes, B, H, S,
+          D, R)
     return out
 
 
@@ -481,11 +499,13 @@ class KV4Cache:
         _need(k, "k", (torch.uint8,))
         pages, heads, page_size, half = k.shape
         _need(v, "v", (torch.uint8,), shape=(pages, heads, page_size // 4, 4 * half))
-        for t, n in ((k_meta, "k_meta"), (v_meta, "v_meta")):
-            _need(t, n, (torch.bfloat16,), shape=(pages, heads, page_size, 2))
+        meta = (pages, heads, page_size, 2)
+        _need(k_meta, "k_meta", (torch.bfloat16,), shape=meta)
+        _need(v_meta, "v_meta", (torch.bfloat16,), shape=meta)
         self.k, self.v, self.k_meta, self.v_meta = k, v, k_meta, v_meta
         self.pages, self.heads, self.page_size, self.head_dim = pages, heads, page_size, 2 * half
-        self._c = JhKV4Cache(_ptr(k), _ptr(v), _ptr(k_meta), _ptr(v_meta), pages, page_size, heads, 2 * half)
+        c = JhKV4Cache(k.data_ptr(), v.data_ptr(), k_meta.data_ptr(), v_meta.data_ptr(), pages, page_size, heads, 2 * half)
+        self._ref = ctypes.byref(c)  # keeps c
 
     @classmethod
     def empty(cls, pages, heads, head_dim, page_size=64, device="cuda"):
@@ -494,8 +514,8 @@ class KV4Cache:
                    torch.empty(pages, heads, page_size // 4, 2 * head_dim, dtype=torch.uint8, device=device),
                    *(torch.empty(pages, heads, page_size, 2, dtype=torch.bfloat16, device=device) for _ in "kv"))
 
-    def _ref(self):
-        return ctypes.byref(self._c)
+
+_KV4_SCALE = {D: default_scale(D) for D in (64, 128)}
 
 
 def _kv4_batch(cache, table, lens, cu_q, max_q, tokens):
@@ -541,10 +561,12 @@ def kv4_append(cache, k, v, table, lens, cu_q=None, max_q=None):
             raise ValueError(f"v: shape {tuple(v.shape)}, expected {tuple(k.shape)}")
     tokens = k.shape[0]
     batch, max_q = _kv4_batch(cache, table, lens, cu_q, max_q, tokens)
-    _on_device(k=k, v=v, cache=cache.k, v_cache=cache.v, k_meta=cache.k_meta, v_meta=cache.v_meta, table=table,
-               lens=lens, cu_q=cu_q)
-    _call(k, lib().jules_hip_kv4_append, _DT[k.dtype], cache._ref(), _ptr(k), k.stride(0), k.stride(1), _ptr(v),
-          v.stride(0), v.stride(1), _ptr(table), table.shape[1], _ptr(lens), _ptr(cu_q), batch, tokens, max_q)
+    _one_device(("k", "v", "cache.k", "cache.v", "cache.k_meta", "cache.v_meta", "table", "lens", "cu_q"), k, v, cache.k,
+                cache.v, cache.k_meta, cache.v_meta, table, lens, cu_q)
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    _call(k, lib().jules_hip_kv4_append, _DT[k.dtype], cache._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+          table.data_ptr(), table.shape[1], lens.data_ptr(), _ptr(cu_q), batch, tokens, max_q)
 
 
 def kv4_read(cache, table, lens, tokens, cu_q=None, max_q=None, dtype=torch.bfloat16, k=None, v=None):
@@ -558,12 +580,12 @@ def kv4_read(cache, table, lens, tokens, cu_q=None, max_q=None, dtype=torch.bflo
     for t, n in ((k, "k"), (v, "v")):
         if t is not None:
             _need(t, n, (dtype,), shape=shape)
-    _on_device(cache=cache.k, v_cache=cache.v, k_meta=cache.k_meta, v_meta=cache.v_meta, table=table, lens=lens,
-               cu_q=cu_q, k=k, v=v)
-    k = torch.empty(shape, dtype=dtype, device=lens.device) if k is None else k
-    v = torch.empty(shape, dtype=dtype, device=lens.device) if v is None else v
-    _call(lens, lib().jules_hip_kv4_read, _DT[dtype], cache._ref(), _ptr(k), _ptr(v), _ptr(table), table.shape[1],
-          _ptr(lens), _ptr(cu_q), batch, tokens, max_q)
+    _one_device(("lens", "table", "cache.k", "cache.v", "cache.k_meta", "cache.v_meta", "cu_q", "k", "v"), lens, table,
+                cache.k, cache.v, cache.k_meta, cache.v_meta, cu_q, k, v)
+    k = lens.new_empty(shape, dtype=dtype) if k is None else k
+    v = lens.new_empty(shape, dtype=dtype) if v is None else v
+    _call(lens, lib().jules_hip_kv4_read, _DT[dtype], cache._ref, k.data_ptr(), v.data_ptr(), table.data_ptr(),
+          table.shape[1], lens.data_ptr(), _ptr(cu_q), batch, tokens, max_q)
     return k, v
 
 
@@ -589,23 +611,24 @@ def kv4_attention(q, cache, table, lens, cu_q=None, max_q=None, max_len=None, sc
     if lse is not None:
         _need(lse, "lse", (torch.float32,), numel=tokens * heads_q)
     ws_bytes = 0 if workspace is None else _workspace(workspace, "workspace")
-    _on_device(q=q, cache=cache.k, v_cache=cache.v, k_meta=cache.k_meta, v_meta=cache.v_meta, table=table, lens=lens,
-               cu_q=cu_q, out=out, lse=lse, workspace=workspace)
+    _one_device(("q", "cache.k", "cache.v", "cache.k_meta", "cache.v_meta", "table", "lens", "cu_q", "out", "lse",
+                 "workspace"), q, cache.k, cache.v, cache.k_meta, cache.v_meta, table, lens, cu_q, out, lse, workspace)
     if max_len is None:
         max_len = min(table.shape[1] * cache.page_size, 2**31 - 1)
     if scale is None:
-        scale = default_scale(cache.head_dim)
+        scale = _KV4_SCALE[cache.head_dim] if cache.head_dim in _KV4_SCALE else default_scale(cache.head_dim)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if lse is None and return_lse:
-        lse = torch.empty((tokens, heads_q), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((tokens, heads_q), dtype=torch.float32)
     if workspace is None:
         ws_bytes = lib().jules_hip_kv4_attention_workspace_size(batch, tokens, heads_q, cache.heads, cache.head_dim,
                                                                 max_q, max_len)
         if ws_bytes:
-            workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
-    _call(q, lib().jules_hip_kv4_attention, float(scale), cache._ref(), _ptr(q), q.stride(0), q.stride(1), _ptr(out),
-          _ptr(lse), heads_q, _ptr(table), table.shape[1], _ptr(lens), _ptr(cu_q), batch, tokens, max_q, int(max_len),
+            workspace = q.new_empty((ws_bytes,), dtype=torch.uint8)
+    qt, qh, _ = q.stride()
+    _call(q, lib().jules_hip_kv4_attention, float(scale), cache._ref, q.data_ptr(), qt, qh, out.data_ptr(), _ptr(lse),
+          heads_q, table.data_ptr(), table.shape[1], lens.data_ptr(), _ptr(cu_q), batch, tokens, max_q, int(max_len),
           _ptr(workspace), ws_bytes)
     return (out, lse) if return_lse else out
 
