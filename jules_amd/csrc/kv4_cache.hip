@@ -16,6 +16,7 @@
 // 8-byte groups of 4 tokens.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "kv4.hpp"
 #include "launch.hpp"
@@ -40,7 +41,26 @@ __device__ __forceinline__ void load8(const uint16_t* p, float* v) {
     for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(u[i]), v[2 * i + 1] = bf16_hi(u[i]);
 }
 
-// a row's codes of this lane's 8 values, and its scale and minimum
+// f over the LANES neighbouring lanes that hold a row, by lane permutations within
+// rows of 16 lanes: with the lane beside, the two beside, the mirror image in 8, in 16
+template <int LANES, typename F>
+__device__ __forceinline__ float over_row(float v, F f) {
+    const auto with = [&](auto ctrl) {
+        const int u = __float_as_int(v);
+        v = f(v, __int_as_float(__builtin_amdgcn_update_dpp(u, u, decltype(ctrl)::value, 0xf, 0xf, false)));
+    };
+    with(std::integral_constant<int, 0xb1>{});
+    with(std::integral_constant<int, 0x4e>{});
+    with(std::integral_constant<int, 0x141>{});
+    if constexpr (LANES == 16) with(std::integral_constant<int, 0x140>{});
+    return v;
+}
+
+// A row's codes of this lane's 8 values, and its scale and minimum.  A quotient is
+// the product with 1 / s, corrected by its remainder: that is the division's own
+// rounding wherever nothing leaves the normal numbers, since s has 8 bits (a
+// correctly rounded reciprocal and one correction give the correctly rounded
+// quotient but for divisors whose bits are all ones, a theorem of Markstein's).
 template <int LANES>
 __device__ __forceinline__ uint32_t quantise(const float* v, uint32_t* code) {
     float lo = v[0], hi = v[0];
@@ -52,11 +72,8 @@ __device__ __forceinline__ uint32_t quantise(const float* v, uint32_t* code) {
         fine = fine && fabsf(v[i]) <= FLT_MAX;
     }
     if (!fine) hi = __builtin_inff();  // kept by fmaxf, and the range with it
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor(lo, o));
-        hi = fmaxf(hi, __shfl_xor(hi, o));
-    }
+    lo = over_row<LANES>(lo, [](float a, float b) { return fminf(a, b); });
+    hi = over_row<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
     const float range = (hi - lo) / 15.0f;
     const uint32_t meta = pack_bf16x2(range, lo);
     const float s = bf16_lo(meta), m = bf16_hi(meta);
@@ -65,31 +82,42 @@ __device__ __forceinline__ uint32_t quantise(const float* v, uint32_t* code) {
         for (int i = 0; i < 8; ++i) code[i] = 0;
         return 0x7fc07fc0u;
     }
+    const auto coded = [](float t) { return (uint32_t)fminf(fmaxf(rintf(t), 0.0f), 15.0f); };
+    if (s > 0x1p-100f && s < 0x1p100f) {
+        const float r = 1.0f / s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        code[i] = s > 0.0f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(v[i] - m, s)), 0.0f), 15.0f) : 0u;
+        for (int i = 0; i < 8; ++i) {
+            const float d = v[i] - m, t = d * r;
+            code[i] = coded(__builtin_fmaf(__builtin_fmaf(-t, s, d), r, t));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = s > 0.0f ? coded(__fdiv_rn(v[i] - m, s)) : 0u;
+    }
     return meta;
 }
 
-// grid: x tokens of a sequence, y heads, z sequences; a block has
-// THREADS / LANES neighbouring tokens
+// grid: x heads within blocks of tokens of a sequence, y sequences; a block has
+// THREADS / LANES neighbouring tokens of a head, and neighbouring blocks the heads
+// of the same tokens, whose rows lie side by side
 template <typename T, int D>
 __global__ __launch_bounds__(THREADS) void kv4_append_kernel(KV4View c, KV4Batch b, RowsIn k, RowsIn v) {
     constexpr int LANES = D / 8, TOKENS = THREADS / LANES;
-    const int h = blockIdx.y, lane = threadIdx.x % LANES;
-    for (int seq = blockIdx.z; seq < b.batch; seq += gridDim.z) {
+    const int h = blockIdx.x % c.heads, lane = threadIdx.x % LANES;
+    const int block = blockIdx.x / c.heads, blocks = gridDim.x / c.heads;
+    for (int seq = blockIdx.y; seq < b.batch; seq += gridDim.y) {
         const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
-        for (int64_t i0 = (int64_t)blockIdx.x * TOKENS; i0 < n; i0 += (int64_t)gridDim.x * TOKENS) {
+        for (int64_t i0 = (int64_t)block * TOKENS; i0 < n; i0 += (int64_t)blocks * TOKENS) {
             const int i = (int)i0 + (int)threadIdx.x / LANES;
             if (i >= n) continue;
+            float x[8], y[8];
+            load8(static_cast<const T*>(k.p) + (first + i) * k.token_stride + h * k.head_stride + 8 * lane, x);
+            load8(static_cast<const T*>(v.p) + (first + i) * v.token_stride + h * v.head_stride + 8 * lane, y);
             const int64_t at = (int64_t)len - n + i;  // a row before the sequence's begin is dropped
             const int page = at >= 0 && at <= INT32_MAX ? kv4_page(c, b, seq, (int)at) : -1;
             if (page < 0) continue;
             const int off = (int)at & (c.page_size - 1);
             const int64_t row = kv4_row(c, page, h, off);
-            float x[8], y[8];
-            load8(static_cast<const T*>(k.p) + (first + i) * k.token_stride + h * k.head_stride + 8 * lane, x);
-            load8(static_cast<const T*>(v.p) + (first + i) * v.token_stride + h * v.head_stride + 8 * lane, y);
             uint32_t code[8];
             uint32_t meta = quantise<LANES>(x, code);
             uint32_t word = 0;
@@ -122,10 +150,11 @@ __device__ __forceinline__ void store8(uint16_t* p, const float* v) {
 template <typename T, int D>
 __global__ __launch_bounds__(THREADS) void kv4_read_kernel(KV4View c, KV4Batch b, T* k, T* v) {
     constexpr int LANES = D / 8, TOKENS = THREADS / LANES;
-    const int h = blockIdx.y, lane = threadIdx.x % LANES;
-    for (int seq = blockIdx.z; seq < b.batch; seq += gridDim.z) {
+    const int h = blockIdx.x % c.heads, lane = threadIdx.x % LANES;
+    const int block = blockIdx.x / c.heads, blocks = gridDim.x / c.heads;
+    for (int seq = blockIdx.y; seq < b.batch; seq += gridDim.y) {
         const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
-        for (int64_t i0 = (int64_t)blockIdx.x * TOKENS; i0 < n; i0 += (int64_t)gridDim.x * TOKENS) {
+        for (int64_t i0 = (int64_t)block * TOKENS; i0 < n; i0 += (int64_t)blocks * TOKENS) {
             const int i = (int)i0 + (int)threadIdx.x / LANES;
             if (i >= n) continue;
             const int64_t at = (int64_t)len - n + i;
@@ -163,8 +192,9 @@ __global__ __launch_bounds__(THREADS) void kv4_read_kernel(KV4View c, KV4Batch b
 template <int D>
 dim3 rows_grid(const KV4View& c, const KV4Batch& b) {
     const int tokens = THREADS / (D / 8);
-    return dim3((unsigned)std::min(65535, (b.max_q + tokens - 1) / tokens), (unsigned)c.heads,
-                (unsigned)std::min(65535, b.batch));
+    // below 2^24 blocks in x
+    const int blocks = std::min((b.max_q + tokens - 1) / tokens, std::max(1, (1 << 23) / c.heads));
+    return dim3((unsigned)(std::max(1, blocks) * c.heads), (unsigned)std::min(65535, b.batch));
 }
 
 }  // namespace
