@@ -414,7 +414,7 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  * JH_ERR_UNSUPPORTED), page_size 16, 32, 64, 128 or 256; heads <=
  * 65535; num_pages >= 1.
  *
- * A batch's new tokens, the same four arguments in the three calls:
+ * A batch's new tokens, the same arguments in the three calls (batch <= 65535):
  *   table   int32 [batch, max_pages], max_pages >= 1: the pages of each sequence in
  *           order
  *   lens    int32 [batch]: tokens of each sequence, the new ones among them

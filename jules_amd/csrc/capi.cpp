@@ -543,7 +543,7 @@ static int kv4_check(const char* who, const jh_kv4_cache* c, const int32_t* tabl
                      bool* done) {
     *done = false;
     if (!c) return fail(JH_ERR_NULL, "%s: null cache", who);
-    if (batch < 0 || tokens < 0 || max_q < 0 || max_pages < 0 || c->num_pages < 1)
+    if (batch < 0 || batch > 65535 || tokens < 0 || max_q < 0 || max_pages < 0 || c->num_pages < 1)
         return fail(JH_ERR_SHAPE, "%s: batch=%d tokens=%d max_q=%d max_pages=%d num_pages=%d", who, batch, tokens, max_q,
                     max_pages, c->num_pages);
     if (c->heads < 1 || c->heads > 65535) return fail(JH_ERR_SHAPE, "%s: %d heads (1..65535)", who, c->heads);
@@ -614,7 +614,7 @@ int jules_hip_kv4_read(int dtype, const jh_kv4_cache* cache, void* k, void* v, c
 
 size_t jules_hip_kv4_attention_workspace_size(int batch, int tokens, int heads_q, int heads, int head_dim, int max_q,
                                               int max_len) {
-    if (batch < 1 || tokens < 1 || heads < 1 || heads_q < heads || heads_q % heads || max_q < 0 || max_len < 0 ||
+    if (batch < 1 || batch > 65535 || tokens < 1 || heads < 1 || heads_q < heads || heads_q % heads || max_q < 0 || max_len < 0 ||
         (head_dim != 64 && head_dim != 128) || (int64_t)tokens * heads_q > int64_t(1) << 30)
         return 0;
     return jh::kv4_attn_workspace_size(batch, tokens, heads_q, heads, head_dim, max_q, max_len);

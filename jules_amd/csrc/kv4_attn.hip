@@ -216,6 +216,8 @@ struct Rows {
     // become 0, and the rows that see it NaN.
     __device__ __forceinline__ void mask(f32x4_t (&x)[RT][2], Raw<D>& v, const Place& p, int base) const {
         const int g = (threadIdx.x >> 4) & 3;
+        float nan = __builtin_nanf(""), unseen = -__builtin_inff();
+        asm volatile("" : "+v"(nan), "+v"(unseen));  // constants for here, not kept in registers
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -224,8 +226,8 @@ struct Rows {
                 v.meta[t][e] = none ? 0u : v.meta[t][e];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    const float y = none ? __builtin_nanf("") : x[r][t][e];
-                    x[r][t][e] = base + 16 * t + 4 * g + e > last[r] ? -__builtin_inff() : y;
+                    const float y = none ? nan : x[r][t][e];
+                    x[r][t][e] = base + 16 * t + 4 * g + e > last[r] ? unseen : y;
                 }
             }
     }
@@ -415,7 +417,7 @@ __device__ __forceinline__ void write(const AttnArgs& a, const Rows<D, RT>& R, i
 // SHARE: the four waves hold the same RT * 16 rows and take steps in turn, their
 // sums are added through LDS; otherwise each has RT * 16 rows of its own.
 template <int D, int RT, bool SHARE, bool P16>
-__global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : 2) void kv4_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : RT == 2 && D == 64 ? 3 : 2) void kv4_attn_kernel(AttnArgs a) {
     constexpr int WROWS = RT * 16, BROWS = SHARE ? WROWS : WROWS * WAVES;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // neighbouring workgroups have the heads of the same pages
@@ -423,140 +425,139 @@ __global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : 2) void kv4_attn_kernel(A
     const int row_blocks = gridDim.x / a.c.heads / a.splits;
     const float kscale = a.scale * LOG2E, kscale16 = 16.0f * kscale;
     const CodeMask mask = code_mask();
-    for (int seq = blockIdx.y; seq < a.b.batch; seq += gridDim.y) {
-        // Workgroups are dealt to an XCD's four shader engines in turn.  The last
-        // splits of short sequences are empty, and so are the last rows of those
-        // with few new tokens: which part a workgroup has moves on as the turn
-        // comes round, or an engine would get the same ones of all (64 sequences
-        // of 512 to 8192 keys in 4 splits: 83 us, so 72).
-        const int parts = a.splits * row_blocks, mine = (part + seq / a.turn) % parts;
-        const int split = mine % a.splits, row_block = mine / a.splits;
-        const int n = kv4_count(a.b, seq), first = kv4_first(a.b, seq);
-        const int len = min(max(0, kv4_scalar(a.b.lens + seq)), INT32_MAX - 2 * KEYS * WAVES);
-        // positions from here on are on no page; one of them is enough to say so
-        const int64_t room = (int64_t)a.b.max_pages << a.c.page_shift;
-        const Pages<P16> pages{a.b.table + (int64_t)seq * a.b.max_pages, a.b.max_pages - 1, a.c.page_shift,
-                               a.c.page_size - 1, (uint32_t)a.c.num_pages, (uint32_t)a.c.heads * a.c.page_size,
-                               (uint32_t)h * a.c.page_size};
-        const int rows = n * a.group;  // at most tokens * heads_q
-        for (int64_t r64 = (int64_t)row_block * BROWS; r64 < rows; r64 += (int64_t)row_blocks * BROWS) {
-            const int r0 = (int)r64, w0 = r0 + (SHARE ? 0 : wave * WROWS);
-            // Lane (n16, g): row n16 of 16, keys 4 g .. 4 g + 3 of 16.  The thread's
-            // index is taken anew here and after the steps: what follows from it is
-            // not kept in registers where it is not used.
-            int tid = threadIdx.x;
-            asm volatile("" : "+v"(tid));
-            const int lane = tid & 63, n16 = lane & 15, g = lane >> 4;
-            // this lane's bytes of 16 tokens' keys and values
-            const uint32_t k_at = n16 * (D / 2) + g * (D / 8), v_at = g * (2 * D) + n16 * (D / 8);
-            // keys that the wave's rows see, and that all of them see
-            int seen = 0, least = INT32_MAX;
-            if (w0 < rows) {
-                const int top = min(rows, w0 + WROWS) - 1;
-                seen = max(0, len - n + top / a.group + 1);
-                least = len - n + w0 / a.group + 1;
+    const int seq = blockIdx.y;
+    // Workgroups are dealt to an XCD's four shader engines in turn.  The last
+    // splits of short sequences are empty, and so are the last rows of those
+    // with few new tokens: which part a workgroup has moves on as the turn
+    // comes round, or an engine would get the same ones of all (64 sequences
+    // of 512 to 8192 keys in 4 splits: 83 us, so 72).
+    const int parts = a.splits * row_blocks, mine = (part + seq / a.turn) % parts;
+    const int split = mine % a.splits, row_block = mine / a.splits;
+    const int n = kv4_count(a.b, seq), first = kv4_first(a.b, seq);
+    const int len = min(max(0, kv4_scalar(a.b.lens + seq)), INT32_MAX - 2 * KEYS * WAVES);
+    // positions from here on are on no page; one of them is enough to say so
+    const int64_t room = (int64_t)a.b.max_pages << a.c.page_shift;
+    const Pages<P16> pages{a.b.table + (int64_t)seq * a.b.max_pages, a.b.max_pages - 1, a.c.page_shift,
+                           a.c.page_size - 1, (uint32_t)a.c.num_pages, (uint32_t)a.c.heads * a.c.page_size,
+                           (uint32_t)h * a.c.page_size};
+    const int rows = n * a.group;  // at most tokens * heads_q
+    for (int64_t r64 = (int64_t)row_block * BROWS; r64 < rows; r64 += (int64_t)row_blocks * BROWS) {
+        const int r0 = (int)r64, w0 = r0 + (SHARE ? 0 : wave * WROWS);
+        // Lane (n16, g): row n16 of 16, keys 4 g .. 4 g + 3 of 16.  The thread's
+        // index is taken anew here and after the steps: what follows from it is
+        // not kept in registers where it is not used.
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, n16 = lane & 15, g = lane >> 4;
+        // this lane's bytes of 16 tokens' keys and values
+        const uint32_t k_at = n16 * (D / 2) + g * (D / 8), v_at = g * (2 * D) + n16 * (D / 8);
+        // keys that the wave's rows see, and that all of them see
+        int seen = 0, least = INT32_MAX;
+        if (w0 < rows) {
+            const int top = min(rows, w0 + WROWS) - 1;
+            seen = max(0, len - n + top / a.group + 1);
+            least = len - n + w0 / a.group + 1;
+        }
+        const int end = (int)min((int64_t)seen, room + KEYS);
+        const int k0 = (int)min((int64_t)end, (int64_t)split * a.chunk);
+        const int k1 = split == a.splits - 1 ? end : (int)min((int64_t)end, (int64_t)k0 + a.chunk);
+        if (a.splits > 1 && k0 >= k1) {
+            // no keys for this split: it says so, its sums are not read
+            const int i = SHARE ? tid : lane;
+            if (i < WROWS && w0 + i < rows) {
+                const int64_t to = out_row(a, h, first, w0 + i);
+                float* m = part_meta(a, D, to, split);
+                float none = -FLT_MAX;
+                asm volatile("" : "+v"(none));  // a constant for here, not kept in a register
+                m[0] = none, m[1] = 0.0f;
             }
-            const int end = (int)min((int64_t)seen, room + KEYS);
-            const int k0 = (int)min((int64_t)end, (int64_t)split * a.chunk);
-            const int k1 = split == a.splits - 1 ? end : (int)min((int64_t)end, (int64_t)k0 + a.chunk);
-            if (a.splits > 1 && k0 >= k1) {
-                // no keys for this split: it says so, its sums are not read
-                const int i = SHARE ? tid : lane;
-                if (i < WROWS && w0 + i < rows) {
-                    const int64_t to = out_row(a, h, first, w0 + i);
-                    float* m = part_meta(a, D, to, split);
-                    float none = -FLT_MAX;
-                    asm volatile("" : "+v"(none));  // a constant for here, not kept in a register
-                    m[0] = none, m[1] = 0.0f;
+            continue;
+        }
+        const int step = SHARE ? KEYS * WAVES : KEYS;
+        int base = __builtin_amdgcn_readfirstlane(k0 + (SHARE ? wave * KEYS : 0));  // all well below 2^31
+        Raw<D> k, v;
+        int page[2];
+        Place here{};
+        bool loaded = base < k1;
+        if (loaded) {
+            pages.entries(base, page);
+            here = pages.place(base, len, page);
+            k.load(a.c.k, a.c.k_meta, here, k_at, 16 * g);
+            v.load(a.c.v, a.c.v_meta, here, v_at, 16 * g);
+        }
+        Rows<D, RT> R;
+        R.clear();
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = w0 + 16 * r + n16;
+            R.last[r] = -1;
+            R.qsum[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < R.KI; ++i) R.q[r][i] = operand(0, 0, 0, 0);
+            if (row < rows) {
+                const int i = row / a.group, head = h * a.group + row % a.group;
+                R.last[r] = len - n + i;
+                const uint16_t* q = a.q + (first + i) * a.q_token + head * a.q_head + g * (D / 4);
+#pragma unroll
+                for (int j = 0; j < R.KI; ++j) {
+                    const u32x4_t u = reinterpret_cast<const u32x4_t*>(q)[j];
+                    R.q[r][j] = __builtin_bit_cast(bf16x8_t, u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) R.qsum[r] += bf16_lo(u[e]) + bf16_hi(u[e]);
                 }
-                continue;
             }
-            const int step = SHARE ? KEYS * WAVES : KEYS;
-            int base = __builtin_amdgcn_readfirstlane(k0 + (SHARE ? wave * KEYS : 0));  // all well below 2^31
-            Raw<D> k, v;
-            int page[2];
-            Place here{};
-            bool loaded = base < k1;
-            if (loaded) {
+            R.qsum[r] = row_sum(R.qsum[r]);
+            R.qscaled[r] = R.qsum[r] * kscale;
+        }
+        // one tile of rows: the second product's operand from LDS, in the order
+        // of the lanes, leaves room for a fourth wave on each SIMD
+        __shared__ u32x4_t q_lds[RT == 1 ? 64 * (D / 32) : 1];
+        if constexpr (RT == 1) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) q_lds[lane + 64 * i] = __builtin_bit_cast(u32x4_t, R.q[0][i]);
+            __syncthreads();
+        }
+        const u32x4_t* q_at = q_lds + lane;
+        f32x4_t x[RT][2];
+        const int whole = min(k1, least - KEYS + 1);  // steps up to there: all rows see all keys
+        if (base < whole) {
+            bool bad = here.bad[0] | here.bad[1];
+            // The next step's keys are loaded once this step's are scores, its
+            // values once this step's are summed, into the same registers.
+            for (base += step; base < whole; base += step) {
+                pages.entries(base, page);
+                __builtin_amdgcn_sched_barrier(0);  // asked for here, looked at after the scores
+                R.scores(k, mask, kscale16, x, q_at);
+                here = pages.place(base, len, page);
+                k.load(a.c.k, a.c.k_meta, here, k_at, 16 * g);
+                R.rescale(x);
+                R.values(x, v, mask);
+                v.load(a.c.v, a.c.v_meta, here, v_at, 16 * g);
+                bad = bad | here.bad[0] | here.bad[1];
+            }
+            R.scores(k, mask, kscale16, x, q_at);
+            R.rescale(x);
+            R.values(x, v, mask);
+            if (bad) R.spoil();
+            loaded = false;
+        }
+        for (; base < k1; base += step) {
+            if (!loaded) {
                 pages.entries(base, page);
                 here = pages.place(base, len, page);
                 k.load(a.c.k, a.c.k_meta, here, k_at, 16 * g);
                 v.load(a.c.v, a.c.v_meta, here, v_at, 16 * g);
             }
-            Rows<D, RT> R;
-            R.clear();
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const int row = w0 + 16 * r + n16;
-                R.last[r] = -1;
-                R.qsum[r] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < R.KI; ++i) R.q[r][i] = operand(0, 0, 0, 0);
-                if (row < rows) {
-                    const int i = row / a.group, head = h * a.group + row % a.group;
-                    R.last[r] = len - n + i;
-                    const uint16_t* q = a.q + (first + i) * a.q_token + head * a.q_head + g * (D / 4);
-#pragma unroll
-                    for (int j = 0; j < R.KI; ++j) {
-                        const u32x4_t u = reinterpret_cast<const u32x4_t*>(q)[j];
-                        R.q[r][j] = __builtin_bit_cast(bf16x8_t, u);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) R.qsum[r] += bf16_lo(u[e]) + bf16_hi(u[e]);
-                    }
-                }
-                R.qsum[r] = row_sum(R.qsum[r]);
-                R.qscaled[r] = R.qsum[r] * kscale;
-            }
-            // one tile of rows: the second product's operand from LDS, in the order
-            // of the lanes, leaves room for a fourth wave on each SIMD
-            __shared__ u32x4_t q_lds[RT == 1 ? 64 * (D / 32) : 1];
-            if constexpr (RT == 1) {
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) q_lds[lane + 64 * i] = __builtin_bit_cast(u32x4_t, R.q[0][i]);
-                __syncthreads();
-            }
-            const u32x4_t* q_at = q_lds + lane;
-            f32x4_t x[RT][2];
-            const int whole = min(k1, least - KEYS + 1);  // steps up to there: all rows see all keys
-            if (base < whole) {
-                bool bad = here.bad[0] | here.bad[1];
-                // The next step's keys are loaded once this step's are scores, its
-                // values once this step's are summed, into the same registers.
-                for (base += step; base < whole; base += step) {
-                    pages.entries(base, page);
-                    __builtin_amdgcn_sched_barrier(0);  // asked for here, looked at after the scores
-                    R.scores(k, mask, kscale16, x, q_at);
-                    here = pages.place(base, len, page);
-                    k.load(a.c.k, a.c.k_meta, here, k_at, 16 * g);
-                    R.rescale(x);
-                    R.values(x, v, mask);
-                    v.load(a.c.v, a.c.v_meta, here, v_at, 16 * g);
-                    bad = bad | here.bad[0] | here.bad[1];
-                }
-                R.scores(k, mask, kscale16, x, q_at);
-                R.rescale(x);
-                R.values(x, v, mask);
-                if (bad) R.spoil();
-                loaded = false;
-            }
-            for (; base < k1; base += step) {
-                if (!loaded) {
-                    pages.entries(base, page);
-                    here = pages.place(base, len, page);
-                    k.load(a.c.k, a.c.k_meta, here, k_at, 16 * g);
-                    v.load(a.c.v, a.c.v_meta, here, v_at, 16 * g);
-                }
-                loaded = false;
-                R.scores(k, mask, kscale16, x, q_at);
-                R.mask(x, v, here, base);
-                R.rescale(x);
-                R.values(x, v, mask);
-            }
-            R.finish();
-            int tid2 = threadIdx.x;
-            asm volatile("" : "+v"(tid2));
-            write<D, RT, SHARE>(a, R, tid2, wave, split, h, first, rows, r0, w0);
+            loaded = false;
+            R.scores(k, mask, kscale16, x, q_at);
+            R.mask(x, v, here, base);
+            R.rescale(x);
+            R.values(x, v, mask);
         }
+        R.finish();
+        int tid2 = threadIdx.x;
+        asm volatile("" : "+v"(tid2));
+        write<D, RT, SHARE>(a, R, tid2, wave, split, h, first, rows, r0, w0);
     }
 }
 
@@ -644,7 +645,7 @@ Plan plan(int D, int batch, int heads_kv, int group, int max_q, int max_len) {
 
 template <int D, bool P16>
 hipError_t launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.row_blocks * p.splits * a.c.heads), (unsigned)std::min(a.b.batch, 65535));
+    const dim3 grid((unsigned)(p.row_blocks * p.splits * a.c.heads), (unsigned)a.b.batch);
     constexpr int T = 64 * WAVES, MOST = D == 128 ? 2 : 4;
     if (!p.share)
         kv4_attn_kernel<D, MOST, false, P16><<<grid, T, 0, s>>>(a);

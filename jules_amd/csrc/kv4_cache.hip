@@ -105,34 +105,33 @@ __global__ __launch_bounds__(THREADS) void kv4_append_kernel(KV4View c, KV4Batch
     constexpr int LANES = D / 8, TOKENS = THREADS / LANES;
     const int h = blockIdx.x % c.heads, lane = threadIdx.x % LANES;
     const int block = blockIdx.x / c.heads, blocks = gridDim.x / c.heads;
-    for (int seq = blockIdx.y; seq < b.batch; seq += gridDim.y) {
-        const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
-        for (int64_t i0 = (int64_t)block * TOKENS; i0 < n; i0 += (int64_t)blocks * TOKENS) {
-            const int i = (int)i0 + (int)threadIdx.x / LANES;
-            if (i >= n) continue;
-            float x[8], y[8];
-            load8(static_cast<const T*>(k.p) + (first + i) * k.token_stride + h * k.head_stride + 8 * lane, x);
-            load8(static_cast<const T*>(v.p) + (first + i) * v.token_stride + h * v.head_stride + 8 * lane, y);
-            const int64_t at = (int64_t)len - n + i;  // a row before the sequence's begin is dropped
-            const int page = at >= 0 && at <= INT32_MAX ? kv4_page(c, b, seq, (int)at) : -1;
-            if (page < 0) continue;
-            const int off = (int)at & (c.page_size - 1);
-            const int64_t row = kv4_row(c, page, h, off);
-            uint32_t code[8];
-            uint32_t meta = quantise<LANES>(x, code);
-            uint32_t word = 0;
+    const int seq = blockIdx.y;
+    const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
+    for (int64_t i0 = (int64_t)block * TOKENS; i0 < n; i0 += (int64_t)blocks * TOKENS) {
+        const int i = (int)i0 + (int)threadIdx.x / LANES;
+        if (i >= n) continue;
+        float x[8], y[8];
+        load8(static_cast<const T*>(k.p) + (first + i) * k.token_stride + h * k.head_stride + 8 * lane, x);
+        load8(static_cast<const T*>(v.p) + (first + i) * v.token_stride + h * v.head_stride + 8 * lane, y);
+        const int64_t at = (int64_t)len - n + i;  // a row before the sequence's begin is dropped
+        const int page = at >= 0 && at <= INT32_MAX ? kv4_page(c, b, seq, (int)at) : -1;
+        if (page < 0) continue;
+        const int off = (int)at & (c.page_size - 1);
+        const int64_t row = kv4_row(c, page, h, off);
+        uint32_t code[8];
+        uint32_t meta = quantise<LANES>(x, code);
+        uint32_t word = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) word |= code[e] << (4 * (e / 2) + 16 * (e % 2));
-            reinterpret_cast<uint32_t*>(c.k)[row * (D / 8) + lane] = word;
-            if (lane == 0) c.k_meta[row] = meta;
-            meta = quantise<LANES>(y, code);
-            // the four tokens' groups of 8 bytes: two of them for 8 values
-            uint16_t* held = reinterpret_cast<uint16_t*>(c.v) + (row - off % 4) * (D / 4) + off % 4;
+        for (int e = 0; e < 8; ++e) word |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+        reinterpret_cast<uint32_t*>(c.k)[row * (D / 8) + lane] = word;
+        if (lane == 0) c.k_meta[row] = meta;
+        meta = quantise<LANES>(y, code);
+        // the four tokens' groups of 8 bytes: two of them for 8 values
+        uint16_t* held = reinterpret_cast<uint16_t*>(c.v) + (row - off % 4) * (D / 4) + off % 4;
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-                held[4 * (2 * lane + g)] = (uint16_t)(code[4 * g] | code[4 * g + 1] << 4 | code[4 * g + 2] << 8 | code[4 * g + 3] << 12);
-            if (lane == 0) c.v_meta[row] = meta;
-        }
+        for (int g = 0; g < 2; ++g)
+            held[4 * (2 * lane + g)] = (uint16_t)(code[4 * g] | code[4 * g + 1] << 4 | code[4 * g + 2] << 8 | code[4 * g + 3] << 12);
+        if (lane == 0) c.v_meta[row] = meta;
     }
 }
 
@@ -152,40 +151,39 @@ __global__ __launch_bounds__(THREADS) void kv4_read_kernel(KV4View c, KV4Batch b
     constexpr int LANES = D / 8, TOKENS = THREADS / LANES;
     const int h = blockIdx.x % c.heads, lane = threadIdx.x % LANES;
     const int block = blockIdx.x / c.heads, blocks = gridDim.x / c.heads;
-    for (int seq = blockIdx.y; seq < b.batch; seq += gridDim.y) {
-        const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
-        for (int64_t i0 = (int64_t)block * TOKENS; i0 < n; i0 += (int64_t)blocks * TOKENS) {
-            const int i = (int)i0 + (int)threadIdx.x / LANES;
-            if (i >= n) continue;
-            const int64_t at = (int64_t)len - n + i;
-            const int page = at >= 0 && at <= INT32_MAX ? kv4_page(c, b, seq, (int)at) : -1;
-            float x[8], y[8];
-            if (page < 0) {
-                const float none = at < 0 ? 0.0f : __builtin_nanf("");
+    const int seq = blockIdx.y;
+    const int n = kv4_count(b, seq), first = kv4_first(b, seq), len = kv4_scalar(b.lens + seq);
+    for (int64_t i0 = (int64_t)block * TOKENS; i0 < n; i0 += (int64_t)blocks * TOKENS) {
+        const int i = (int)i0 + (int)threadIdx.x / LANES;
+        if (i >= n) continue;
+        const int64_t at = (int64_t)len - n + i;
+        const int page = at >= 0 && at <= INT32_MAX ? kv4_page(c, b, seq, (int)at) : -1;
+        float x[8], y[8];
+        if (page < 0) {
+            const float none = at < 0 ? 0.0f : __builtin_nanf("");
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = y[e] = none;
-            } else {
-                const int off = (int)at & (c.page_size - 1);
-                const int64_t row = kv4_row(c, page, h, off);
-                const uint32_t word = reinterpret_cast<const uint32_t*>(c.k)[row * (D / 8) + lane];
-                uint32_t meta = c.k_meta[row];
+            for (int e = 0; e < 8; ++e) x[e] = y[e] = none;
+        } else {
+            const int off = (int)at & (c.page_size - 1);
+            const int64_t row = kv4_row(c, page, h, off);
+            const uint32_t word = reinterpret_cast<const uint32_t*>(c.k)[row * (D / 8) + lane];
+            uint32_t meta = c.k_meta[row];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = __builtin_fmaf(bf16_lo(meta), (float)(word >> (4 * (e / 2) + 16 * (e % 2)) & 15u), bf16_hi(meta));
-                meta = c.v_meta[row];
-                const uint16_t* held = reinterpret_cast<const uint16_t*>(c.v) + (row - off % 4) * (D / 4) + off % 4;
+            for (int e = 0; e < 8; ++e)
+                x[e] = __builtin_fmaf(bf16_lo(meta), (float)(word >> (4 * (e / 2) + 16 * (e % 2)) & 15u), bf16_hi(meta));
+            meta = c.v_meta[row];
+            const uint16_t* held = reinterpret_cast<const uint16_t*>(c.v) + (row - off % 4) * (D / 4) + off % 4;
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const uint32_t u = held[4 * (2 * lane + g)];
+            for (int g = 0; g < 2; ++g) {
+                const uint32_t u = held[4 * (2 * lane + g)];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        y[4 * g + e] = __builtin_fmaf(bf16_lo(meta), (float)(u >> (4 * e) & 15u), bf16_hi(meta));
-                }
+                for (int e = 0; e < 4; ++e)
+                    y[4 * g + e] = __builtin_fmaf(bf16_lo(meta), (float)(u >> (4 * e) & 15u), bf16_hi(meta));
             }
-            const int64_t to = ((int64_t)(first + i) * c.heads + h) * D + 8 * lane;
-            store8(k + to, x);
-            store8(v + to, y);
         }
+        const int64_t to = ((int64_t)(first + i) * c.heads + h) * D + 8 * lane;
+        store8(k + to, x);
+        store8(v + to, y);
     }
 }
 
@@ -194,7 +192,7 @@ dim3 rows_grid(const KV4View& c, const KV4Batch& b) {
     const int tokens = THREADS / (D / 8);
     // below 2^24 blocks in x
     const int blocks = std::min((b.max_q + tokens - 1) / tokens, std::max(1, (1 << 23) / c.heads));
-    return dim3((unsigned)(std::max(1, blocks) * c.heads), (unsigned)std::min(65535, b.batch));
+    return dim3((unsigned)(std::max(1, blocks) * c.heads), (unsigned)b.batch);
 }
 
 }  // namespace
