@@ -433,8 +433,8 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  *
  * jules_hip_kv4_append: writes the new rows.  dtype JH_F32 or JH_BF16, k and v
  *   [tokens, heads, D] with strides in elements between tokens and heads (the D
- *   elements side by side); s = bf16((max - min) / 15), m = bf16(min), c =
- *   clamp(rint((x - m) / s), 0, 15), 0 where s is 0.  A row with a NaN or an
+ *   elements side by side); s = bf16((max - min) * (1.0f / 15)), m = bf16(min),
+ *   c = clamp(rint((x - m) / s), 0, 15), 0 where s is 0, in fp32.  A row with a NaN or an
  *   infinity, or a range past fp32 or a minimum past bf16, is held as NaN throughout.
  *   A row before position 0 is dropped.
  * jules_hip_kv4_read: the new rows as values m + s c into dense k and v

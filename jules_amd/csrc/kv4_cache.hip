@@ -2,7 +2,7 @@
 // kv4.hpp).  No counterpart in the reference.
 //
 // Writing a row x of D values:
-//   s = bf16((max x - min x) / 15),  m = bf16(min x),
+//   s = bf16((max x - min x) * fp32(1/15)),  m = bf16(min x),
 //   c = clamp(rint((x - m) / s), 0, 15)          (0 where s = 0)
 // The rounded s and m are the ones that the codes are formed with, so a value
 // is off by half a step and, at the row's ends, by what s and m were rounded.
@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t quantise(const float* v, uint32_t* code) {
     if (!fine) hi = __builtin_inff();  // kept by fmaxf, and the range with it
     lo = over_row<LANES>(lo, [](float a, float b) { return fminf(a, b); });
     hi = over_row<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
-    const float range = (hi - lo) / 15.0f;
+    const float range = (hi - lo) * (1.0f / 15.0f);
     const uint32_t meta = pack_bf16x2(range, lo);
     const float s = bf16_lo(meta), m = bf16_hi(meta);
     if (!(range <= FLT_MAX) || !(fabsf(m) <= FLT_MAX)) {

@@ -72,7 +72,7 @@ def quantise(x):
     x = np.asarray(x, np.float32)
     lo, hi = x.min(-1, keepdims=True), x.max(-1, keepdims=True)
     with np.errstate(all="ignore"):
-        rng = ((hi - lo) / np.float32(15.0)).astype(np.float32)
+        rng = ((hi - lo) * (np.float32(1.0) / np.float32(15.0))).astype(np.float32)
         s, m = bf16(rng), bf16(lo)
         bad = ~np.isfinite(x).all(-1, keepdims=True) | ~np.isfinite(rng) | ~np.isfinite(m)
         c = np.rint(((x - m) / s).astype(np.float32))

@@ -276,7 +276,7 @@ def test_growing_scores(dev):
         p["K"].m[:] = 0.0
         for at in range(500):
             pg, off = p["table"][0][at // 16], at % 16
-            p["K"].m[pg, 0, off] = bf16(sign * at / 10.0)
+            p["K"].m[pg, 0, off] = bf16([sign * at / 10.0])[0]
         k, _, km = p["K"].packed(dev)
         p["cache"] = ops.KV4Cache(k, p["cache"].v, km, p["cache"].v_meta)
         p["qd"] = torch.from_numpy(p["q"]).to(b16).to(dev)
