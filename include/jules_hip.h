@@ -391,7 +391,7 @@ int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const 
  * may be x with the same strides and dtype; other overlaps are not allowed.
  * positions int32 [axes, B, S], any sign; inv_freq fp64 [R/2]; pair_axis int32
  * [R/2] or NULL (axis 0); a pair whose axis is outside [0, axes) gives NaN.
- * 2 <= R <= D, R even, D <= 1024, 1 <= axes <= 16, B * S <= 2^28, H <= 65535.
+ * 2 <= R <= D, R even, D <= 1024, 1 <= axes <= 16, B * S <= 2^27, H <= 65535.
  */
 int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const void* x,
                      const int64_t* x_strides, void* out, const int64_t* out_strides,

@@ -510,7 +510,7 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
     if (!real(x_dtype) || !real(out_dtype)) return fail(JH_ERR_DTYPE, "rotary: dtypes %d %d", x_dtype, out_dtype);
     if ((pairing != 0 && pairing != 1) || (inverse != 0 && inverse != 1))
         return fail(JH_ERR_ARG, "rotary: pairing %d, inverse %d (0 or 1)", pairing, inverse);
-    if (B < 0 || H < 0 || S < 0 || H > 65535 || (int64_t)B * S > (int64_t(1) << 28))
+    if (B < 0 || H < 0 || S < 0 || H > 65535 || (int64_t)B * S > (int64_t(1) << 27))
         return fail(JH_ERR_SHAPE, "rotary: B=%d H=%d S=%d", B, H, S);
     if (D < 2 || D > 1024 || R < 2 || R > D || R % 2)
         return fail(JH_ERR_SHAPE, "rotary: D=%d R=%d (2 <= R <= D <= 1024, R even)", D, R);

@@ -186,7 +186,9 @@ struct Rows {
     }
 
     // Scores of the step's keys base .. base + 31, relative to `ref`.
-    __device__ __forceinline__ void scores(const Raw<D>& k, CodeMask m, float kscale16, f32x4_t (&x)[RT][2], const u32x4_t* q_at) const {
+    // q_at: with one tile of rows, this lane's operands of the queries in LDS.
+    __device__ __forceinline__ void scores(const Raw<D>& k, CodeMask m, float kscale16, f32x4_t (&x)[RT][2],
+                                           const u32x4_t* q_at) const {
 #pragma unroll
         for (int r = 0; r < RT; ++r) x[r][0] = x[r][1] = f32x4_t{-qsum[r], -qsum[r], -qsum[r], -qsum[r]};
 #pragma unroll
@@ -196,8 +198,13 @@ struct Rows {
                 const uint32_t w = k.w[t][i];
                 const bf16x8_t kc = operand(codes(m, w, 0), codes(m, w, 1), codes(m, w, 2), codes(m, w, 3));
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
-                    x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, RT == 1 ? __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const volatile u32x4_t*>(q_at + 64 * i)) : q[r][i], x[r][t], 0, 0, 0);
+                for (int r = 0; r < RT; ++r) {
+                    // volatile: read at each step, not once and kept
+                    const bf16x8_t qi = RT == 1 ? __builtin_bit_cast(
+                                                      bf16x8_t, *reinterpret_cast<const volatile u32x4_t*>(q_at + 64 * i))
+                                                : q[r][i];
+                    x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, qi, x[r][t], 0, 0, 0);
+                }
             }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -625,14 +632,15 @@ struct Plan {
 // in 64 splits, 27 + 4 in 48, 25 + 6 in 96, 23 + 7 in 128; 15627 keys of 3022
 // new tokens: 311 us whole, 375 + 32 in 2).  A split costs a second launch too:
 // none below 1024 keys (1000 keys: 11 us whole, 7 + 3 in 4 splits).
-Plan plan(int D, int batch, int heads_kv, int group, int max_q, int max_len) {
+Plan plan(int D, int batch, int tokens, int heads_kv, int group, int max_q, int max_len) {
     Plan p;
-    const int64_t rows = (int64_t)max_q * group;
+    const int64_t rows = (int64_t)std::max(1, std::min(max_q, tokens)) * group;
     p.rt = rows <= 16 ? 1 : rows <= 32 || D == 128 ? 2 : rows <= 48 ? 3 : 4;  // what a wave's registers hold
     p.share = rows <= 64;
     const int64_t brows = p.share ? p.rt * 16 : p.rt * 16 * WAVES;
-    p.row_blocks = (int)std::min((int64_t)65536, (rows + brows - 1) / brows);
-    const int64_t groups = std::max((int64_t)1, (int64_t)batch * heads_kv * p.row_blocks);
+    // below 2^24 workgroups of 256 threads; a workgroup goes on to the rows that are left
+    p.row_blocks = (int)std::min((int64_t)std::max(1, (1 << 22) / heads_kv), (rows + brows - 1) / brows);
+    const int64_t groups = (int64_t)batch * heads_kv * p.row_blocks;
     const int full = p.rt == 1 ? 2048 : p.rt == 2 ? p.share ? 1024 : 512 : 256;
     const int64_t want = std::max((int64_t)1, full / groups);
     const int unit = KEYS * WAVES;
@@ -673,14 +681,14 @@ hipError_t launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
 }  // namespace
 
 size_t kv4_attn_workspace_size(int batch, int tokens, int heads_q, int heads_kv, int D, int max_q, int max_len) {
-    const Plan p = plan(D, batch, heads_kv, heads_q / heads_kv, max_q, max_len);
+    const Plan p = plan(D, batch, tokens, heads_kv, heads_q / heads_kv, max_q, max_len);
     return p.splits > 1 ? (size_t)tokens * heads_q * p.splits * (D + 2) * sizeof(float) : 0;
 }
 
 hipError_t launch_kv4_attn(float scale, const KV4View& c, const KV4Batch& b, const uint16_t* q, int64_t q_token,
                            int64_t q_head, uint16_t* o, float* lse, int heads_q, int max_len, void* ws, hipStream_t s) {
     const int group = heads_q / c.heads;
-    const Plan p = plan(c.D, b.batch, c.heads, group, b.max_q, max_len);
+    const Plan p = plan(c.D, b.batch, b.tokens, c.heads, group, b.max_q, max_len);
     const AttnArgs a{c, b, q, q_token, q_head, o, lse, static_cast<float*>(ws), scale, heads_q, group, p.splits, p.chunk,
                      p.splits * p.row_blocks % 4 == 0 ? 1 : p.splits * p.row_blocks % 2 == 0 ? 2 : 4};
     return c.D == 128 ? launch<128>(a, p, s) : launch<64>(a, p, s);

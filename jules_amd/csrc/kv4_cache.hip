@@ -190,9 +190,10 @@ __global__ __launch_bounds__(THREADS) void kv4_read_kernel(KV4View c, KV4Batch b
 template <int D>
 dim3 rows_grid(const KV4View& c, const KV4Batch& b) {
     const int tokens = THREADS / (D / 8);
+    const int rows = std::max(1, std::min(b.max_q, b.tokens));
     // below 2^24 blocks in x
-    const int blocks = std::min((b.max_q + tokens - 1) / tokens, std::max(1, (1 << 23) / c.heads));
-    return dim3((unsigned)(std::max(1, blocks) * c.heads), (unsigned)b.batch);
+    const int blocks = std::min((rows - 1) / tokens + 1, std::max(1, (1 << 23) / c.heads));
+    return dim3((unsigned)(blocks * c.heads), (unsigned)b.batch);
 }
 
 }  // namespace

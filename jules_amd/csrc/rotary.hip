@@ -190,8 +190,8 @@ hipError_t launch_rotary(int x_dtype, int out_dtype, bool half, bool inverse, co
         a.hc = std::min(H, lanes);  // few tokens: one step a thread, on as many blocks as there are
     else
         a.tb = std::max(1, std::min(16, 1024 / std::min(1024, H * pieces)));  // at least four steps a thread
-    // fewer than 2^24 blocks of 256 threads
-    while ((a.tokens + a.tb - 1) / a.tb >= (1 << 24) && a.tb < 16) a.tb *= 2;
+    // fewer than 2^24 blocks of 256 threads (at most 2^27 tokens)
+    while ((a.tokens + a.tb - 1) / a.tb >= (1 << 24)) a.tb *= 2;
     if (x_dtype == JH_F32)
         return out_dtype == JH_F32 ? launch<float, float>(half, a, v, s) : launch<float, uint16_t>(half, a, v, s);
     return out_dtype == JH_F32 ? launch<uint16_t, float>(half, a, v, s) : launch<uint16_t, uint16_t>(half, a, v, s);

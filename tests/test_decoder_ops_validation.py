@@ -43,7 +43,7 @@ def test_add_rmsnorm_statuses(change, status):
 
 @pytest.mark.parametrize("change,status", [
     (dict(x_dtype=2), DTYPE), (dict(out_dtype=7), DTYPE), (dict(pairing=2), ARG), (dict(inverse=-1), ARG),
-    (dict(B=-1), SHAPE), (dict(H=65536), SHAPE), (dict(B=1 << 15, S=1 << 14), SHAPE), (dict(D=1), SHAPE),
+    (dict(B=-1), SHAPE), (dict(H=65536), SHAPE), (dict(B=1 << 14, S=(1 << 13) + 1), SHAPE), (dict(D=1), SHAPE),
     (dict(D=1026, R=64), SHAPE), (dict(R=63), SHAPE), (dict(R=0), SHAPE), (dict(R=130), SHAPE), (dict(axes=0), SHAPE),
     (dict(axes=17), SHAPE), (dict(x=None), NULL), (dict(xs=None), NULL), (dict(pos=None), NULL), (dict(freq=None), NULL),
     (dict(x=P + 2), ALIGN), (dict(out=P + 1), ALIGN), (dict(freq=P + 4), ALIGN), (dict(axis=P + 2), ALIGN),
@@ -123,7 +123,7 @@ def test_kv4_workspace_size():
         assert f(*bad) == 0
     # whatever the sizes, the sums of all splits fit what a row may have
     for batch in (1, 3, 64, 65535):
-        for max_q in (0, 1, 7, 1000, 2**31 - 1):
+        for max_q in (0, 1, 7, 16, 1000, 2**31 - 1):
             for max_len in (0, 1, 1000, 10**6, 2**31 - 1):
                 n = f(batch, 16, 16, 4, 128, max_q, max_len)
                 assert n % (16 * 16 * 130 * 4) == 0 and n // (16 * 16 * 130 * 4) <= 4096

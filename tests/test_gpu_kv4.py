@@ -159,6 +159,11 @@ def test_append_outside(dev):
     assert rows_changed([[7, 3]], [32], [0, 32]) == 16     # 7 is not a page of the pool
     assert rows_changed([[0, 1]], [-5], None) == 0
     assert rows_changed([[0, 1]], [2**31 - 1], None) == 0
+    was = _state(cache)
+    ops.kv4_append(cache, x, x, _int(dev, [[0, 1]]), _int(dev, [20]), cu_q=_int(dev, [0, 20]), max_q=0)
+    ops.kv4_append(cache, -x, -x, _int(dev, [[2, 3]]), _int(dev, [32]), cu_q=_int(dev, [0, 32]), max_q=2**31 - 1)
+    torch.cuda.synchronize()
+    assert int((cache.k != was[0]).flatten(2).any(-1).any(-1).sum()) == 4  # a hint costs time only
     assert rows_changed([[0], [1]], [8, 8], [30, 20, 50]) == 8  # none, then rows 20 .. 39 of which 8 fit
     assert rows_changed([[0, 1], [2, 3]], [20, 20], [-7, 5, 5]) == 5
     k, v = ops.kv4_read(cache, _int(dev, [[0, 9]]), _int(dev, [30]), 40)
@@ -257,6 +262,8 @@ def test_many_tokens(dev, D, heads, group, new):
     _run(p, max_q=max(new), max_len=max(lens))
     _run(p)                      # no hints
     _run(p, max_q=1, max_len=1)  # hints that are too small
+    _run(p, max_q=0, max_len=0)
+    _run(p, max_q=2**31 - 1, max_len=2**31 - 1)  # and much too large
 
 
 @pytest.mark.parametrize("scale_q,scale", [(1.0, 0.01), (8.0, 1.0), (0.02, 1.0), (30.0, 0.5)])
@@ -430,6 +437,30 @@ def test_graph(dev):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want), i
+
+
+def test_graph_with_splits(dev):
+    """Keys enough for several ranges: each captured graph has its own workspace,
+    and eager calls go on beside them."""
+    p = _problem(dev, 128, 64, 2, 4, [5000, 4097], [1, 1], seed=15, cu=False)
+    q, args = p["qd"], dict(p["args"], max_len=5000)
+    assert ops.lib().jules_hip_kv4_attention_workspace_size(2, 2, 8, 2, 128, 1, 5000) > 0
+    graphs = []
+    for _ in range(2):
+        out, lse, g = torch.empty_like(q), torch.empty(2, 8, device=dev), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.kv4_attention(q, p["cache"], out=out, lse=lse, **args)
+        graphs.append((g, out, lse))
+    for i in range(5):
+        q.copy_(torch.randn_like(q.float()))
+        p["args"]["lens"].copy_(_int(dev, [5000 - 600 * i, 4097 - 1000 * i]))
+        want = ops.kv4_attention(q, p["cache"], return_lse=True, **args)
+        torch.cuda.synchronize()
+        for g, out, lse in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out, lse in graphs:
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
 
 
 def test_offsets_past_32_bits(dev):
