@@ -15,7 +15,7 @@
 // multiplied by is the code's distance from the middle of the row's range, about
 // the value's distance from the row's mean: the error is that of an attention
 // with bf16 probabilities.  (With MID = 1 it was 0.0049 of the output at 8192
-// keys of unit variance, with this one 0.0020; bf16 outputs alone are 0.0017.)
+// keys of unit variance, with this one 0.0023; bf16 outputs alone are 0.0017.)
 //
 // One wave holds 16 rows (new tokens x heads of the group) times RT, and takes 32 keys
 // at a time.  Both products are transposed, S^T = K Q^T and O^T = V^T P^T: the
@@ -23,6 +23,15 @@
 // second product's operand, 4 neighbouring keys of each 16, and the softmax
 // needs no exchange between lanes but for the row's maximum when it grows.
 // Keys and values go from memory to the matrix cores through registers alone.
+//
+// Bound, one new token and 8 heads a key head, 64 sequences of 8192 keys: HBM, 4.9
+// TB/s (116 us); of 4096: 4.5 TB/s (64 us).  A short text of one sequence: what one
+// CU takes in, 27 bytes/ns (1000 keys 10 us, 128 keys 5 us, 1 key 5 us).  From 32 rows on:
+// vector instructions, a score's scale, exponential and rounding and a code's shift
+// and and-or, 62 % of the cycles to the matrix cores' 30 %: chunks of 1024 tokens
+// over 8192 keys, 8 sequences, 32 heads, D 128, 699 TFLOP/s, D 64 622.  Keys and values converted
+// once for a workgroup, through LDS, were no faster (314 us to 311 over 15627
+// keys; D 64 1034 to 829): the conversion saved went into writing and reading.
 #include <algorithm>
 #include <cfloat>
 
@@ -437,7 +446,7 @@ __global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : RT == 2 && D == 64 ? 3 : 
     // splits of short sequences are empty, and so are the last rows of those
     // with few new tokens: which part a workgroup has moves on as the turn
     // comes round, or an engine would get the same ones of all (64 sequences
-    // of 512 to 8192 keys in 4 splits: 83 us, so 72).
+    // of 512 to 8192 keys in 4 splits: 83 us, so 68).
     const int parts = a.splits * row_blocks, mine = (part + seq / a.turn) % parts;
     const int split = mine % a.splits, row_block = mine / a.splits;
     const int n = kv4_count(a.b, seq), first = kv4_first(a.b, seq);
@@ -627,11 +636,11 @@ struct Plan {
 
 // Rows of a sequence and key head decide the tile.  The keys are split until
 // the card is full: 8 workgroups a CU of one tile (64 sequences of 512 to 8192
-// keys: 80 us whole, 79 + 5 in 2 splits, 70 + 5 in 4, 67 + 7 in 8), fewer of more
-// tiles, whose start and end cost more (131072 keys, 40 rows of 64: 23 + 4 us
-// in 64 splits, 27 + 4 in 48, 25 + 6 in 96, 23 + 7 in 128; 15627 keys of 3022
-// new tokens: 311 us whole, 375 + 32 in 2).  A split costs a second launch too:
-// none below 1024 keys (1000 keys: 11 us whole, 7 + 3 in 4 splits).
+// keys: 82 us whole, 78 + 5 in 2 splits, 68 + 5 in 4, 66 + 7 in 8), fewer of more
+// tiles, whose start and end cost more (131072 keys, 40 rows of 64: 23 + 5 us
+// in 64 splits, 27 + 5 in 48, 24 + 6 in 96, 21 + 7 in 128; 15627 keys of 3022
+// new tokens: 315 us whole, 382 + 32 in 2).  A split costs a second launch too:
+// none below 1024 keys (1000 keys: 10 us whole, 7 + 3 in 4 splits).
 Plan plan(int D, int batch, int tokens, int heads_kv, int group, int max_q, int max_len) {
     Plan p;
     const int64_t rows = (int64_t)std::max(1, std::min(max_q, tokens)) * group;
