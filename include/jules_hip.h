@@ -452,7 +452,9 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  *   arguments, 16-byte aligned, no initialisation, overwritten by every call;
  *   calls that overlap in time need separate ones (0 bytes: NULL will do).
  *   fp32 accumulation and softmax; probabilities times the value's scale are
- *   rounded to bf16.  Deterministic.  The calls may be captured in a graph.
+ *   rounded to bf16.  Scores have to stay within fp32; values of a magnitude past
+ *   2^116 / keys may pass it in the sums (to infinity or NaN), below 2^-100 they
+ *   lose precision.  Deterministic.  The calls may be captured in a graph.
  */
 typedef struct jh_kv4_cache {
     void* k;

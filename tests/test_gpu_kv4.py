@@ -274,6 +274,23 @@ def test_scales(dev, scale_q, scale):
     _run(p, scale=scale)
 
 
+@pytest.mark.parametrize("power", [90, 16, -60])
+@pytest.mark.parametrize("D,lens,new", [(128, [400, 64, 33], [1, 1, 1]), (64, [5000], [2]), (128, [300, 90], [40, 33])])
+def test_scaled_values(dev, D, lens, new, power):
+    """Values times a power of two: each sum and rounding scales with them, bit for bit.
+    5000 keys leave 2^103 for the largest, and with scores of unit variance no
+    probability is below 2^-30."""
+    case(f"kv4 attention values times 2^{power} D={D} lens={lens}")
+    p = _problem(dev, D, 64, 2, 4, lens, new, seed=15)
+    hints = dict(max_q=max(new), max_len=max(lens))
+    o, lse = _run(p, **hints)
+    p["V"].m[:], p["V"].s[:] = p["V"].m * 2.0**power, p["V"].s * 2.0**power
+    _, v, vm = p["V"].packed(dev)
+    p["cache"] = ops.KV4Cache(p["cache"].k, v, p["cache"].k_meta, vm)
+    o2, lse2 = _run(p, **hints)
+    assert torch.equal(o2.float(), o.float() * 2.0**power) and torch.equal(lse2, lse)
+
+
 def test_growing_scores(dev):
     """Keys whose scores rise from first to last: the reference moves at every step;
     and scores far below zero."""
