@@ -10,6 +10,8 @@
 //   q . K  = 16 s_k (q . C - sum q) + m_k sum q
 //   sum p V = 16 (sum P' C - MID sum P') + sum p (m_v + 7.5 s_v),
 //   P' = bf16(p s_v),  MID = 1 + 7.5/16
+// (the values' lowest codes of each 16 bits are not shifted, and C = 1 + c/128, with
+// 128 for 16: a sixteenth of the shifts less, 316 us for 322 over 15627 keys).
 // -sum q is the accumulator that the first product starts from.  P' is rounded
 // once and both of its sums take the rounded number, so what its rounding is
 // multiplied by is the code's distance from the middle of the row's range, about
@@ -28,10 +30,13 @@
 // TB/s (116 us); of 4096: 4.5 TB/s (64 us).  A short text of one sequence: what one
 // CU takes in, 27 bytes/ns (1000 keys 10 us, 128 keys 5 us, 1 key 5 us).  From 32 rows on:
 // vector instructions, a score's scale, exponential and rounding and a code's shift
-// and and-or, 62 % of the cycles to the matrix cores' 30 %: chunks of 1024 tokens
-// over 8192 keys, 8 sequences, 32 heads, D 128, 699 TFLOP/s, D 64 622.  Keys and values converted
-// once for a workgroup, through LDS, were no faster (314 us to 311 over 15627
-// keys; D 64 1034 to 829): the conversion saved went into writing and reading.
+// and and-or, about 290 beside 34 of the matrix cores' for 32 rows and 32 keys: chunks
+// of 1024 tokens over 8192 keys, 8 sequences, 32 heads, D 128, 743 TFLOP/s, D 64 670.
+// Keys and values converted once for a workgroup, through LDS, were no faster (314
+// us to 311 over 15627 keys; D 64 1034 to 829): the conversion saved went into
+// writing and reading.  Keys as bytes, of which e4m3 holds 0 to 15 exactly, and q as
+// two parts of bytes need fewer conversions (269 us to 293 a call), but that
+// product adds in fewer bits: the log-sum-exp's error was 10^-5 and not 4 10^-7.
 #include <algorithm>
 #include <cfloat>
 
@@ -44,7 +49,6 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int KEYS = 32;     // keys of a step
 constexpr int WAVES = 4;     // waves of a workgroup
-constexpr float MID = 1.0f + 7.5f / 16.0f;  // C of the middle of a row's range
 constexpr float GROW = 8.0f; // a row's reference grows when a score passes it by this (log2)
 
 struct AttnArgs {
@@ -63,19 +67,24 @@ struct AttnArgs {
 
 // C of the low nibble of each half, bits 3-6 of a bf16 1.x
 struct CodeMask {
-    uint32_t keep, one;
+    uint32_t keep, low, one;
 };
 // The two constants in registers, a vector and a scalar one, as one and-or
 // takes them: as literals they are an and and an or.
 __device__ __forceinline__ CodeMask code_mask() {
-    CodeMask m{0x00780078u, 0x3f803f80u};
+    CodeMask m{0x00780078u, 0x000f000fu, 0x3f803f80u};
     asm volatile("" : "+v"(m.keep));
+    asm volatile("" : "+v"(m.low));
     asm volatile("" : "+s"(m.one));
     return m;
 }
 __device__ __forceinline__ uint32_t codes(CodeMask m, uint32_t w, int j) {
     const uint32_t x = j == 0 ? w << 3 : w >> (4 * j - 3);
     return (x & m.keep) | m.one;
+}
+// the value's, whose lowest code stays where it is: 1 + c/128
+__device__ __forceinline__ uint32_t value_codes(CodeMask m, uint32_t w, int j) {
+    return j == 0 ? (w & m.low) | m.one : codes(m, w, j);
 }
 __device__ __forceinline__ bf16x8_t operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(bf16x8_t, u32x4_t{a, b, c, d});
@@ -201,20 +210,24 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < RT; ++r) x[r][0] = x[r][1] = f32x4_t{-qsum[r], -qsum[r], -qsum[r], -qsum[r]};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < KI; ++i) {
+            bf16x8_t kc[2];
 #pragma unroll
-            for (int i = 0; i < KI; ++i) {
+            for (int t = 0; t < 2; ++t) {
                 const uint32_t w = k.w[t][i];
-                const bf16x8_t kc = operand(codes(m, w, 0), codes(m, w, 1), codes(m, w, 2), codes(m, w, 3));
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    // volatile: read at each step, not once and kept
-                    const bf16x8_t qi = RT == 1 ? __builtin_bit_cast(
-                                                      bf16x8_t, *reinterpret_cast<const volatile u32x4_t*>(q_at + 64 * i))
-                                                : q[r][i];
-                    x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, qi, x[r][t], 0, 0, 0);
-                }
+                kc[t] = operand(codes(m, w, 0), codes(m, w, 1), codes(m, w, 2), codes(m, w, 3));
             }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                // volatile: read at each step, not once and kept
+                const bf16x8_t qi = RT == 1 ? __builtin_bit_cast(
+                                                  bf16x8_t, *reinterpret_cast<const volatile u32x4_t*>(q_at + 64 * i))
+                                            : q[r][i];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    x[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc[t], qi, x[r][t], 0, 0, 0);
+            }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -310,8 +323,8 @@ struct Rows {
         for (int u = 0; u < D / 64; ++u)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bf16x8_t vc = operand(codes(m, v.w[0][2 * u], e), codes(m, v.w[0][2 * u + 1], e),
-                                            codes(m, v.w[1][2 * u], e), codes(m, v.w[1][2 * u + 1], e));
+                const bf16x8_t vc = operand(value_codes(m, v.w[0][2 * u], e), value_codes(m, v.w[0][2 * u + 1], e),
+                                            value_codes(m, v.w[1][2 * u], e), value_codes(m, v.w[1][2 * u + 1], e));
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
                     acc[r][4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vc, pb[r], acc[r][4 * u + e], 0, 0, 0);
@@ -335,7 +348,11 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < VI; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[r][i][e] = __builtin_fmaf(16.0f, acc[r][i][e] - MID * psum[r][e], pm[r]);
+                for (int e = 0; e < 4; ++e) {
+                    // elements 4 u of the lane's groups have the lowest codes; the middle of a row's range is code 7.5
+                    const float unit = i % 4 == 0 ? 128.0f : 16.0f, mid = 1.0f + 7.5f / unit;
+                    acc[r][i][e] = __builtin_fmaf(unit, acc[r][i][e] - mid * psum[r][e], pm[r]);
+                }
         }
     }
 };
@@ -539,15 +556,21 @@ __global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : RT == 2 && D == 64 ? 3 : 
         if (base < whole) {
             bool bad = here.bad[0] | here.bad[1];
             // The next step's keys are loaded once this step's are scores, its
-            // values once this step's are summed, into the same registers.
+            // values once this step's are summed, into the same registers.  A wave
+            // with scores goes first at the vector unit, so that the other's
+            // matrix products come to run beside its softmax: 301 us with it, 316
+            // without (chunks of 1024 tokens, 15627 keys); first with the
+            // keys' product too: 312 to 330.
             for (base += step; base < whole; base += step) {
                 pages.entries(base, page);
                 __builtin_amdgcn_sched_barrier(0);  // asked for here, looked at after the scores
                 R.scores(k, mask, kscale16, x, q_at);
                 here = pages.place(base, len, page);
                 k.load(a.c.k, a.c.k_meta, here, k_at, 16 * g);
+                __builtin_amdgcn_s_setprio(1);
                 R.rescale(x);
                 R.values(x, v, mask);
+                __builtin_amdgcn_s_setprio(0);
                 v.load(a.c.v, a.c.v_meta, here, v_at, 16 * g);
                 bad = bad | here.bad[0] | here.bad[1];
             }
@@ -566,9 +589,11 @@ __global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : RT == 2 && D == 64 ? 3 : 
             }
             loaded = false;
             R.scores(k, mask, kscale16, x, q_at);
+            __builtin_amdgcn_s_setprio(1);
             R.mask(x, v, here, base);
             R.rescale(x);
             R.values(x, v, mask);
+            __builtin_amdgcn_s_setprio(0);
         }
         R.finish();
         int tid2 = threadIdx.x;
