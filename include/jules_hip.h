@@ -365,8 +365,8 @@ int jules_hip_cross_entropy(const float* logits, const int32_t* targets,
  *   -127 .. 127 and scale fp32 [M] receives s = max|y| / 127 of each row: the A
  *   and scale_A of jules_hip_matmul_w8a8.  A row of zeros gives scale 0 and
  *   codes 0.  A row with a NaN or an infinity, or where x + residual or h *
- *   weight passes fp32, gives scale NaN and codes 0, so that every product of
- *   the row is NaN.
+ *   weight passes fp32 or is no number (a NaN in weight, an infinite one over
+ *   h = 0), gives scale NaN and codes 0, so that every product of the row is NaN.
  * Sums of squares are held in 64 bits.  Deterministic.  epsilon >= 0; with 0 a
  * row of zeros is NaN in fp32 and bf16, and the factor of one whose root mean
  * square is below 2^-127 passes fp32.  Pointers aligned to their elements.

@@ -58,6 +58,9 @@ __device__ __forceinline__ void store8(uint16_t* p, const f32x8_t& r) {
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(uint16_t* p, float v) { *p = (uint16_t)pack_bf16x2(v, 0.0f); }
 
+// the larger of two, NaN where one is NaN (fmaxf drops it): one instruction on gfx950
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // sum and largest of the group's values, the same order for every row.  The waves'
 // parts alternate between two places, so that one barrier a row is enough: a wave
 // that writes a place again has passed the barrier after which it was read.
@@ -70,7 +73,7 @@ __device__ __forceinline__ RowStats reduce_row(RowStats a, int turn) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         a.sum += __shfl_xor(a.sum, o);
-        a.top = fmaxf(a.top, __shfl_xor(a.top, o));
+        a.top = larger(a.top, __shfl_xor(a.top, o));
     }
     if constexpr (G > 64) {
         __shared__ RowStats parts[2][G / 64];
@@ -81,7 +84,7 @@ __device__ __forceinline__ RowStats reduce_row(RowStats a, int turn) {
 #pragma unroll
         for (int w = 1; w < G / 64; ++w) {
             a.sum += part[w].sum;
-            a.top = fmaxf(a.top, part[w].top);
+            a.top = larger(a.top, part[w].top);
         }
     }
     return a;
@@ -99,8 +102,8 @@ __device__ __forceinline__ RowFactors row_factors(RowStats a, int N, float eps) 
     // 127 / top overflows below 2^-121: tiny rows are lifted by a power of two
     f.lift = a.top < 0x1p-100f ? 0x1p100f : 1.0f;
     f.inv = a.top > 0.0f ? 127.0f / (a.top * f.lift) : 0.0f;
-    // a NaN or an infinity in the row, or h w past fp32: the sum of squares or
-    // the largest says so (fmaxf drops a NaN, the sum keeps it)
+    // a NaN or an infinity in the row: the sum of squares says so; h w past fp32, or
+    // no number for the weight's sake: the largest does
     f.bad = !(a.sum <= DBL_MAX) || !(a.top <= FLT_MAX);
     f.scale = f.bad ? __builtin_nanf("") : a.top * f.rstd / 127.0f;
     if (!f.bad && a.top == 0.0f) f.scale = 0.0f;
@@ -205,7 +208,7 @@ __device__ __forceinline__ void count(RowStats* s, const f32x8_t& h, const f32x8
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         s->sum = __builtin_fma((double)h.v[i], (double)h.v[i], s->sum);
-        s->top = fmaxf(s->top, fabsf(h.v[i] * w.v[i]));
+        s->top = larger(s->top, fabsf(h.v[i] * w.v[i]));
     }
 }
 

@@ -157,3 +157,31 @@ def test_stream_and_graph(dev):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(scale, want[1]) and torch.equal(kept, want[2])
+
+
+# a row count and width for each kernel: one and 4 waves a row, 1024 threads of 8,
+# 256 of 16 and of 32, 512 and 1024 of 32, and rows that are read twice
+KERNELS = [(5, 40), (5, 1000), (5, 3000), (600, 3001), (600, 5001), (5, 10000), (5, 20001), (3, 33000)]
+
+
+@pytest.mark.parametrize("M,N", KERNELS)
+@pytest.mark.parametrize("what", ["one NaN", "the last NaN", "all NaN", "infinite over zeros", "minus infinite"])
+def test_weights_that_are_no_numbers(dev, M, N, what):
+    """y is NaN or infinite somewhere, so int8 rows have no scale: NaN and codes 0, as
+    with a NaN in x.  fp32 rows are NaN or infinite in the weight's columns alone; the residual is as ever."""
+    case(f"add_rmsnorm {M}x{N} weight: {what}")
+    x, r, w = _operands(dev, M, N, f32, f32, 17)
+    j = {"one NaN": N // 2, "the last NaN": N - 1, "all NaN": slice(None), "infinite over zeros": N // 3, "minus infinite": 1}[what]
+    x[:, j], r[:, j] = (0.0, 0.0) if what == "infinite over zeros" else (x[:, j], r[:, j])
+    plain, h0 = ops.add_rmsnorm(x, r, w, EPS)
+    w[j] = float("inf") if "over" in what else float("-inf") if "minus" in what else float("nan")
+    q, s, h = ops.add_rmsnorm_int8(x, r, w, EPS)
+    y, h2 = ops.add_rmsnorm(x, r, w, EPS)
+    torch.cuda.synchronize()
+    assert torch.equal(h, h0) and torch.equal(h2, h0)
+    assert torch.isnan(s).all() and not q.any()
+    own = torch.zeros(N, dtype=torch.bool, device=dev)
+    own[j] = True
+    assert torch.equal(y[:, ~own], plain[:, ~own])
+    assert not torch.isfinite(y[:, own]).any()
+    assert torch.isnan(y[:, own]).all() == ("minus" not in what)
