@@ -451,8 +451,8 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  *   workspace: jules_hip_kv4_attention_workspace_size(...) bytes for the same
  *   arguments, 16-byte aligned, no initialisation, overwritten by every call;
  *   calls that overlap in time need separate ones (0 bytes: NULL will do).
- *   fp32 accumulation and softmax; probabilities times the value's scale are
- *   rounded to bf16.  Scores have to stay within fp32; values of a magnitude past
+ *   fp32 accumulation and softmax, whose error is the same at 2^18 keys as at
+ *   2^13; probabilities times the value's scale are rounded to bf16.  Scores have to stay within fp32; values of a magnitude past
  *   2^116 / keys may pass it in the sums (to infinity or NaN), below 2^-100 they
  *   lose precision.  Deterministic.  The calls may be captured in a graph.
  */

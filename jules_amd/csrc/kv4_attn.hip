@@ -18,6 +18,13 @@
 // the value's distance from the row's mean: the error is that of an attention
 // with bf16 probabilities.  (With MID = 1 it was 0.0049 of the output at 8192
 // keys of unit variance, with this one 0.0023; bf16 outputs alone are 0.0017.)
+// The accumulators hold sum P' C, of which MID sum P' is by far the larger part and
+// grows with the keys, and with it their roundings: taken out at the end alone, it
+// made errors of 0.007 of the output at 65536 keys a wave and 0.015 at 131072.  So
+// it is taken out every CENTER steps, of 1024 keys, and the error is 0.0024 from
+// there to 262144 keys: an instruction an accumulator and 32 steps (chunks over
+// 15627 keys 272 us for 270; with C = 1 + c/16 throughout, whose middle's part weighs
+// an eighth, 273 us too).
 //
 // One wave holds 16 rows (new tokens x heads of the group) times RT, and takes 32 keys
 // at a time.  Both products are transposed, S^T = K Q^T and O^T = V^T P^T: the
@@ -49,6 +56,7 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int KEYS = 32;     // keys of a step
 constexpr int WAVES = 4;     // waves of a workgroup
+constexpr int CENTER = 32;   // steps between two times that the middle's part leaves a wave's sums
 constexpr float GROW = 8.0f; // a row's reference grows when a score passes it by this (log2)
 
 struct AttnArgs {
@@ -337,9 +345,29 @@ struct Rows {
         for (int r = 0; r < RT; ++r) l[r] = __builtin_nanf("");
     }
 
+    // Elements 4 u of the lane's groups have the lowest codes; the middle of a row's
+    // range is code 7.5.
+    static __device__ __forceinline__ constexpr float unit(int i) { return i % 4 == 0 ? 128.0f : 16.0f; }
+    // The middle's part leaves `acc`: what stays of C is the code's distance from it,
+    // whose sum does not grow with the keys' number but with its root.
+    __device__ __forceinline__ void center() {
+        float mid[2] = {-(1.0f + 7.5f / 128.0f), -(1.0f + 7.5f / 16.0f)};
+        asm volatile("" : "+s"(mid[0]), "+s"(mid[1]));  // constants for here, not kept in registers
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+#pragma unroll
+            for (int i = 0; i < VI; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[r][i][e] = __builtin_fmaf(mid[i % 4 != 0], psum[r][e], acc[r][i][e]);
+            psum[r] = f32x4_t{0, 0, 0, 0};
+        }
+    }
+
     // what the lane's four parts of a row add up to; after it `acc` holds sums
     // of p V relative to `ref`, which is lower than any other's without a key
     __device__ __forceinline__ void finish() {
+        center();
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             ref[r] = limit[r] == GROW ? ref[r] : -FLT_MAX;
@@ -348,11 +376,7 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < VI; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // elements 4 u of the lane's groups have the lowest codes; the middle of a row's range is code 7.5
-                    const float unit = i % 4 == 0 ? 128.0f : 16.0f, mid = 1.0f + 7.5f / unit;
-                    acc[r][i][e] = __builtin_fmaf(unit, acc[r][i][e] - mid * psum[r][e], pm[r]);
-                }
+                for (int e = 0; e < 4; ++e) acc[r][i][e] = __builtin_fmaf(unit(i), acc[r][i][e], pm[r]);
         }
     }
 };
@@ -562,6 +586,7 @@ __global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : RT == 2 && D == 64 ? 3 : 
             // without (chunks of 1024 tokens, 15627 keys); first with the
             // keys' product too: 312 to 330.
             for (base += step; base < whole; base += step) {
+                if (base / step % CENTER == 0) R.center();  // here, where no scores or values wait in registers
                 pages.entries(base, page);
                 __builtin_amdgcn_sched_barrier(0);  // asked for here, looked at after the scores
                 R.scores(k, mask, kscale16, x, q_at);
