@@ -492,7 +492,8 @@ class KV4Cache:
     """A paged key/value cache held in 4 bits (jh_kv4_cache; layout in
     include/jules_hip.h): k uint8 [pages, heads, page_size, D/2], v uint8
     [pages, heads, page_size/4, 2*D], k_meta and v_meta bf16 [pages, heads,
-    page_size, 2] with each row's scale and minimum."""
+    page_size, 2] with each row's scale and minimum.  Its attributes cannot be
+    assigned: a larger pool is a new KV4Cache."""
 
     def __init__(self, k, v, k_meta, v_meta):
         _rank(k, "k", 4)
@@ -502,10 +503,21 @@ class KV4Cache:
         meta = (pages, heads, page_size, 2)
         _need(k_meta, "k_meta", (torch.bfloat16,), shape=meta)
         _need(v_meta, "v_meta", (torch.bfloat16,), shape=meta)
-        self.k, self.v, self.k_meta, self.v_meta = k, v, k_meta, v_meta
-        self.pages, self.heads, self.page_size, self.head_dim = pages, heads, page_size, 2 * half
-        c = JhKV4Cache(k.data_ptr(), v.data_ptr(), k_meta.data_ptr(), v_meta.data_ptr(), pages, page_size, heads, 2 * half)
-        self._ref = ctypes.byref(c)  # keeps c
+        c = JhKV4Cache(None, None, None, None, pages, page_size, heads, 2 * half)
+        self.__dict__.update(k=k, v=v, k_meta=k_meta, v_meta=v_meta, pages=pages, heads=heads, page_size=page_size,
+                             head_dim=2 * half, _struct=c, _ref=ctypes.byref(c),
+                             _numels=(k.numel(), v.numel(), k_meta.numel(), v_meta.numel()))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name} of a KV4Cache cannot be assigned: make a new KV4Cache")
+
+    def _at(self):
+        """jh_kv4_cache of the tensors where they lie now."""
+        k, v, k_meta, v_meta, c = self.k, self.v, self.k_meta, self.v_meta, self._struct
+        if (k.numel(), v.numel(), k_meta.numel(), v_meta.numel()) != self._numels:
+            raise ValueError("cache: the size of a tensor has changed")
+        c.k, c.v, c.k_meta, c.v_meta = k.data_ptr(), v.data_ptr(), k_meta.data_ptr(), v_meta.data_ptr()
+        return self._ref
 
     @classmethod
     def empty(cls, pages, heads, head_dim, page_size=64, device="cuda"):
@@ -565,7 +577,7 @@ def kv4_append(cache, k, v, table, lens, cu_q=None, max_q=None):
                 cache.v, cache.k_meta, cache.v_meta, table, lens, cu_q)
     kt, kh, _ = k.stride()
     vt, vh, _ = v.stride()
-    _call(k, lib().jules_hip_kv4_append, _DT[k.dtype], cache._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+    _call(k, lib().jules_hip_kv4_append, _DT[k.dtype], cache._at(), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
           table.data_ptr(), table.shape[1], lens.data_ptr(), _ptr(cu_q), batch, tokens, max_q)
 
 
@@ -584,7 +596,7 @@ def kv4_read(cache, table, lens, tokens, cu_q=None, max_q=None, dtype=torch.bflo
                 cache.k, cache.v, cache.k_meta, cache.v_meta, cu_q, k, v)
     k = lens.new_empty(shape, dtype=dtype) if k is None else k
     v = lens.new_empty(shape, dtype=dtype) if v is None else v
-    _call(lens, lib().jules_hip_kv4_read, _DT[dtype], cache._ref, k.data_ptr(), v.data_ptr(), table.data_ptr(),
+    _call(lens, lib().jules_hip_kv4_read, _DT[dtype], cache._at(), k.data_ptr(), v.data_ptr(), table.data_ptr(),
           table.shape[1], lens.data_ptr(), _ptr(cu_q), batch, tokens, max_q)
     return k, v
 
@@ -627,7 +639,7 @@ def kv4_attention(q, cache, table, lens, cu_q=None, max_q=None, max_len=None, sc
         if ws_bytes:
             workspace = q.new_empty((ws_bytes,), dtype=torch.uint8)
     qt, qh, _ = q.stride()
-    _call(q, lib().jules_hip_kv4_attention, float(scale), cache._ref, q.data_ptr(), qt, qh, out.data_ptr(), _ptr(lse),
+    _call(q, lib().jules_hip_kv4_attention, float(scale), cache._at(), q.data_ptr(), qt, qh, out.data_ptr(), _ptr(lse),
           heads_q, table.data_ptr(), table.shape[1], lens.data_ptr(), _ptr(cu_q), batch, tokens, max_q, int(max_len),
           _ptr(workspace), ws_bytes)
     return (out, lse) if return_lse else out

@@ -222,3 +222,41 @@ def test_kv4_checks():
     _raises(ops.kv4_attention, q, c, table, lens, out=q.float(), match="dtype")
     _raises(ops.kv4_attention, q, c, table, lens, lse=_t((6, 7)), match="elements")
     _raises(ops.kv4_attention, q, c, table, lens, workspace=_t((8, 8)).t()[:3], match="contiguous")
+
+
+def test_kv4_cache_tensors_are_fixed():
+    """Assigning another tensor (a larger pool), or the sizes, would leave the calls
+    with the old one's address: refused."""
+    c = _pool()
+    for name, value in dict(k=c.k.clone(), v=c.v.clone(), k_meta=c.k_meta.clone(), v_meta=c.v_meta.clone(), pages=9, heads=1,
+                            page_size=16, head_dim=128).items():
+        _raises(setattr, c, name, value, exc=AttributeError, match="new KV4Cache")
+        assert getattr(c, name) is not value
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_meta", "v_meta"])
+def test_kv4_cache_addresses_are_the_tensors(monkeypatch, name):
+    """A tensor whose memory has moved is passed where it now lies; one whose size
+    is another is refused."""
+    c, table, lens = _pool(), _t((3, 5), i32), _t((3,), i32)
+    k, q = _t((6, 2, 64), bf16), _t((6, 8, 64), bf16)
+    passed = []
+
+    def call(t, fn, *args):
+        passed.extend(a._obj for a in args if isinstance(getattr(a, "_obj", None), _lib.JhKV4Cache))
+
+    monkeypatch.setattr(ops, "_one_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_call", call)
+    calls = [lambda: ops.kv4_append(c, k, k, table, lens), lambda: ops.kv4_read(c, table, lens, 6),
+             lambda: ops.kv4_attention(q, c, table, lens)]
+    t = getattr(c, name)
+    held = [t.data]  # the old memory stays, so that the new is elsewhere
+    for fn in calls:
+        t.data = t.data.clone()
+        held.append(t.data)
+        fn()
+        assert getattr(passed.pop(), name) == t.data_ptr() and not passed
+    t.data = t.data[:3].clone()
+    for fn in calls:
+        _raises(fn, match="size")
+    assert not passed
