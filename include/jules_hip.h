@@ -450,7 +450,9 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  *   tokens * heads_q <= 2^30.
  *   workspace: jules_hip_kv4_attention_workspace_size(...) bytes for the same
  *   arguments, 16-byte aligned, no initialisation, overwritten by every call;
- *   calls that overlap in time need separate ones (0 bytes: NULL will do).
+ *   calls that overlap in time need separate ones (0 bytes: NULL will do).  At
+ *   most 256 MiB: up to 35 MB where max_q is right and tokens holds no padding,
+ *   more where max_q is too small.
  *   fp32 accumulation and softmax, whose error is the same at 2^18 keys as at
  *   2^13; probabilities times the value's scale are rounded to bf16.  Scores have to stay within fp32; values of a magnitude past
  *   2^116 / keys may pass it in the sums (to infinity or NaN), below 2^-100 they

@@ -691,6 +691,10 @@ struct Plan {
 // in 64 splits, 27 + 5 in 48, 24 + 6 in 96, 21 + 7 in 128; 15627 keys of 3022
 // new tokens: 315 us whole, 382 + 32 in 2).  A split costs a second launch too:
 // none below 1024 keys (1000 keys: 10 us whole, 7 + 3 in 4 splits).
+// With a max_q of the longest sequence the splits' sums are 35 MB at most.  One that is
+// too small (a single token's, for a prompt's rows) would ask for splits of rows
+// that fill the card by themselves, and for gigabytes: no more than WORKSPACE.
+constexpr int64_t WORKSPACE = int64_t(256) << 20;
 Plan plan(int D, int batch, int tokens, int heads_kv, int group, int max_q, int max_len) {
     Plan p;
     const int64_t rows = (int64_t)std::max(1, std::min(max_q, tokens)) * group;
@@ -701,7 +705,8 @@ Plan plan(int D, int batch, int tokens, int heads_kv, int group, int max_q, int 
     p.row_blocks = (int)std::min((int64_t)std::max(1, (1 << 22) / heads_kv), (rows + brows - 1) / brows);
     const int64_t groups = (int64_t)batch * heads_kv * p.row_blocks;
     const int full = p.rt == 1 ? 2048 : p.rt == 2 ? p.share ? 1024 : 512 : 256;
-    const int64_t want = std::max((int64_t)1, full / groups);
+    const int64_t each = (int64_t)tokens * heads_kv * group * (D + 2) * (int64_t)sizeof(float);
+    const int64_t want = std::max((int64_t)1, std::min(full / groups, WORKSPACE / each));
     const int unit = KEYS * WAVES;
     int64_t chunk = std::max((int64_t)1024, ((int64_t)max_len + want - 1) / want);
     chunk = (chunk + unit - 1) / unit * unit;

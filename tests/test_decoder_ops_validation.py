@@ -260,3 +260,20 @@ def test_kv4_cache_addresses_are_the_tensors(monkeypatch, name):
     for fn in calls:
         _raises(fn, match="size")
     assert not passed
+
+
+def test_kv4_workspace_of_wrong_hints():
+    """A max_q that is too small asks for many splits of many rows: bounded, and of
+    what right hints ask for nothing is taken."""
+    f = _lib.lib().jules_hip_kv4_attention_workspace_size
+    most = 256 << 20
+    assert f(1, 8192, 32, 8, 128, 1, 131072) <= most
+    for batch in (1, 2, 7, 64, 1000):
+        for tokens in (batch, 100 * batch, 1 << 20, (1 << 30) // 64):
+            for heads_q, heads, D in ((64, 8, 128), (8, 8, 64), (64, 1, 64)):
+                for max_q in (0, 1, 5, 20, 1000, tokens):
+                    for max_len in (1, 5000, 131072, 2**31 - 1):
+                        assert f(batch, tokens, heads_q, heads, D, max_q, max_len) <= most
+    # single tokens of 64 sequences of 8 heads of 8 in 4 splits, 5 drafted of one in 64
+    assert f(64, 64, 64, 8, 128, 1, 8192) == 64 * 64 * 4 * 130 * 4
+    assert f(1, 5, 32, 4, 64, 5, 131072) == 5 * 32 * 64 * 66 * 4

@@ -500,6 +500,15 @@ def test_offsets_past_32_bits(dev):
     assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
+def test_hints_that_disagree(dev):
+    """A prompt's rows with the hints of one token over a long text: more splits
+    would not fit the workspace than are taken."""
+    p = _problem(dev, 64, 32, 2, 4, [1500], [1000], seed=16)
+    case("kv4 attention of 1000 tokens, max_q=1 max_len=131072")
+    assert 0 < ops.lib().jules_hip_kv4_attention_workspace_size(1, 1000, 8, 2, 64, 1, 131072) <= 256 << 20
+    _run(p, max_q=1, max_len=131072)
+
+
 # ---- together ----------------------------------------------------------------------------
 
 
