@@ -185,3 +185,41 @@ def test_weights_that_are_no_numbers(dev, M, N, what):
     assert torch.equal(y[:, ~own], plain[:, ~own])
     assert not torch.isfinite(y[:, own]).any()
     assert torch.isnan(y[:, own]).all() == ("minus" not in what)
+
+
+def _check_on(x, r, w, y, q, s, h):
+    """_check with the formula on the device, for many rows, a block of them at a time."""
+    for i in range(0, x.shape[0], 512):
+        at = slice(i, i + 512)
+        h64 = x[at].double() + (0.0 if r is None else r[at].double())
+        y64 = h64 / torch.sqrt(h64.square().mean(-1, keepdim=True) + EPS) * w.double()
+        s64 = y64.abs().amax(-1) / 127.0
+        if r is not None:
+            step = F32 + (BF16 if r.dtype == bf16 else 0)
+            assert ((h[at].double() - h64).abs() <= 1.01 * step * h64.abs()).all(), i
+        step = 6 * F32 + (BF16 if y.dtype == bf16 else 0)
+        assert ((y[at].double() - y64).abs() <= 1.01 * step * y64.abs()).all(), i
+        assert ((s[at].double() - s64).abs() <= 8 * F32 * s64).all(), i
+        assert ((q[at].double() - y64 / s64[:, None]).abs() <= 0.5 + 8 * 127 * F32).all(), i
+
+
+@pytest.mark.parametrize("M,N,xt,rt", [
+    # widths at the borders of the kernels for more than 512 rows
+    (513, 2049, bf16, bf16), (513, 4096, f32, f32), (513, 4097, bf16, f32), (513, 5001, f32, bf16), (513, 8192, bf16, bf16),
+    (512, 8192, f32, bf16),
+    # more rows than are resident: each block goes on to a third and a fourth
+    (33000, 200, bf16, f32), (6200, 513, f32, f32), (3100, 2050, bf16, bf16), (3100, 5001, f32, None), (1550, 8193, bf16, f32),
+    (1550, 16385, bf16, None), (4100, 32769, bf16, None)])
+def test_rows_beyond_the_blocks(dev, M, N, xt, rt):
+    """Rows of sizes a million apart side by side: what a row is scaled by is its own."""
+    case(f"add_rmsnorm {M}x{N} {xt} {rt}")
+    g = torch.Generator(dev).manual_seed(M + N)
+    size = 10.0 ** (6.0 * torch.rand(M, 1, generator=g, device=dev) - 3.0)
+    x = (size * torch.randn(M, N, generator=g, device=dev)).to(xt)
+    r = None if rt is None else (2.0 * size * torch.randn(M, N, generator=g, device=dev)).to(rt)
+    w = 1.0 + 0.3 * torch.randn(N, generator=g, device=dev)
+    y, h = ops.add_rmsnorm(x, r, w, EPS)
+    q, s, h2 = ops.add_rmsnorm_int8(x, r, w, EPS)
+    torch.cuda.synchronize()
+    assert r is None or torch.equal(h, h2)
+    _check_on(x, r, w, y, q, s, h)

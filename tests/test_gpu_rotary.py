@@ -176,3 +176,38 @@ def test_empty(dev):
     freq, _ = ops.rotary_frequencies(64, device=dev)
     pos = torch.zeros(1, 0, dtype=torch.int32, device=dev)
     assert ops.rotary(torch.empty(3, 0, 64, device=dev), pos, freq).shape == (3, 0, 64)
+
+
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+@pytest.mark.parametrize("B,S,H,D,R,axes", [
+    (2, 33001, 1, 128, 128, 1), (2, 8003, 3, 128, 64, 2), (2, 1003, 40, 128, 128, 3), (3, 9001, 5, 7, 6, 1),
+    (2, 4101, 1, 1024, 1024, 2), (5, 701, 8, 256, 128, 1)])
+def test_large(dev, B, S, H, D, R, axes, pairing):
+    """Enough work for several tokens a block: numbers of tokens that do not divide
+    by a block's, so that blocks cross from one batch to the next and the last is
+    ragged; out of place from a fused projection, and in place."""
+    case(f"rotary {B}x{H}x{S}x{D} R={R} {pairing}")
+    g = torch.Generator(dev).manual_seed(S)
+    freq, axis = ops.rotary_frequencies(R, None if axes == 1 else (R // 2 - axes + 1,) + (1,) * (axes - 1), device=dev)
+    pos = torch.randint(0, 5000, (axes, B, S), generator=g, device=dev).to(torch.int32)
+    x = torch.randn(B, S, H + 1, D, generator=g, device=dev).to(bf16)[:, :, :H].transpose(1, 2)
+    a = pos.double()[axis.long()] if axis is not None else pos.double().expand(R // 2, B, S)
+    a = (a * freq[:, None, None]).permute(1, 2, 0)[:, None]
+    i = torch.arange(R // 2, device=dev) * (1 if pairing == "half" else 2)
+    j = i + (R // 2 if pairing == "half" else 1)
+    u, v = x[..., i].double(), x[..., j].double()
+    want, bound = x.double(), torch.zeros(x.shape, dtype=torch.float64, device=dev)
+    want[..., i], want[..., j] = u * a.cos() - v * a.sin(), u * a.sin() + v * a.cos()
+    # as rotary_bound; the angle here, of up to 5000 radians, is 2^-40 off
+    bound[..., i] = bound[..., j] = (u.abs() + v.abs()) * (3 * 2.0**-23 + 3 * F32 + 2.0**-40)
+
+    def check(y, step):
+        assert ((y.double() - want).abs() <= 1.01 * (bound + step * (want.abs() + bound))).all()
+        assert torch.equal(y[..., R:], x[..., R:].to(y.dtype))
+
+    y = ops.rotary(x, pos, freq, axis, pairing=pairing)
+    check(y, BF16)
+    check(ops.rotary(x, pos, freq, axis, pairing=pairing, dtype=f32), F32)
+    kept = x.clone(memory_format=torch.preserve_format)
+    ops.rotary(kept, pos, freq, axis, pairing=pairing, out=kept)
+    assert torch.equal(kept, y)
