@@ -492,8 +492,8 @@ class KV4Cache:
     """A paged key/value cache held in 4 bits (jh_kv4_cache; layout in
     include/jules_hip.h): k uint8 [pages, heads, page_size, D/2], v uint8
     [pages, heads, page_size/4, 2*D], k_meta and v_meta bf16 [pages, heads,
-    page_size, 2] with each row's scale and minimum.  Its attributes cannot be
-    assigned: a larger pool is a new KV4Cache."""
+    page_size, 2] with each row's scale and minimum.  These and the sizes
+    cannot be assigned: a larger pool is a new KV4Cache."""
 
     def __init__(self, k, v, k_meta, v_meta):
         _rank(k, "k", 4)
@@ -505,11 +505,16 @@ class KV4Cache:
         _need(v_meta, "v_meta", (torch.bfloat16,), shape=meta)
         c = JhKV4Cache(None, None, None, None, pages, page_size, heads, 2 * half)
         self.__dict__.update(k=k, v=v, k_meta=k_meta, v_meta=v_meta, pages=pages, heads=heads, page_size=page_size,
-                             head_dim=2 * half, _struct=c, _ref=ctypes.byref(c),
-                             _numels=(k.numel(), v.numel(), k_meta.numel(), v_meta.numel()))
+                             head_dim=2 * half)
+        self._struct, self._ref = c, ctypes.byref(c)
+        self._numels = (k.numel(), v.numel(), k_meta.numel(), v_meta.numel())
+
+    _FIXED = frozenset(("k", "v", "k_meta", "v_meta", "pages", "heads", "page_size", "head_dim"))
 
     def __setattr__(self, name, value):
-        raise AttributeError(f"{name} of a KV4Cache cannot be assigned: make a new KV4Cache")
+        if name in self._FIXED:
+            raise AttributeError(f"{name} of a KV4Cache cannot be assigned: make a new KV4Cache")
+        super().__setattr__(name, value)
 
     def _at(self):
         """jh_kv4_cache of the tensors where they lie now."""

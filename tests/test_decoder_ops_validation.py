@@ -234,6 +234,18 @@ def test_kv4_cache_tensors_are_fixed():
         assert getattr(c, name) is not value
 
 
+def test_kv4_cache_takes_attributes_of_its_user():
+    class Layer(ops.KV4Cache):
+        def __init__(self, *tensors, index):
+            self.index = index
+            super().__init__(*tensors)
+
+    c = _pool()
+    c.owner = "layer 3"
+    layer = Layer(c.k, c.v, c.k_meta, c.v_meta, index=3)
+    assert c.owner == "layer 3" and layer.index == 3 and layer.pages == 4
+
+
 @pytest.mark.parametrize("name", ["k", "v", "k_meta", "v_meta"])
 def test_kv4_cache_addresses_are_the_tensors(monkeypatch, name):
     """A tensor whose memory has moved is passed where it now lies; one whose size
