@@ -369,7 +369,8 @@ int jules_hip_cross_entropy(const float* logits, const int32_t* targets,
  *   h = 0), gives scale NaN and codes 0, so that every product of the row is NaN.
  * Sums of squares are held in 64 bits.  Deterministic.  epsilon >= 0; with 0 a
  * row of zeros is NaN in fp32 and bf16, and the factor of one whose root mean
- * square is below 2^-127 passes fp32.  Pointers aligned to their elements.
+ * square is below 2^-127 passes fp32.  Pointers aligned to their elements;
+ * overlaps other than the two named are not allowed.
  */
 int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const void* x,
                           const void* residual, const float* weight, void* residual_out,
@@ -384,7 +385,7 @@ int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const 
  * from that of out.  No counterpart in the reference: the positions of
  * jules_hip_flash_attn_fwd's or jules_hip_kv4_attention's queries and keys.
  * x_dtype, out_dtype: JH_F32 or JH_BF16, each by itself; arithmetic in fp32,
- * angles in fp64 (less than 10^-6 off at any int32 position).
+ * angles in fp64 (with |inv_freq| <= 1 less than 10^-6 off at any int32 position).
  * x_strides, out_strides: host arrays of 3, the elements between two batches,
  * heads and tokens; the D elements of a head lie side by side.  x may have
  * strides of 0; out's must keep its elements apart (JH_ERR_ARG otherwise).  out
@@ -423,7 +424,9 @@ int jules_hip_rotary(int x_dtype, int out_dtype, int pairing, int inverse, const
  *           outside cu_q[0] .. cu_q[batch] - 1 are not touched.  NULL: max_q rows
  *           each, tokens = batch * max_q.
  *   max_q   the largest number of new tokens of a sequence.  With cu_q it is a
- *           hint: a wrong one costs time, not results.
+ *           hint: a wrong one costs time and workspace, not results.  It decides the
+ *           attention's tile for the whole batch, so that single tokens beside a
+ *           chunk take the chunk's.
  * These arrays are on the device, so their contents are not checked by a status;
  * whatever they hold, nothing outside the arrays is read or written.  Page
  * numbers outside [0, num_pages) and positions past max_pages * page_size are no pages:

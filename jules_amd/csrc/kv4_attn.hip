@@ -11,7 +11,8 @@
 //   sum p V = 16 (sum P' C - MID sum P') + sum p (m_v + 7.5 s_v),
 //   P' = bf16(p s_v),  MID = 1 + 7.5/16
 // (the values' lowest codes of each 16 bits are not shifted, and C = 1 + c/128, with
-// 128 for 16: a sixteenth of the shifts less, 316 us for 322 over 15627 keys).
+// 128 for 16: a sixteenth of the shifts less, 272 us for 273 over 15627 keys of chunks,
+// 1291 for 1304 over 65536).
 // -sum q is the accumulator that the first product starts from.  P' is rounded
 // once and both of its sums take the rounded number, so what its rounding is
 // multiplied by is the code's distance from the middle of the row's range, about
@@ -23,8 +24,7 @@
 // made errors of 0.007 of the output at 65536 keys a wave and 0.015 at 131072.  So
 // it is taken out every CENTER steps, of 1024 keys, and the error is 0.0024 from
 // there to 262144 keys: an instruction an accumulator and 32 steps (chunks over
-// 15627 keys 272 us for 270; with C = 1 + c/16 throughout, whose middle's part weighs
-// an eighth, 273 us too).
+// 15627 keys 272 us for 270).
 //
 // One wave holds 16 rows (new tokens x heads of the group) times RT, and takes 32 keys
 // at a time.  Both products are transposed, S^T = K Q^T and O^T = V^T P^T: the
@@ -33,12 +33,13 @@
 // needs no exchange between lanes but for the row's maximum when it grows.
 // Keys and values go from memory to the matrix cores through registers alone.
 //
-// Bound, one new token and 8 heads a key head, 64 sequences of 8192 keys: HBM, 4.9
-// TB/s (116 us); of 4096: 4.5 TB/s (64 us).  A short text of one sequence: what one
-// CU takes in, 27 bytes/ns (1000 keys 10 us, 128 keys 5 us, 1 key 5 us).  From 32 rows on:
+// Bound, one new token and 8 heads a key head, 64 sequences of 8192 keys: HBM, 5.1
+// TB/s (112 us with the join); of 4096: 4.7 TB/s (61 us).  A short text of one sequence: what one
+// CU takes in, 27 bytes/ns (1000 keys 10.5 us, 128 keys 5.3 us, 1 key 5.4 us).  From 32 rows on:
 // vector instructions, a score's scale, exponential and rounding and a code's shift
 // and and-or, about 290 beside 34 of the matrix cores' for 32 rows and 32 keys: chunks
-// of 1024 tokens over 8192 keys, 8 sequences, 32 heads, D 128, 743 TFLOP/s, D 64 670.
+// of 1024 tokens over 8192 keys, 8 sequences, 32 heads, D 128, 780 to 810 TFLOP/s on
+// two cards, D 64 680.  What follows names both sides as they were when compared.
 // Keys and values converted once for a workgroup, through LDS, were no faster (314
 // us to 311 over 15627 keys; D 64 1034 to 829): the conversion saved went into
 // writing and reading.  Keys as bytes, of which e4m3 holds 0 to 15 exactly, and q as
@@ -582,8 +583,8 @@ __global__ __launch_bounds__(64 * WAVES, RT == 1 ? 4 : RT == 2 && D == 64 ? 3 : 
             // The next step's keys are loaded once this step's are scores, its
             // values once this step's are summed, into the same registers.  A wave
             // with scores goes first at the vector unit, so that the other's
-            // matrix products come to run beside its softmax: 301 us with it, 316
-            // without (chunks of 1024 tokens, 15627 keys); first with the
+            // matrix products come to run beside its softmax: 277 us with it, 294
+            // without (chunks of 1024 tokens, 15627 keys; D 64, 65536 keys: 757, 819); first with the
             // keys' product too: 312 to 330.
             for (base += step; base < whole; base += step) {
                 if (base / step % CENTER == 0) R.center();  // here, where no scores or values wait in registers

@@ -14,8 +14,8 @@
 // of 8 values, so its minimum and maximum are four or three exchanges within 16
 // lanes; a wave has neighbouring tokens of one head, whose value codes share the
 // 8-byte groups of 4 tokens.  Ragged prompts of up to 2048 tokens, 16 sequences, 8
-// heads of 128, fp32: 40 us, 4.4 TB/s in, and 20 us, 5.0 TB/s, for the read of the
-// same rows; one token each of 64 sequences: 4.7 and 3.2 us.
+// heads of 128, fp32: 37 us, 4.7 TB/s, and 19 us, 5.2 TB/s, for the read of the
+// same rows; one token each of 64 sequences: 4.3 and 2.9 us.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>

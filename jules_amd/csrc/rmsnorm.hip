@@ -285,11 +285,11 @@ void launch(const NormArgs& a, int blocks, hipStream_t s) {
 }
 
 // Few threads with many elements each keep the most rows in flight: 8192 rows of
-// 8192 bf16 take 92 us (5.1 TB/s) with 256 threads of 32 elements, 165 us with
+// 8192 bf16 take 87 us (5.4 TB/s) with 256 threads of 32 elements, 165 us with
 // 1024 of 8, of which a CU holds one row at a time.  Up to two rows a CU 1024
-// threads are the faster, a row being done sooner (8 rows: 5.6 us).  Four blocks a
+// threads are the faster, a row being done sooner (8 rows: 5.2 us).  Four blocks a
 // CU, as many as are resident, read the weight once each; a block a row: 98 us.
-// Rows of odd width, at 4-byte addresses: 4.1 TB/s (1999 of 5001 fp32, 39 us).
+// Rows of odd width, at 4-byte addresses: 4.8 TB/s (1999 of 5001 fp32, 34 us).
 template <typename XT, typename RT, bool RES>
 hipError_t launch(const NormArgs& a, hipStream_t s) {
     if (a.N <= 512)

@@ -10,9 +10,9 @@
 // Bound by HBM: every element is read and written once.  An angle is needed
 // once a token and pair but used by all heads, so a block first puts the
 // cosines and sines of its tokens into LDS.  The angle is formed in fp64 and
-// reduced to a fraction of a turn there: at position 10^6 an fp32 angle is off
-// by 0.03, this one by less than 10^-9.  bf16, 2 x 8000 tokens, 40 heads of 128:
-// 62 us, 5.3 TB/s; 8 x 4096, 32 heads of 128 with half of each rotated: 107 us,
+// reduced to a fraction of a turn there, which is then rounded to fp32: at position
+// 10^6 an fp32 angle is off by 0.03, this one by 10^-7.  bf16, 2 x 8000 tokens, 40 heads of 128:
+// 64 us, 5.1 TB/s; 8 x 4096, 32 heads of 128 with half of each rotated: 107 us,
 // 5.0 TB/s, a copy's rate; 8 tokens: 3.4 us.
 #include <algorithm>
 
@@ -191,8 +191,10 @@ hipError_t launch_rotary(int x_dtype, int out_dtype, bool half, bool inverse, co
     if (a.tokens * H * pieces < (int64_t)2048 * THREADS)
         a.hc = std::min(H, lanes);  // few tokens: one step a thread, on as many blocks as there are
     else
-        a.tb = std::max(1, std::min(16, 1024 / std::min(1024, H * pieces)));  // at least four steps a thread
-    // fewer than 2^24 blocks of 256 threads (at most 2^27 tokens)
+        // up to four steps a thread, and 16 tokens: with R = 1024 their angles take the 64 KB of LDS that a
+        // launch gets unasked
+        a.tb = std::max(1, std::min(16, 1024 / std::min(1024, H * pieces)));
+    // fewer than 2^24 blocks of 256 threads (at most 2^27 tokens, so tb stays within 16)
     while ((a.tokens + a.tb - 1) / a.tb >= (1 << 24)) a.tb *= 2;
     if (x_dtype == JH_F32)
         return out_dtype == JH_F32 ? launch<float, float>(half, a, v, s) : launch<float, uint16_t>(half, a, v, s);

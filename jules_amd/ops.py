@@ -569,7 +569,9 @@ def kv4_append(cache, k, v, table, lens, cu_q=None, max_q=None):
     last is 1.  table int32 [batch, max_pages]: the pages of each sequence;
     lens int32 [batch]: tokens of each, the new ones among them; rows cu_q[b]
     .. cu_q[b+1] - 1 are the last ones of sequence b (None: the same number
-    each).  max_q: the largest number of new rows, where the caller knows it."""
+    each).  max_q: the largest number of new rows of a sequence, where the caller
+    knows it; left out beside cu_q it counts as all of them, and the call starts
+    that many workgroups for every sequence."""
     tail = (cache.heads, cache.head_dim) if isinstance(cache, KV4Cache) else (0, 0)
     if tail != (0, 0):
         _kv4_rows(k, "k", _REAL, tail)
@@ -612,8 +614,8 @@ def kv4_attention(q, cache, table, lens, cu_q=None, max_q=None, max_len=None, sc
     counterpart in the reference): q bf16 [tokens, heads_q, D], heads_q a
     multiple of the cache's heads, each token over its sequence's keys up to
     its own position; table, lens, cu_q and max_q as in kv4_append, which comes
-    before.  max_len: the largest of lens, where the caller knows it (None: what
-    the table has room for).  scale defaults to 1/sqrtf(D).  Returns out
+    before (max_q also decides the tile, one for the batch).  max_len: the largest
+    of lens, where the caller knows it (None: what the table has room for).  scale defaults to 1/sqrtf(D).  Returns out
     [tokens, heads_q, D], or (out, lse [tokens, heads_q]) with return_lse."""
     if isinstance(cache, KV4Cache):
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
