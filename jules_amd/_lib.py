@@ -19,6 +19,7 @@ STATUS = {0: "JH_OK", 1: "JH_ERR_NULL", 2: "JH_ERR_SHAPE", 3: "JH_ERR_DTYPE",
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
 _i64 = ctypes.c_int64
+_u64 = ctypes.c_uint64
 _f32 = ctypes.c_float
 _size = ctypes.c_size_t
 
@@ -71,6 +72,13 @@ SIGNATURES = {
     "jules_hip_cross_entropy_workspace_size": (_size, [_int]),
     "jules_hip_cross_entropy": (_int, [_vp, _vp, _vp, _vp, _int, _int, _vp, _size, _vp]),
     "jules_hip_add_rmsnorm": (_int, [_int, _int, _int] + [_vp] * 6 + [_int, _int, _f32, _vp]),
+    "jules_hip_dropout": (_int, [_int, _int, _f32, _vp, _u64] + [_vp] * 3 + [_int, _int, _vp]),
+    "jules_hip_add_layernorm": (_int, [_int] * 3 + [_f32, _vp, _u64] + [_vp] * 8 + [_int, _int, _f32, _vp]),
+    "jules_hip_add_layernorm_bwd_workspace_size": (_size, [_int, _int]),
+    "jules_hip_add_layernorm_bwd": (_int, [_int, _int, _f32, _vp, _u64] + [_vp] * 10 + [_int, _int, _vp, _size, _vp]),
+    "jules_hip_token_logprobs_workspace_size": (_size, [_int] * 3),
+    "jules_hip_token_logprobs": (_int, [_int, _vp, _i64, _f32] + [_vp] * 4 + [_int, _vp, _vp, _int, _int, _vp, _size, _vp]),
+    "jules_hip_token_logprobs_bwd": (_int, [_int, _vp, _i64, _f32] + [_vp] * 6 + [_i64, _int, _int, _vp]),
     "jules_hip_rotary": (_int, [_int] * 4 + [_vp, ctypes.POINTER(_i64), _vp, ctypes.POINTER(_i64)] + [_vp] * 3 +
                          [_int] * 6 + [_vp]),
     "jules_hip_kv4_append": (_int, [_int, ctypes.POINTER(JhKV4Cache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _int,

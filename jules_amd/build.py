@@ -28,7 +28,7 @@ DEVICE = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-p
           "-munsafe-fp-atomics"]
 
 SOURCES = ["gemm_f32.hip", "gemm_f32_tile.hip", "gemm_f32_tile_t.hip", "gemm_bf16.hip", "flash_fwd.hip", "flash_bwd.hip", "flash_bwd_dq.hip", "flash_pad.hip", "w8a16.hip", "w8a16_packed.hip", "matmul_int8.hip",
-           "rowops.hip", "rmsnorm.hip", "rotary.hip", "kv4_cache.hip", "kv4_attn.hip", "mlp.hip", "calib.hip", "pjrt_ops.hip", "scratch.hip", "capi.cpp", "kernel_shims.cpp",
+           "rowops.hip", "rmsnorm.hip", "layernorm.hip", "dropout.hip", "logprobs.hip", "rotary.hip", "kv4_cache.hip", "kv4_attn.hip", "mlp.hip", "calib.hip", "pjrt_ops.hip", "scratch.hip", "capi.cpp", "kernel_shims.cpp",
            "pjrt.cpp"]
 
 

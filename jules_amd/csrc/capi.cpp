@@ -487,6 +487,154 @@ int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const 
                      "add_rmsnorm launch");
 }
 
+// A dropout's arguments as the kernels take them.  p that rounds to 0: nothing is
+// dropped, and rng is not looked at.
+static int drop_args(const char* who, float p, const int64_t* rng, uint64_t offset, jh::Dropout* d) {
+    if (!(p >= 0.0f && p < 1.0f)) return fail(JH_ERR_ARG, "%s: p %g (0 <= p < 1)", who, p);
+    const uint32_t t = (uint32_t)std::nearbyint((double)p * 65536.0);
+    if (t == 65536) return fail(JH_ERR_ARG, "%s: p %.9g rounds to 1", who, p);
+    if (t && !aligned(rng, 8)) return fail(JH_ERR_ALIGN, "%s: rng must be 8-byte aligned", who);
+    *d = {rng, offset, t, (float)(65536.0 / (65536 - t))};
+    return JH_OK;
+}
+
+static bool real_dtype(int t) { return t == JH_F32 || t == JH_BF16; }
+static size_t real_size(int t) { return t == JH_F32 ? 4 : 2; }
+
+int jules_hip_dropout(int x_dtype, int out_dtype, float p, const int64_t* rng, uint64_t offset, const void* x,
+                      const void* residual, void* out, int M, int N, void* stream) {
+    if (!real_dtype(x_dtype) || !real_dtype(out_dtype)) return fail(JH_ERR_DTYPE, "dropout: dtypes %d %d", x_dtype, out_dtype);
+    int st = row_shape("dropout", M, N);
+    if (st != JH_OK) return st;
+    jh::Dropout d;
+    st = drop_args("dropout", p, rng, offset, &d);
+    if (st != JH_OK) return st;
+    if (M == 0 || N == 0) return JH_OK;
+    if (!x || !out || (d.t && !rng)) return fail(JH_ERR_NULL, "dropout: null x, out or rng");
+    if (!aligned(x, real_size(x_dtype)) || !aligned(out, real_size(out_dtype)) || !aligned(residual, real_size(out_dtype)))
+        return fail(JH_ERR_ALIGN, "dropout: pointers must be aligned to their elements");
+    return check_hip(jh::launch_dropout(x_dtype, out_dtype, d, x, residual, out, M, N, static_cast<hipStream_t>(stream)),
+                     "dropout launch");
+}
+
+int jules_hip_add_layernorm(int x_dtype, int h_dtype, int out_dtype, float p, const int64_t* rng, uint64_t offset,
+                            const void* x, const void* residual, const float* gamma, const float* beta, void* h, void* out,
+                            float* mean, float* rstd, int M, int N, float epsilon, void* stream) {
+    if (!real_dtype(x_dtype) || !real_dtype(out_dtype) || ((residual || h) && !real_dtype(h_dtype)))
+        return fail(JH_ERR_DTYPE, "add_layernorm: dtypes %d %d %d", x_dtype, h_dtype, out_dtype);
+    int st = row_shape("add_layernorm", M, N);
+    if (st != JH_OK) return st;
+    if (!(std::isfinite(epsilon) && epsilon >= 0.0f)) return fail(JH_ERR_ARG, "add_layernorm: epsilon %g", epsilon);
+    jh::Dropout d;
+    st = drop_args("add_layernorm", p, rng, offset, &d);
+    if (st != JH_OK) return st;
+    if (M == 0 || N == 0) return JH_OK;
+    if (!x || !out || (d.t && !rng)) return fail(JH_ERR_NULL, "add_layernorm: null x, out or rng");
+    if (!aligned(x, real_size(x_dtype)) || !aligned(out, real_size(out_dtype)) || !aligned(gamma, 4) || !aligned(beta, 4) ||
+        !aligned(mean, 4) || !aligned(rstd, 4) ||
+        ((residual || h) && (!aligned(residual, real_size(h_dtype)) || !aligned(h, real_size(h_dtype)))))
+        return fail(JH_ERR_ALIGN, "add_layernorm: pointers must be aligned to their elements");
+    return check_hip(jh::launch_add_layernorm(x_dtype, h_dtype, out_dtype, d, x, residual, gamma, beta, h, out, mean, rstd, M, N,
+                                              epsilon, static_cast<hipStream_t>(stream)),
+                     "add_layernorm launch");
+}
+
+size_t jules_hip_add_layernorm_bwd_workspace_size(int M, int N) {
+    if (M <= 0 || N <= 0 || (int64_t)M * N > kMaxElems) return 0;
+    return jh::add_layernorm_bwd_workspace_size(M, N);
+}
+
+int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t* rng, uint64_t offset, const void* dy,
+                                const void* h, const void* dh, const float* mean, const float* rstd, const float* gamma,
+                                void* dx, void* dresidual, float* dgamma, float* dbeta, int M, int N, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    if (!real_dtype(x_dtype) || !real_dtype(h_dtype))
+        return fail(JH_ERR_DTYPE, "add_layernorm_bwd: dtypes %d %d", x_dtype, h_dtype);
+    int st = row_shape("add_layernorm_bwd", M, N);
+    if (st != JH_OK) return st;
+    jh::Dropout d;
+    st = drop_args("add_layernorm_bwd", p, rng, offset, &d);
+    if (st != JH_OK) return st;
+    if (N == 0) return JH_OK;
+    if (!aligned(dgamma, 4) || !aligned(dbeta, 4))
+        return fail(JH_ERR_ALIGN, "add_layernorm_bwd: pointers must be aligned to their elements");
+    if (M > 0) {
+        if (!dy || !h || !mean || !rstd || (d.t && !rng))
+            return fail(JH_ERR_NULL, "add_layernorm_bwd: null dy, h, mean, rstd or rng");
+        if (!aligned(dy, real_size(x_dtype)) || !aligned(dx, real_size(x_dtype)) || !aligned(h, real_size(h_dtype)) ||
+            !aligned(dh, real_size(h_dtype)) || !aligned(dresidual, real_size(h_dtype)) || !aligned(mean, 4) ||
+            !aligned(rstd, 4) || !aligned(gamma, 4))
+            return fail(JH_ERR_ALIGN, "add_layernorm_bwd: pointers must be aligned to their elements");
+        if (dgamma || dbeta) {
+            const size_t need = jh::add_layernorm_bwd_workspace_size(M, N);
+            if (!workspace || workspace_bytes < need)
+                return fail(JH_ERR_WORKSPACE, "add_layernorm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+            if (!aligned(workspace, 4)) return fail(JH_ERR_ALIGN, "add_layernorm_bwd: workspace must be 4-byte aligned");
+        }
+    }
+    return check_hip(jh::launch_add_layernorm_bwd(x_dtype, h_dtype, d, dy, h, dh, mean, rstd, gamma, dx, dresidual, dgamma, dbeta,
+                                                  M, N, workspace, static_cast<hipStream_t>(stream)),
+                     "add_layernorm_bwd launch");
+}
+
+static int logprob_shape(const char* who, int dtype, int64_t stride, float scale, int M, int N) {
+    if (!real_dtype(dtype)) return fail(JH_ERR_DTYPE, "%s: dtype %d", who, dtype);
+    const int st = row_shape(who, M, N);
+    if (st != JH_OK) return st;
+    if (N < 1 || N > jh::kMaxLogprobVocab) return fail(JH_ERR_SHAPE, "%s: N=%d (1..%d)", who, N, jh::kMaxLogprobVocab);
+    // M rows apart by it stay within the addresses that kMaxElems allows
+    if (stride < N || (M > 0 && stride > kMaxElems / M)) return fail(JH_ERR_ARG, "%s: row stride %lld", who, (long long)stride);
+    if (!(scale > 1e-30f && scale < 1e30f)) return fail(JH_ERR_ARG, "%s: scale %g", who, scale);
+    return JH_OK;
+}
+
+size_t jules_hip_token_logprobs_workspace_size(int M, int N, int top) {
+    if (M <= 0 || N <= 0 || N > jh::kMaxLogprobVocab || (int64_t)M * N > kMaxElems || top < 0 || top > jh::kMaxLogprobTop) return 0;
+    return jh::token_logprobs_workspace_size(M, N, top);
+}
+
+int jules_hip_token_logprobs(int dtype, const void* logits, int64_t row_stride, float scale, const int32_t* tokens, float* logp,
+                             float* lse, float* entropy, int top, int32_t* top_ids, float* top_logp, int M, int N,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = logprob_shape("token_logprobs", dtype, row_stride, scale, M, N);
+    if (st != JH_OK) return st;
+    if (top < 0 || top > jh::kMaxLogprobTop || top > N)
+        return fail(JH_ERR_ARG, "token_logprobs: top %d (at most %d and N=%d)", top, jh::kMaxLogprobTop, N);
+    if (M == 0) return JH_OK;
+    if (!logits || (logp && !tokens) || (top && (!top_ids || !top_logp)))
+        return fail(JH_ERR_NULL, "token_logprobs: null logits, tokens, top_ids or top_logp");
+    if (!aligned(logits, real_size(dtype)) || !aligned(tokens, 4) || !aligned(logp, 4) || !aligned(lse, 4) || !aligned(entropy, 4) ||
+        !aligned(top_ids, 4) || !aligned(top_logp, 4))
+        return fail(JH_ERR_ALIGN, "token_logprobs: pointers must be aligned to their elements");
+    const size_t need = jh::token_logprobs_workspace_size(M, N, top);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(JH_ERR_WORKSPACE, "token_logprobs: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need && !aligned(workspace, 8)) return fail(JH_ERR_ALIGN, "token_logprobs: workspace must be 8-byte aligned");
+    return check_hip(jh::launch_token_logprobs(dtype, logits, row_stride, scale, tokens, logp, lse, entropy, top, top_ids, top_logp,
+                                               M, N, workspace, static_cast<hipStream_t>(stream)),
+                     "token_logprobs launch");
+}
+
+int jules_hip_token_logprobs_bwd(int dtype, const void* logits, int64_t row_stride, float scale, const int32_t* tokens,
+                                 const float* lse, const float* entropy, const float* dlogp, const float* dentropy, void* dlogits,
+                                 int64_t dlogits_stride, int M, int N, void* stream) {
+    int st = logprob_shape("token_logprobs_bwd", dtype, row_stride, scale, M, N);
+    if (st != JH_OK) return st;
+    st = logprob_shape("token_logprobs_bwd", dtype, dlogits_stride, scale, M, N);
+    if (st != JH_OK) return st;
+    if (dlogits == logits && logits && dlogits_stride != row_stride)
+        return fail(JH_ERR_ARG, "token_logprobs_bwd: in place needs the same strides");
+    if (M == 0) return JH_OK;
+    if (!logits || !tokens || !lse || !dlogp || !dlogits || (dentropy && !entropy))
+        return fail(JH_ERR_NULL, "token_logprobs_bwd: null logits, tokens, lse, dlogp, dlogits or entropy");
+    if (!aligned(logits, real_size(dtype)) || !aligned(dlogits, real_size(dtype)) || !aligned(tokens, 4) || !aligned(lse, 4) ||
+        !aligned(entropy, 4) || !aligned(dlogp, 4) || !aligned(dentropy, 4))
+        return fail(JH_ERR_ALIGN, "token_logprobs_bwd: pointers must be aligned to their elements");
+    return check_hip(jh::launch_token_logprobs_bwd(dtype, logits, row_stride, scale, tokens, lse, entropy, dlogp, dentropy, dlogits,
+                                                   dlogits_stride, M, N, static_cast<hipStream_t>(stream)),
+                     "token_logprobs_bwd launch");
+}
+
 // Whether the elements of a [sizes] array with these strides, rows of D side by
 // side, lie apart: each axis steps past everything the smaller ones span.
 static bool apart(const int64_t* strides, const int* sizes, int D) {

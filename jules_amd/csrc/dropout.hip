@@ -1,0 +1,67 @@
+// dropout.hip - dropout whose mask is made from a counter each time and never
+// stored (philox.hpp), with a residual's addition or without; its backward pass
+// is the same call on the gradient.  No counterpart in the reference.
+//
+//   out = [residual +] (kept ? x * scale : 0)
+//
+// A thread takes pieces of 8 neighbouring elements of a row, one counter each.
+#include <algorithm>
+
+#include "launch.hpp"
+#include "philox.hpp"
+
+namespace jh {
+namespace {
+
+template <typename XT, typename OT, bool RES>
+__global__ __launch_bounds__(256) void dropout_kernel(Dropout d, const XT* x, const OT* r, OT* out, int M, int N) {
+    const int pieces = N / 8 + (N % 8 != 0);
+    const DropKey key = drop_key(d);
+    // a thread's pieces lie `stride` apart, in rows and pieces: one division for all of them
+    const uint32_t stride = gridDim.x * 256, first = blockIdx.x * 256 + threadIdx.x;
+    const int rows_on = (int)(stride / (uint32_t)pieces), pieces_on = (int)(stride % (uint32_t)pieces);
+    int64_t row = first / (uint32_t)pieces;
+    int piece = (int)(first % (uint32_t)pieces);
+    while (row < M) {
+        const int n = min(8, N - 8 * piece);
+        const int64_t at = row * N + 8 * (int64_t)piece;
+        f32x8_t y = drop8(load_piece(x + at, n), key, d, (uint32_t)row, (uint32_t)piece);
+        if constexpr (RES) {
+            const f32x8_t old = load_piece(r + at, n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y.v[i] += old.v[i];
+        }
+        store_piece(out + at, y, n);
+        row += rows_on;
+        piece += pieces_on;
+        if (piece >= pieces) {
+            piece -= pieces;
+            ++row;
+        }
+    }
+}
+
+template <typename XT, typename OT>
+hipError_t launch(const Dropout& d, const void* x, const void* r, void* out, int M, int N, hipStream_t s) {
+    const int64_t blocks = ((int64_t)M * (N / 8 + (N % 8 != 0)) + 255) / 256;
+    const unsigned grid = (unsigned)std::min(blocks, (int64_t)2048);
+    if (r)
+        dropout_kernel<XT, OT, true><<<grid, 256, 0, s>>>(d, static_cast<const XT*>(x), static_cast<const OT*>(r),
+                                                          static_cast<OT*>(out), M, N);
+    else
+        dropout_kernel<XT, OT, false><<<grid, 256, 0, s>>>(d, static_cast<const XT*>(x), nullptr, static_cast<OT*>(out), M, N);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_dropout(int x_dtype, int out_dtype, const Dropout& d, const void* x, const void* residual, void* out, int M,
+                          int N, hipStream_t s) {
+    if (x_dtype == JH_F32)
+        return out_dtype == JH_F32 ? launch<float, float>(d, x, residual, out, M, N, s)
+                                   : launch<float, uint16_t>(d, x, residual, out, M, N, s);
+    return out_dtype == JH_F32 ? launch<uint16_t, float>(d, x, residual, out, M, N, s)
+                               : launch<uint16_t, uint16_t>(d, x, residual, out, M, N, s);
+}
+
+}  // namespace jh

@@ -179,6 +179,39 @@ hipError_t launch_rotary(int x_dtype, int out_dtype, bool half, bool inverse, co
                          void* out, const int64_t* os, const int32_t* pos, const double* freq, const int32_t* axis,
                          int axes, int B, int H, int S, int D, int R, hipStream_t s);
 
+// Dropout's random bits (philox.hpp): dropped where an element's 16 bits are below
+// t, multiplied by scale elsewhere
+struct Dropout {
+    const int64_t* rng;  // device: seed, position
+    uint64_t offset;     // added to the position
+    uint32_t t;          // 0: nothing is dropped, rng is not read
+    float scale;
+};
+// out = [residual +] dropout of x (dropout.hip); residual of out's type, or null
+hipError_t launch_dropout(int x_dtype, int out_dtype, const Dropout& drop, const void* x, const void* residual, void* out,
+                          int M, int N, hipStream_t s);
+// h = r + dropout of x; out = its layer norm (layernorm.hip).  Null: r, gamma (ones),
+// beta (zeros), and h_out, mean and rstd where they are not wanted
+hipError_t launch_add_layernorm(int x_dtype, int h_dtype, int out_dtype, const Dropout& drop, const void* x, const void* r,
+                                const float* gamma, const float* beta, void* h_out, void* out, float* mean, float* rstd,
+                                int M, int N, float eps, hipStream_t s);
+// its gradients; ws: add_layernorm_bwd_workspace_size bytes where dgamma or dbeta is wanted
+size_t add_layernorm_bwd_workspace_size(int M, int N);
+hipError_t launch_add_layernorm_bwd(int x_dtype, int h_dtype, const Dropout& drop, const void* dy, const void* h,
+                                    const void* dh, const float* mean, const float* rstd, const float* gamma, void* dx,
+                                    void* dr, float* dgamma, float* dbeta, int M, int N, void* ws, hipStream_t s);
+// log probabilities of tokens, entropy, alternatives, and the logits' gradient
+// (logprobs.hip); ws: token_logprobs_workspace_size bytes
+constexpr int kMaxLogprobTop = 64;
+constexpr int kMaxLogprobVocab = 1 << 22;
+size_t token_logprobs_workspace_size(int M, int N, int top);
+hipError_t launch_token_logprobs(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens,
+                                 float* logp, float* lse, float* entropy, int top, int32_t* top_ids, float* top_logp,
+                                 int M, int N, void* ws, hipStream_t s);
+hipError_t launch_token_logprobs_bwd(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens,
+                                     const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
+                                     void* dlogits, int64_t out_stride, int M, int N, hipStream_t s);
+
 // the 4-bit key/value cache (layout: kv4.hpp)
 struct KV4View {
     uint8_t *k, *v;

@@ -1,0 +1,461 @@
+// layernorm.hip - layer norm of a training step: forward with the residual's
+// addition and dropout (philox.hpp), and backward with the gradients of the
+// norm's weight and bias.  No counterpart in the reference, whose fusedLayerNorm
+// (rowops.hip) is fp32 and forward only.
+//
+//   h = r + drop(x),  y_j = (h_j - mean) rstd gamma_j + beta_j,
+//   mean = sum h / N,  rstd = 1 / sqrt(sum (h - mean)^2 / N + eps)
+//
+//   n_j = (h_j - mean) rstd,  a_j = dy_j gamma_j
+//   dr_j = rstd (a_j - sum a / N - n_j sum a n / N) + dh_j,  dx = drop(dr)
+//   dgamma_j = sum over rows of dy_j n_j,  dbeta_j = sum over rows of dy_j
+//
+// A row is read once, held in registers, and written once.  The mean is summed in
+// 64 bits and the squares are those of the distances from it, also in 64 bits: no
+// row that fp32 holds overflows or cancels in them.
+//
+// Backward: a group of threads goes over many rows with its columns' two sums in
+// registers, so dy and h are read once for the row's gradient and the columns'; a
+// block leaves one row of partial sums in the workspace, and a second kernel adds
+// those in order.  No atomics: the results do not depend on timing.
+#include <algorithm>
+
+#include "launch.hpp"
+#include "philox.hpp"
+
+namespace jh {
+namespace {
+
+// Sum over the G threads of a group (blocks of 256 threads hold 256 / G groups
+// where G is less), the same order for every row.  The waves' parts alternate
+// between two places, so that one barrier is enough: a wave that writes a place
+// again has passed the barrier after which it was read.
+template <int G, int K, typename T>
+__device__ __forceinline__ void reduce_group(T (&a)[K], int& turn) {
+#pragma unroll
+    for (int o = G < 64 ? G / 2 : 32; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) a[k] += __shfl_xor(a[k], o);
+    if constexpr (G > 64) {
+        __shared__ T parts[2][G / 64][K];
+        T(*part)[K] = parts[turn & 1];
+        ++turn;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) part[threadIdx.x >> 6][k] = a[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            a[k] = part[0][k];
+#pragma unroll
+            for (int w = 1; w < G / 64; ++w) a[k] += part[w][k];
+        }
+    }
+}
+
+struct ForwardArgs {
+    const void *x, *r;
+    const float *gamma, *beta;  // null: ones, zeros
+    void *h_out, *out;
+    float *mean, *rstd;  // null: not kept
+    Dropout drop;
+    int M, N, h_dtype, out_dtype;
+    float eps;
+};
+
+__device__ __forceinline__ f32x8_t load_vector(const float* v, int j, int n, float none) {
+    if (v) return load_piece(v + j, n);
+    f32x8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = none;
+    return r;
+}
+
+template <typename XT>
+__device__ __forceinline__ f32x8_t read_h(const ForwardArgs& a, const DropKey& key, int64_t row, int j, int n) {
+    const int64_t at = row * a.N + j;
+    f32x8_t h = load_piece(static_cast<const XT*>(a.x) + at, n);
+    if (a.drop.t) h = drop8(h, key, a.drop, (uint32_t)row, (uint32_t)j / 8);
+    if (a.r) {
+        const f32x8_t r = a.h_dtype == JH_F32 ? load_piece(static_cast<const float*>(a.r) + at, n)
+                                              : load_piece(static_cast<const uint16_t*>(a.r) + at, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h.v[i] += r.v[i];
+    }
+    return h;
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t at, const f32x8_t& v, int n) {
+    if (dtype == JH_F32)
+        store_piece(static_cast<float*>(p) + at, v, n);
+    else
+        store_piece(static_cast<uint16_t*>(p) + at, v, n);
+}
+__device__ __forceinline__ void write_y(const ForwardArgs& a, int64_t row, int j, int n, const f32x8_t& h, float mean,
+                                        float rstd) {
+    const int64_t at = row * a.N + j;
+    if (a.h_out) store_any(a.h_out, a.h_dtype, at, h, n);
+    const f32x8_t g = load_vector(a.gamma, j, n, 1.0f), b = load_vector(a.beta, j, n, 0.0f);
+    f32x8_t y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.v[i] = __builtin_fmaf((h.v[i] - mean) * rstd, g.v[i], b.v[i]);
+    store_any(a.out, a.out_dtype, at, y, n);
+}
+
+__device__ __forceinline__ double sum8(const f32x8_t& h, int n) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += i < n ? (double)h.v[i] : 0.0;
+    return s;
+}
+__device__ __forceinline__ double squares8(const f32x8_t& h, double mean, int n) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double d = i < n ? (double)h.v[i] - mean : 0.0;
+        s = __builtin_fma(d, d, s);
+    }
+    return s;
+}
+__device__ __forceinline__ float row_rstd(double squares, int N, float eps) {
+    return (float)(1.0 / sqrt(squares / (double)N + (double)eps));
+}
+
+// G threads a row, NP pieces of 8 neighbouring elements a thread
+template <typename XT, int G, int NP>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_kernel(ForwardArgs a) {
+    constexpr int ROWS = G < 256 ? 256 / G : 1;
+    const int tid = G < 256 ? threadIdx.x % G : threadIdx.x;
+    const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + (G < 256 ? threadIdx.x / G : 0); row < a.M;
+         row += (int64_t)gridDim.x * ROWS) {
+        f32x8_t h[NP];
+        double s[1] = {0.0};
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n > 0) h[t] = read_h<XT>(a, key, row, j, n);
+        }
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int n = min(8, a.N - 8 * (tid + G * t));
+            if (n > 0) s[0] += sum8(h[t], n);
+        }
+        reduce_group<G>(s, turn);
+        const double center = s[0] / (double)a.N;
+        const float mean = (float)center;
+        s[0] = 0.0;
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int n = min(8, a.N - 8 * (tid + G * t));
+            if (n > 0) s[0] += squares8(h[t], center, n);
+        }
+        reduce_group<G>(s, turn);
+        const float rstd = row_rstd(s[0], a.N, a.eps);
+        if (tid == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n > 0) write_y(a, row, j, n, h[t], mean, rstd);
+        }
+    }
+}
+
+// rows longer than a block holds: read three times.  An element of x and r is last
+// read by the thread that then writes it, so the outputs may be the inputs here too.
+template <typename XT>
+__global__ __launch_bounds__(1024) void add_layernorm_long_kernel(ForwardArgs a) {
+    const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
+    int turn = 0;
+    const auto pieces = [&](auto&& f) {
+        for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) f((int)j, (int)min((int64_t)8, a.N - j));
+    };
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        double s[1] = {0.0};
+        pieces([&](int j, int n) { s[0] += sum8(read_h<XT>(a, key, row, j, n), n); });
+        reduce_group<1024>(s, turn);
+        const double center = s[0] / (double)a.N;
+        const float mean = (float)center;
+        s[0] = 0.0;
+        pieces([&](int j, int n) { s[0] += squares8(read_h<XT>(a, key, row, j, n), center, n); });
+        reduce_group<1024>(s, turn);
+        const float rstd = row_rstd(s[0], a.N, a.eps);
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+        pieces([&](int j, int n) { write_y(a, row, j, n, read_h<XT>(a, key, row, j, n), mean, rstd); });
+    }
+}
+
+template <typename XT, int G, int NP>
+void launch_forward(const ForwardArgs& a, int blocks, hipStream_t s) {
+    constexpr int ROWS = G < 256 ? 256 / G : 1;
+    const int64_t rows = ((int64_t)a.M + ROWS - 1) / ROWS;
+    add_layernorm_kernel<XT, G, NP><<<(unsigned)std::min((int64_t)blocks, rows), G < 256 ? 256 : G, 0, s>>>(a);
+}
+
+template <typename XT>
+hipError_t launch_forward(const ForwardArgs& a, hipStream_t s) {
+    if (a.N <= 128)
+        launch_forward<XT, 16, 1>(a, 8192, s);
+    else if (a.N <= 512)
+        launch_forward<XT, 64, 1>(a, 8192, s);
+    else if (a.N <= 2048)
+        launch_forward<XT, 256, 1>(a, 2048, s);
+    else if (a.N <= 4096)
+        launch_forward<XT, 256, 2>(a, 2048, s);
+    else if (a.N <= 8192)
+        launch_forward<XT, 256, 4>(a, 1024, s);
+    else if (a.N <= 16384)
+        launch_forward<XT, 512, 4>(a, 512, s);
+    else
+        add_layernorm_long_kernel<XT><<<(unsigned)std::min(a.M, 2048), 1024, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+// ---- backward -----------------------------------------------------------------
+
+struct BackwardArgs {
+    const void *dy, *h, *dh;  // dh null: none
+    const float *mean, *rstd, *gamma;
+    void *dx, *dr;   // either may be null: not wanted
+    float* partial;  // [blocks][2][N]: sums of dy n and of dy over the block's rows; null: not wanted
+    Dropout drop;
+    int M, N, x_dtype, h_dtype;  // dy and dx, h, dh and dr
+};
+
+__device__ __forceinline__ f32x8_t load_any(const void* p, int dtype, int64_t at, int n) {
+    return dtype == JH_F32 ? load_piece(static_cast<const float*>(p) + at, n)
+                           : load_piece(static_cast<const uint16_t*>(p) + at, n);
+}
+// dr and dx of a piece
+__device__ __forceinline__ void write_gradient(const BackwardArgs& a, const DropKey& key, int64_t row, int j, int n,
+                                               const f32x8_t& dy, const f32x8_t& norm, const f32x8_t& gamma, float rstd, float c1,
+                                               float c2) {
+    const int64_t at = row * a.N + j;
+    f32x8_t g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g.v[i] = rstd * (__builtin_fmaf(dy.v[i], gamma.v[i], -c1) - norm.v[i] * c2);
+    if (a.dh) {
+        const f32x8_t dh = load_any(a.dh, a.h_dtype, at, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g.v[i] += dh.v[i];
+    }
+    if (a.dr) store_any(a.dr, a.h_dtype, at, g, n);
+    if (a.dx) {
+        if (a.drop.t) g = drop8(g, key, a.drop, (uint32_t)row, (uint32_t)j / 8);
+        store_any(a.dx, a.x_dtype, at, g, n);
+    }
+}
+
+template <int G, int NP>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(BackwardArgs a) {
+    constexpr int ROWS = G < 256 ? 256 / G : 1;
+    const int tid = G < 256 ? threadIdx.x % G : threadIdx.x, group = G < 256 ? threadIdx.x / G : 0;
+    const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
+    int turn = 0;
+    f32x8_t gamma[NP], sum_n[NP], sum_y[NP];
+#pragma unroll
+    for (int t = 0; t < NP; ++t) {
+        const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+        if (n > 0) gamma[t] = load_vector(a.gamma, j, n, 1.0f);
+        sum_n[t] = sum_y[t] = f32x8_t{};
+    }
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.M; row += (int64_t)gridDim.x * ROWS) {
+        f32x8_t dy[NP], norm[NP];
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float c[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n <= 0) continue;
+            dy[t] = load_any(a.dy, a.x_dtype, row * a.N + j, n);
+            norm[t] = load_any(a.h, a.h_dtype, row * a.N + j, n);
+        }
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n <= 0) continue;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                norm[t].v[i] = (norm[t].v[i] - mean) * rstd;
+                const float g = dy[t].v[i] * gamma[t].v[i];  // 0 behind the row's end
+                c[0] += g;
+                c[1] = __builtin_fmaf(g, norm[t].v[i], c[1]);
+                sum_n[t].v[i] = __builtin_fmaf(dy[t].v[i], norm[t].v[i], sum_n[t].v[i]);
+                sum_y[t].v[i] += dy[t].v[i];
+            }
+        }
+        reduce_group<G>(c, turn);
+        const float c1 = c[0] / (float)a.N, c2 = c[1] / (float)a.N;
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n > 0) write_gradient(a, key, row, j, n, dy[t], norm[t], gamma[t], rstd, c1, c2);
+        }
+    }
+    if (!a.partial) return;
+    float* out = a.partial + (int64_t)blockIdx.x * 2 * a.N;
+    if constexpr (ROWS > 1) {
+        // the block's groups, in order
+        __shared__ float sums[ROWS][2][8 * G];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sums[group][0][8 * tid + i] = sum_n[0].v[i];
+            sums[group][1][8 * tid + i] = sum_y[0].v[i];
+        }
+        __syncthreads();
+        for (int k = threadIdx.x; k < 16 * G; k += 256) {
+            const int which = k / (8 * G), j = k % (8 * G);
+            if (j >= a.N) continue;
+            float s = 0.0f;
+            for (int g = 0; g < ROWS; ++g) s += sums[g][which][j];
+            out[which * (int64_t)a.N + j] = s;
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < NP; ++t) {
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n <= 0) continue;
+            store_piece(out + j, sum_n[t], n);
+            store_piece(out + a.N + j, sum_y[t], n);
+        }
+    }
+}
+
+// rows longer than a block holds: dy, h are read twice, and once more for the columns
+__global__ __launch_bounds__(1024) void add_layernorm_bwd_long_kernel(BackwardArgs a) {
+    const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        const auto pieces = [&](auto&& f) {
+            for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) {
+                const int n = (int)min((int64_t)8, a.N - j);
+                const f32x8_t dy = load_any(a.dy, a.x_dtype, row * a.N + j, n);
+                f32x8_t norm = load_any(a.h, a.h_dtype, row * a.N + j, n);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) norm.v[i] = (norm.v[i] - mean) * rstd;
+                f((int)j, n, dy, norm, load_vector(a.gamma, (int)j, n, 1.0f));
+            }
+        };
+        float c[2] = {0.0f, 0.0f};
+        pieces([&](int, int, const f32x8_t& dy, const f32x8_t& norm, const f32x8_t& gamma) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float g = dy.v[i] * gamma.v[i];
+                c[0] += g;
+                c[1] = __builtin_fmaf(g, norm.v[i], c[1]);
+            }
+        });
+        reduce_group<1024>(c, turn);
+        const float c1 = c[0] / (float)a.N, c2 = c[1] / (float)a.N;
+        pieces([&](int j, int n, const f32x8_t& dy, const f32x8_t& norm, const f32x8_t& gamma) {
+            write_gradient(a, key, row, j, n, dy, norm, gamma, rstd, c1, c2);
+        });
+    }
+}
+// the columns' sums of rows blockIdx.y, blockIdx.y + gridDim.y, .. of long rows
+__global__ __launch_bounds__(256) void layernorm_columns_kernel(BackwardArgs a) {
+    for (int64_t j = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x); j < a.N; j += 8 * 256 * (int64_t)gridDim.x) {
+        const int n = (int)min((int64_t)8, a.N - j);
+        f32x8_t sum_n{}, sum_y{};
+        for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
+            const f32x8_t dy = load_any(a.dy, a.x_dtype, row * a.N + j, n), h = load_any(a.h, a.h_dtype, row * a.N + j, n);
+            const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum_n.v[i] = __builtin_fmaf(dy.v[i], (h.v[i] - mean) * rstd, sum_n.v[i]);
+                sum_y.v[i] += dy.v[i];
+            }
+        }
+        float* out = a.partial + (int64_t)blockIdx.y * 2 * a.N + j;
+        store_piece(out, sum_n, n);
+        store_piece(out + a.N, sum_y, n);
+    }
+}
+
+// dgamma, dbeta = the partial rows' sums: 32 columns a block, 8 threads a column
+__global__ __launch_bounds__(256) void layernorm_fold_kernel(const float* partial, int parts, float* dgamma, float* dbeta,
+                                                             int N) {
+    __shared__ float sums[8][32];
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    for (int64_t j0 = 32 * (int64_t)blockIdx.x; j0 < 2 * (int64_t)N; j0 += 32 * (int64_t)gridDim.x) {
+        const int64_t j = j0 + lane;
+        float s = 0.0f;
+        if (j < 2 * (int64_t)N)
+            for (int p = group; p < parts; p += 8) s += partial[p * 2 * (int64_t)N + j];
+        sums[group][lane] = s;
+        __syncthreads();
+        if (group == 0 && j < 2 * (int64_t)N) {
+            for (int g = 1; g < 8; ++g) s += sums[g][lane];
+            float* out = j < N ? dgamma : dbeta;
+            if (out) out[j < N ? j : j - N] = s;
+        }
+        __syncthreads();
+    }
+}
+
+// how many blocks, and with them partial rows, the backward pass has
+int backward_blocks(int M, int N) {
+    if (N <= 512) {
+        const int rows = N <= 128 ? 16 : 4;
+        return std::min(M / rows + (M % rows != 0), 1024);
+    }
+    return std::min(M, N <= 2048 ? 1024 : N <= 16384 ? 512 : 64);
+}
+
+template <int G, int NP>
+void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
+    add_layernorm_bwd_kernel<G, NP><<<(unsigned)blocks, G < 256 ? 256 : G, 0, s>>>(a);
+}
+
+}  // namespace
+
+hipError_t launch_add_layernorm(int x_dtype, int h_dtype, int out_dtype, const Dropout& drop, const void* x, const void* r,
+                                const float* gamma, const float* beta, void* h_out, void* out, float* mean, float* rstd, int M,
+                                int N, float eps, hipStream_t s) {
+    const ForwardArgs a{x, r, gamma, beta, h_out, out, mean, rstd, drop, M, N, h_dtype, out_dtype, eps};
+    return x_dtype == JH_F32 ? launch_forward<float>(a, s) : launch_forward<uint16_t>(a, s);
+}
+
+size_t add_layernorm_bwd_workspace_size(int M, int N) { return (size_t)backward_blocks(M, N) * 2 * (size_t)N * sizeof(float); }
+
+hipError_t launch_add_layernorm_bwd(int x_dtype, int h_dtype, const Dropout& drop, const void* dy, const void* h, const void* dh,
+                                    const float* mean, const float* rstd, const float* gamma, void* dx, void* dr, float* dgamma,
+                                    float* dbeta, int M, int N, void* ws, hipStream_t s) {
+    const bool columns = dgamma || dbeta;
+    const BackwardArgs a{dy, h, dh, mean, rstd, gamma, dx, dr, columns ? static_cast<float*>(ws) : nullptr, drop, M, N, x_dtype,
+                         h_dtype};
+    const int blocks = backward_blocks(M, N);
+    if (M == 0) {
+        // no rows: the columns' sums are 0
+    } else if (N <= 128) {
+        launch_backward<16, 1>(a, blocks, s);
+    } else if (N <= 512) {
+        launch_backward<64, 1>(a, blocks, s);
+    } else if (N <= 2048) {
+        launch_backward<256, 1>(a, blocks, s);
+    } else if (N <= 4096) {
+        launch_backward<256, 2>(a, blocks, s);
+    } else if (N <= 8192) {
+        launch_backward<512, 2>(a, blocks, s);
+    } else if (N <= 16384) {
+        launch_backward<512, 4>(a, blocks, s);
+    } else {
+        // the columns first: dx and dr may be dy and dh
+        if (columns) layernorm_columns_kernel<<<dim3((unsigned)std::min((N + 2047) / 2048, 65535), blocks), 256, 0, s>>>(a);
+        if (dx || dr) add_layernorm_bwd_long_kernel<<<(unsigned)std::min(M, 2048), 1024, 0, s>>>(a);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !columns) return e;
+    layernorm_fold_kernel<<<(unsigned)std::min((2 * (int64_t)N + 31) / 32, (int64_t)2048), 256, 0, s>>>(a.partial, blocks, dgamma,
+                                                                                                  dbeta, N);
+    return hipGetLastError();
+}
+
+}  // namespace jh

@@ -1,0 +1,416 @@
+// logprobs.hip - log probabilities of given tokens, with the log-sum-exp, the
+// entropy and the most likely alternatives of each row of logits, and the
+// gradient with respect to the logits.  No counterpart in the reference, whose
+// fusedCrossEntropyLoss (rowops.hip) gives one mean loss of fp32 rows.
+//
+//   z = scale x,  m = max z,  s = sum e^(z - m),  w = sum e^(z - m) (z - m)
+//   lse = m + ln s,  logp = z_t - m - ln s,  entropy = ln s - w / s
+//
+// One pass over a row: every thread keeps the maximum and the sums of its own
+// pieces of 8 neighbouring elements, the sums relative to its maximum, and the
+// block joins them at the end.
+//
+// The k alternatives are the first in the order (value falling, index rising).
+// Each thread also keeps the largest value of each of its pieces.  The k-th
+// largest pair (value, piece) among the threads' largest bounds what can be among
+// the first k, since k threads hold one at least as large; at most k threads reach
+// it, so at most 8 NP k elements do.  Those threads read their pieces that reach
+// it again and put the elements in LDS, where each counts those before it.
+//
+// A row may be split over blocks (few rows, or more than 65536 elements); the
+// blocks' results, their k alternatives among them, are then joined by a second
+// kernel.
+//
+//   dx_j = scale (g ([j = t] - p_j) - gh p_j (ln p_j + entropy)),  p = e^(z - lse)
+#include <algorithm>
+#include <cfloat>
+
+#include "launch.hpp"
+#include "pieces.hpp"
+
+namespace jh {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// where a distance from the maximum is -infinity: e^ of it is 0, and so is its product with that
+constexpr float FAR = -1e30f;
+constexpr int MAX_TOP = kMaxLogprobTop;
+constexpr int MAX_PARTS = kMaxLogprobVocab / 65536;
+
+// a float's place in an order of unsigned numbers, 0 where nothing is; -0 is +0
+__device__ __forceinline__ uint32_t order_of(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+    return __uint_as_float(o ^ ((int32_t)o < 0 ? 0x80000000u : 0xffffffffu));
+}
+// (value falling, place rising)
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t place) { return (uint64_t)order_of(v) << 32 | (0xffffffffu - place); }
+__device__ __forceinline__ uint32_t place_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+
+// maximum, and the sums relative to it: e^((x - m) scale), and that times its exponent in powers of 2
+struct Sums {
+    float m, s, w;
+};
+__device__ __forceinline__ Sums no_sums() { return Sums{-FLT_MAX, 0.0f, 0.0f}; }
+// relative to a maximum m at least as large; c2 = scale log2(e)
+__device__ __forceinline__ void raise(Sums* a, float m, float c2) {
+    const float d = larger((a->m - m) * c2, FAR), f = __builtin_amdgcn_exp2f(d);
+    a->w = f * __builtin_fmaf(d, a->s, a->w);
+    a->s *= f;
+    a->m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c2) {
+    const float m = larger(a.m, b.m);
+    raise(&a, m, c2);
+    raise(&b, m, c2);
+    return Sums{m, a.s + b.s, a.w + b.w};
+}
+
+struct LogprobArgs {
+    const void* logits;
+    const int32_t* tokens;
+    float *logp, *lse, *entropy;  // null: not wanted
+    int32_t* top_ids;
+    float* top_logp;
+    int64_t stride;
+    float scale, c2;
+    int M, N, top, parts, width;  // width: elements of a part, a multiple of 8
+    // of split rows: [M][parts] sums, [M][parts][top] keys
+    Sums* sums;
+    uint64_t* keys;
+};
+
+// ln of the sum; what a row of nothing but -infinity gets: probability 0 everywhere, no entropy
+struct RowNumbers {
+    float m, log_s, entropy;
+    bool bad, none;  // a NaN or +infinity; nothing but -infinity
+};
+__device__ __forceinline__ RowNumbers row_numbers(const Sums& a) {
+    RowNumbers r;
+    r.bad = !(a.s <= FLT_MAX);
+    r.none = a.s == 0.0f;
+    r.m = a.m;
+    r.log_s = logf(a.s);
+    r.entropy = r.bad ? __builtin_nanf("") : r.none ? 0.0f : fmaxf(r.log_s - LN2 * (a.w / a.s), 0.0f);
+    return r;
+}
+__device__ __forceinline__ float log_prob(const RowNumbers& r, float x, float scale) {
+    return r.bad ? __builtin_nanf("") : r.none ? -INFINITY : (x - r.m) * scale - r.log_s;
+}
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, const RowNumbers& r) {
+    if (a.lse) a.lse[row] = r.bad ? __builtin_nanf("") : r.none ? -INFINITY : __builtin_fmaf(r.m, a.scale, r.log_s);
+    if (a.entropy) a.entropy[row] = r.entropy;
+    if (a.logp) {
+        const int t = a.tokens[row];
+        float v = 0.0f;  // a negative token: none
+        if (t >= a.N)
+            v = __builtin_nanf("");
+        else if (t >= 0)
+            v = log_prob(r, load1(static_cast<const T*>(a.logits) + row * a.stride + t), a.scale);
+        a.logp[row] = v;
+    }
+}
+__device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, int rank, uint64_t key, const RowNumbers& r) {
+    const int64_t at = row * a.top + rank;
+    a.top_ids[at] = r.bad ? -1 : (int32_t)place_of(key);
+    a.top_logp[at] = log_prob(r, value_of((uint32_t)(key >> 32)), a.scale);
+}
+
+// how many of n keys in LDS come before this one
+__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += keys[i] > key;
+    return rank;
+}
+
+template <typename T, int BT, int NP, bool TOP>
+__global__ __launch_bounds__(BT) void logprobs_kernel(LogprobArgs a) {
+    constexpr int WAVES = BT / 64, B = NP < 4 ? NP : 4;
+    __shared__ Sums wave_sums[WAVES];
+    __shared__ uint64_t keys[TOP ? std::max(BT, MAX_TOP * 8 * NP + 8) : 1];
+    __shared__ uint32_t groups[64];
+    __shared__ int found[2];
+    __shared__ uint64_t threshold;
+    __shared__ uint32_t group_threshold;
+    const int tid = threadIdx.x;
+    for (int64_t item = blockIdx.x; item < (int64_t)a.M * a.parts; item += gridDim.x) {
+        const int64_t row = item / a.parts;
+        const int part = (int)(item % a.parts);
+        const int first = part * a.width, len = min(a.width, a.N - first);
+        const T* x = static_cast<const T*>(a.logits) + row * a.stride + first;
+        Sums mine = no_sums();
+        float u[TOP ? NP : 1];
+        float best = -INFINITY;
+        int best_piece = -1;
+#pragma unroll
+        for (int b = 0; b < NP; b += B) {
+            f32x8_t v[B];
+#pragma unroll
+            for (int t = 0; t < B; ++t) {
+                const int j = 8 * (tid + BT * (b + t)), n = min(8, len - j);
+                if (n > 0) v[t] = load_piece(x + j, n, -INFINITY);
+            }
+            float m = mine.m;
+#pragma unroll
+            for (int t = 0; t < B; ++t) {
+                const int piece = tid + BT * (b + t);
+                if (8 * piece >= len) continue;
+                float top = v[t].v[0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) top = larger(top, v[t].v[i]);
+                m = larger(m, top);
+                if constexpr (TOP) {
+                    u[b + t] = top;
+                    if (top > best || best_piece < 0) best = top, best_piece = piece;
+                }
+            }
+            raise(&mine, m, a.c2);
+#pragma unroll
+            for (int t = 0; t < B; ++t) {
+                if (8 * (tid + BT * (b + t)) >= len) continue;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float d = larger((v[t].v[i] - m) * a.c2, FAR), e = __builtin_amdgcn_exp2f(d);
+                    mine.s += e;
+                    mine.w = __builtin_fmaf(e, d, mine.w);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            mine = join(mine, Sums{__shfl_xor(mine.m, o), __shfl_xor(mine.s, o), __shfl_xor(mine.w, o)}, a.c2);
+        if ((tid & 63) == 0) wave_sums[tid >> 6] = mine;
+        if constexpr (TOP) {
+            uint32_t g = best_piece < 0 ? 0 : order_of(best);
+#pragma unroll
+            for (int o = 1; o < BT / 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor((int)g, o));
+            if (tid % (BT / 64) == 0) groups[tid / (BT / 64)] = g;
+            if (tid < 2) found[tid] = 0;
+            if (tid == 0) threshold = 0;
+        }
+        __syncthreads();
+        Sums all = wave_sums[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) all = join(all, wave_sums[w], a.c2);
+        const RowNumbers r = row_numbers(all);
+        if (a.parts > 1) {
+            if (tid == 0) a.sums[item] = all;
+        } else if (tid == 0) {
+            write_row<T>(a, row, r);
+        }
+        if constexpr (TOP) {
+            uint64_t* part_keys = a.parts > 1 ? a.keys + item * a.top : nullptr;
+            if (r.bad) {  // no order among these
+                for (int i = tid; i < a.top; i += BT) {
+                    if (part_keys)
+                        part_keys[i] = 0;
+                    else
+                        write_top(a, row, i, 0, r);
+                }
+            } else {
+                // the top-th largest of 64 groups' largest values: a bound from below
+                if (tid < 64) {
+                    const uint32_t g = groups[tid];
+                    int rank = 0;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)g, i);
+                        rank += o > g || (o == g && i < tid);
+                    }
+                    if (rank == a.top - 1) group_threshold = g;
+                }
+                __syncthreads();
+                // the top-th largest of the threads'
+                const uint64_t own = best_piece < 0 ? 0 : key_of(best, (uint32_t)best_piece);
+                if (own && (uint32_t)(own >> 32) >= group_threshold) keys[atomicAdd(&found[0], 1)] = own;
+                __syncthreads();
+                const int threads = found[0];
+                if (tid < threads && rank_of(keys[tid], keys, threads) == a.top - 1) threshold = keys[tid];
+                __syncthreads();
+                // their elements that reach it
+                const uint64_t bound = threshold;
+                if (own && own >= bound) {
+#pragma unroll
+                    for (int t = 0; t < NP; ++t) {
+                        const int piece = tid + BT * t, n = min(8, len - 8 * piece);
+                        if (n <= 0 || key_of(u[t], (uint32_t)piece) < bound) continue;
+                        const f32x8_t v = load_piece(x + 8 * piece, n);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (i < n && key_of(v.v[i], (uint32_t)piece) >= bound)
+                                keys[atomicAdd(&found[1], 1)] = key_of(v.v[i], (uint32_t)(first + 8 * piece + i));
+                    }
+                }
+                __syncthreads();
+                const int n = found[1];
+                if (part_keys && tid >= n && tid < a.top) part_keys[tid] = 0;  // a part shorter than that
+                for (int i = tid; i < n; i += BT) {
+                    const uint64_t key = keys[i];
+                    const int rank = rank_of(key, keys, n);
+                    if (rank >= a.top) continue;
+                    if (part_keys)
+                        part_keys[rank] = key;
+                    else
+                        write_top(a, row, rank, key, r);
+                }
+            }
+        }
+        __syncthreads();  // the shared values are the next item's
+    }
+}
+
+// rows that were split: a block each
+template <typename T>
+__global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
+    __shared__ uint64_t keys[MAX_PARTS * MAX_TOP];
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        Sums all = no_sums();
+        for (int p = 0; p < a.parts; ++p) all = join(all, a.sums[row * a.parts + p], a.c2);
+        const RowNumbers r = row_numbers(all);
+        if (threadIdx.x == 0) write_row<T>(a, row, r);
+        if (!a.top) continue;
+        const int n = a.parts * a.top;
+        for (int i = threadIdx.x; i < n; i += 256) keys[i] = a.keys[row * n + i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const uint64_t key = keys[i];
+            if (r.bad) {
+                if (i < a.top) write_top(a, row, i, 0, r);
+            } else if (key) {
+                const int rank = rank_of(key, keys, n);
+                if (rank < a.top) write_top(a, row, rank, key, r);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+struct Split {
+    int parts, width;
+};
+Split split_of(int M, int N) {
+    int parts = N / 65536 + (N % 65536 != 0);
+    if (M < 256) parts = std::max(parts, std::min((512 + M - 1) / M, N / 2048));
+    parts = std::min(std::max(parts, 1), MAX_PARTS);
+    const int width = (N / parts + (N % parts != 0) + 7) / 8 * 8;
+    return Split{N / width + (N % width != 0), width};
+}
+
+template <typename T, int BT, int NP>
+void launch_part(const LogprobArgs& a, hipStream_t s) {
+    const unsigned grid = (unsigned)std::min((int64_t)a.M * a.parts, (int64_t)1 << 20);
+    if (a.top)
+        logprobs_kernel<T, BT, NP, true><<<grid, BT, 0, s>>>(a);
+    else
+        logprobs_kernel<T, BT, NP, false><<<grid, BT, 0, s>>>(a);
+}
+
+template <typename T>
+hipError_t launch(const LogprobArgs& a, hipStream_t s) {
+    if (a.width <= 2048)
+        launch_part<T, 256, 1>(a, s);
+    else if (a.width <= 4096)
+        launch_part<T, 256, 2>(a, s);
+    else if (a.width <= 8192)
+        launch_part<T, 256, 4>(a, s);
+    else if (a.width <= 16384)
+        launch_part<T, 256, 8>(a, s);
+    else if (a.width <= 32768)
+        launch_part<T, 1024, 4>(a, s);
+    else
+        launch_part<T, 1024, 8>(a, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.parts == 1) return e;
+    logprobs_join_kernel<T><<<(unsigned)std::min(a.M, 1 << 20), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+// ---- gradient ------------------------------------------------------------------
+
+struct GradArgs {
+    const void* logits;
+    const int32_t* tokens;
+    const float *lse, *entropy, *dlogp, *dentropy;  // entropy and dentropy null: no gradient of the entropy
+    void* dlogits;
+    int64_t stride, out_stride;
+    float scale;
+    int M, N, chunks;
+};
+
+constexpr int GRAD_PIECES = 2;
+constexpr int GRAD_CHUNK = 256 * 8 * GRAD_PIECES;
+
+template <typename T>
+__global__ __launch_bounds__(256) void logprobs_bwd_kernel(GradArgs a) {
+    for (int64_t item = blockIdx.x; item < (int64_t)a.M * a.chunks; item += gridDim.x) {
+        const int64_t row = item / a.chunks;
+        const int first = (int)(item % a.chunks) * GRAD_CHUNK;
+        const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+        T* out = static_cast<T*>(a.dlogits) + row * a.out_stride;
+        const int token = a.tokens[row];
+        const float lse = a.lse[row], entropy = a.entropy ? a.entropy[row] : 0.0f;
+        // a row of nothing but -infinity has no gradient, whatever reaches it
+        const bool none = lse == -INFINITY;
+        float g = token < 0 || none ? 0.0f : a.dlogp[row] * a.scale;
+        const float gh = !a.dentropy || none ? 0.0f : a.dentropy[row] * a.scale;
+        if (token >= a.N) g = __builtin_nanf("");
+        f32x8_t v[GRAD_PIECES];
+#pragma unroll
+        for (int t = 0; t < GRAD_PIECES; ++t) {
+            const int j = first + 8 * ((int)threadIdx.x + 256 * t), n = min(8, a.N - j);
+            if (n > 0) v[t] = load_piece(x + j, n);
+        }
+#pragma unroll
+        for (int t = 0; t < GRAD_PIECES; ++t) {
+            const int j = first + 8 * ((int)threadIdx.x + 256 * t), n = min(8, a.N - j);
+            if (n <= 0) continue;
+            f32x8_t y;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float log = none ? FAR : larger(__builtin_fmaf(v[t].v[i], a.scale, -lse), FAR);
+                const float p = __builtin_amdgcn_exp2f(log * LOG2E);
+                y.v[i] = -p * __builtin_fmaf(gh, log + entropy, g);
+                if (j + i == token) y.v[i] += g;
+            }
+            store_piece(out + j, y, n);
+        }
+    }
+}
+
+}  // namespace
+
+size_t token_logprobs_workspace_size(int M, int N, int top) {
+    const Split p = split_of(M, N);
+    return p.parts == 1 ? 0 : (size_t)M * p.parts * (sizeof(uint64_t) * top + 16);
+}
+
+hipError_t launch_token_logprobs(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens, float* logp,
+                                 float* lse, float* entropy, int top, int32_t* top_ids, float* top_logp, int M, int N, void* ws,
+                                 hipStream_t s) {
+    const Split p = split_of(M, N);
+    LogprobArgs a{logits, tokens, logp, lse, entropy, top_ids, top_logp, stride, scale, scale * LOG2E,
+                  M, N, top, p.parts, p.width, nullptr, nullptr};
+    if (p.parts > 1) {
+        a.keys = static_cast<uint64_t*>(ws);
+        a.sums = reinterpret_cast<Sums*>(a.keys + (size_t)M * p.parts * top);
+    }
+    return dtype == JH_F32 ? launch<float>(a, s) : launch<uint16_t>(a, s);
+}
+
+hipError_t launch_token_logprobs_bwd(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens,
+                                     const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
+                                     void* dlogits, int64_t out_stride, int M, int N, hipStream_t s) {
+    const GradArgs a{logits, tokens, lse, entropy, dlogp, dentropy, dlogits, stride, out_stride, scale, M, N,
+                     N / GRAD_CHUNK + (N % GRAD_CHUNK != 0)};
+    const unsigned grid = (unsigned)std::min((int64_t)M * a.chunks, (int64_t)1 << 20);
+    if (dtype == JH_F32)
+        logprobs_bwd_kernel<float><<<grid, 256, 0, s>>>(a);
+    else
+        logprobs_bwd_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace jh

@@ -17,49 +17,14 @@
 
 #include "common.hpp"
 #include "launch.hpp"
+#include "pieces.hpp"
 
 namespace jh {
 namespace {
 
-struct f32x8_t {
-    float v[8];
-};
-
-// 8 elements of a row at any address that is a multiple of the element's size
-template <typename T>
-__device__ __forceinline__ f32x8_t load8(const T* p) {
-    f32x8_t r;
-    if constexpr (sizeof(T) == 4) {
-        const f32x4_t a = reinterpret_cast<const f32x4_any_t*>(p)[0].v, b = reinterpret_cast<const f32x4_any_t*>(p)[1].v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.v[i] = a[i], r.v[4 + i] = b[i];
-    } else {
-        const u32x4_t u = reinterpret_cast<const u32x4_any2_t*>(p)->v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.v[2 * i] = bf16_lo(u[i]), r.v[2 * i + 1] = bf16_hi(u[i]);
-    }
-    return r;
-}
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ float load1(const uint16_t* p) { return bf16_lo(*p); }
-
 struct __attribute__((packed, aligned(1))) u32x2_any1_t {
     u32x2_t v;
 };
-
-__device__ __forceinline__ void store8(float* p, const f32x8_t& r) {
-    reinterpret_cast<f32x4_any_t*>(p)[0].v = f32x4_t{r.v[0], r.v[1], r.v[2], r.v[3]};
-    reinterpret_cast<f32x4_any_t*>(p)[1].v = f32x4_t{r.v[4], r.v[5], r.v[6], r.v[7]};
-}
-__device__ __forceinline__ void store8(uint16_t* p, const f32x8_t& r) {
-    reinterpret_cast<u32x4_any2_t*>(p)->v = u32x4_t{pack_bf16x2(r.v[0], r.v[1]), pack_bf16x2(r.v[2], r.v[3]),
-                                                    pack_bf16x2(r.v[4], r.v[5]), pack_bf16x2(r.v[6], r.v[7])};
-}
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(uint16_t* p, float v) { *p = (uint16_t)pack_bf16x2(v, 0.0f); }
-
-// the larger of two, NaN where one is NaN (fmaxf drops it): one instruction on gfx950
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // sum and largest of the group's values, the same order for every row.  The waves'
 // parts alternate between two places, so that one barrier a row is enough: a wave

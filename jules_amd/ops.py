@@ -11,6 +11,7 @@ reference's jules::kernel functions (include/jules/Kernel/FusedKernels.h,
 FlashAttention.h).
 """
 import ctypes
+from typing import NamedTuple, Optional
 
 import numpy as np
 
@@ -404,6 +405,260 @@ def add_rmsnorm_int8(x, residual, weight, eps=1e-5, out=None, scale=None, residu
     with y = q * scale to half a step, q and scale being the A and scale_a of
     matmul_w8a8."""
     return _add_rmsnorm(x, residual, weight, eps, out, (torch.int8,), scale, residual_out)
+
+
+def _drop_args(p, rng, offset):
+    """Dropout's p, rng and offset as the C ABI takes them."""
+    p = float(p)
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"p {p} must be at least 0 and below 1")
+    if p > 0.0 or rng is not None:
+        _need(rng, "rng", (torch.int64,), numel=2)
+    if not 0 <= offset < 2**64:
+        raise ValueError(f"offset {offset} must be within 64 bits")
+    return p, _ptr(rng), int(offset)
+
+
+def dropout(x, p, rng=None, offset=0, residual=None, dtype=None, out=None):
+    """[residual +] x with each element dropped with probability p and the others
+    scaled by 1 / (1 - p) (jules_hip_dropout; no counterpart in the reference).  No
+    mask is stored: which elements are dropped follows from their place in
+    [M, N] (N the last dimension), p, rng (int64 [2] on the device: seed and position,
+    read when the kernel runs) and offset, so the gradient is
+    dropout(grad, p, rng, offset) with rng as it was.  p is rounded to a multiple of
+    2^-16.  x fp32 or bf16; the result of `dtype` (x's), or of residual's and of
+    its shape.  out may be x or residual."""
+    _need(x, "x", _REAL)
+    p, rng_ptr, offset = _drop_args(p, rng, offset)
+    if residual is not None:
+        _need(residual, "residual", _REAL if dtype is None else (dtype,), shape=x.shape)
+        dtype = residual.dtype
+    elif dtype is None:
+        dtype = x.dtype if out is None else out.dtype
+    if dtype not in _DT:
+        raise ValueError(f"dtype {dtype} not in {tuple(_DT)}")
+    if out is not None:
+        _need(out, "out", (dtype,), shape=x.shape)
+    _one_device(("x", "rng", "residual", "out"), x, rng, residual, out)
+    if out is None:
+        out = torch.empty_like(x, dtype=dtype)
+    M, N = _rows(x)
+    _call(x, lib().jules_hip_dropout, _DT[x.dtype], _DT[dtype], p, rng_ptr, offset, x.data_ptr(), _ptr(residual), out.data_ptr(),
+          M, N)
+    return out
+
+
+def add_layernorm(x, residual=None, gamma=None, beta=None, eps=1e-5, p=0.0, rng=None, offset=0, out=None, h=None, mean=None,
+                  rstd=None):
+    """h = residual + dropout(x), y = (h - mean(h)) / sqrt(var(h) + eps) * gamma +
+    beta over the last dimension (jules_hip_add_layernorm; no counterpart in the
+    reference, whose fusedLayerNorm is layernorm above).  x and residual fp32 or bf16, each by
+    itself, residual or None; gamma, beta fp32 or None (ones, zeros); p, rng,
+    offset: dropout's.  Returns (y, h, mean, rstd), what add_layernorm_bwd takes: y of x's dtype (or of
+    out's), h of residual's, or of x's without one (x itself where p is 0), mean and rstd
+    fp32.  out may be x, h may be residual."""
+    _need(x, "x", _REAL)
+    M, N = _rows(x)
+    p, rng_ptr, offset = _drop_args(p, rng, offset)
+    if gamma is not None:
+        _need(gamma, "gamma", (torch.float32,), numel=N)
+    if beta is not None:
+        _need(beta, "beta", (torch.float32,), numel=N)
+    if residual is not None:
+        _need(residual, "residual", _REAL, shape=x.shape)
+    if h is not None:
+        _need(h, "h", _REAL if residual is None else (residual.dtype,), shape=x.shape)
+    if out is not None:
+        _need(out, "out", _REAL, shape=x.shape)
+    if mean is not None:
+        _need(mean, "mean", (torch.float32,), numel=M)
+    if rstd is not None:
+        _need(rstd, "rstd", (torch.float32,), numel=M)
+    _one_device(("x", "residual", "gamma", "beta", "rng", "out", "h", "mean", "rstd"), x, residual, gamma, beta, rng, out, h, mean,
+                rstd)
+    if h is None and (residual is not None or p > 0.0):
+        h = torch.empty_like(x if residual is None else residual)
+    if out is None:
+        out = torch.empty_like(x)
+    if mean is None:
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    if rstd is None:
+        rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _call(x, lib().jules_hip_add_layernorm, _DT[x.dtype], F32 if h is None else _DT[h.dtype], _DT[out.dtype], p, rng_ptr, offset,
+          x.data_ptr(), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(h), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), M, N,
+          float(eps))
+    return out, x if h is None else h, mean, rstd
+
+
+def add_layernorm_bwd_workspace(M, N, device):
+    nbytes = lib().jules_hip_add_layernorm_bwd_workspace_size(int(M), int(N))
+    return torch.empty((max(nbytes, 4) // 4,), dtype=torch.float32, device=device)
+
+
+def add_layernorm_bwd(dy, h, mean, rstd, gamma=None, dh=None, p=0.0, rng=None, offset=0, dx=None, dresidual=None, dgamma=None,
+                      dbeta=None, weight_grads=True, workspace=None):
+    """Gradients of add_layernorm (jules_hip_add_layernorm_bwd): dy of y's dtype, h,
+    mean and rstd as it returned them, gamma, p, rng (as it was) and offset those
+    that it was given, dh (of h's dtype) what reaches h past the norm.  Returns
+    (dx, dresidual, dgamma, dbeta): dresidual, of h's dtype, is the gradient of h;
+    dx, of dy's, that of x, which is dresidual itself where p is 0, the types are
+    the same and neither was passed; dgamma, dbeta fp32 [N], None where
+    weight_grads is false.  dx may be dy, dresidual may be dh."""
+    _need(dy, "dy", _REAL)
+    M, N = _rows(dy)
+    _need(h, "h", _REAL, shape=dy.shape)
+    _need(mean, "mean", (torch.float32,), numel=M)
+    _need(rstd, "rstd", (torch.float32,), numel=M)
+    p, rng_ptr, offset = _drop_args(p, rng, offset)
+    if gamma is not None:
+        _need(gamma, "gamma", (torch.float32,), numel=N)
+    if dh is not None:
+        _need(dh, "dh", (h.dtype,), shape=h.shape)
+    if dx is not None:
+        _need(dx, "dx", (dy.dtype,), shape=dy.shape)
+    if dresidual is not None:
+        _need(dresidual, "dresidual", (h.dtype,), shape=h.shape)
+    if not weight_grads and (dgamma is not None or dbeta is not None):
+        raise ValueError("dgamma or dbeta without weight_grads")
+    if dgamma is not None:
+        _need(dgamma, "dgamma", (torch.float32,), numel=N)
+    if dbeta is not None:
+        _need(dbeta, "dbeta", (torch.float32,), numel=N)
+    ws_bytes = 0 if workspace is None else _workspace(workspace, "workspace")
+    _one_device(("dy", "h", "mean", "rstd", "gamma", "dh", "rng", "dx", "dresidual", "dgamma", "dbeta", "workspace"), dy, h, mean,
+                rstd, gamma, dh, rng, dx, dresidual, dgamma, dbeta, workspace)
+    one = p == 0.0 and dy.dtype == h.dtype and dx is None and dresidual is None
+    if dresidual is None:
+        dresidual = torch.empty_like(h)
+    if dx is None and not one:
+        dx = torch.empty_like(dy)
+    if weight_grads:
+        if dgamma is None:
+            dgamma = dy.new_empty((N,), dtype=torch.float32)
+        if dbeta is None:
+            dbeta = dy.new_empty((N,), dtype=torch.float32)
+        if workspace is None:
+            workspace = add_layernorm_bwd_workspace(M, N, dy.device)
+            ws_bytes = workspace.numel() * 4
+    _call(dy, lib().jules_hip_add_layernorm_bwd, _DT[dy.dtype], _DT[h.dtype], p, rng_ptr, offset, dy.data_ptr(), h.data_ptr(), _ptr(dh),
+          mean.data_ptr(), rstd.data_ptr(), _ptr(gamma), _ptr(dx), dresidual.data_ptr(), _ptr(dgamma), _ptr(dbeta), M, N,
+          _ptr(workspace), ws_bytes)
+    return dresidual if one else dx, dresidual, dgamma, dbeta
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns, or writes into."""
+    logp: Optional[torch.Tensor] = None
+    lse: Optional[torch.Tensor] = None
+    entropy: Optional[torch.Tensor] = None
+    top_ids: Optional[torch.Tensor] = None
+    top_logp: Optional[torch.Tensor] = None
+
+
+def _row_stride(t, name):
+    """Elements between two rows of a tensor whose last dimension is dense and whose
+    others lie as those of a dense one would, rows of a padded width among them."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
+        raise ValueError(f"{name}: fp32 or bf16 tensor expected")
+    if t.dim() < 1:
+        raise ValueError(f"{name} must have at least one dimension")
+    N = t.shape[-1]
+    if t.is_contiguous():
+        return N
+    if N > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last stride must be 1")
+    step = span = None
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if step is None:
+            step = stride
+        elif stride != span:
+            raise ValueError(f"{name}: rows must be equally far apart")
+        span = stride * size
+    if step is None:
+        return N
+    if step < N:
+        raise ValueError(f"{name}: rows overlap")
+    return step
+
+
+def token_logprobs_workspace(M, N, top, device):
+    nbytes = lib().jules_hip_token_logprobs_workspace_size(int(M), int(N), int(top))
+    return torch.empty((max(nbytes, 8) // 8 + 1,), dtype=torch.int64, device=device)
+
+
+def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=None):
+    """Log probabilities of `tokens` under softmax(scale * logits) over the last
+    dimension, with the log-sum-exp, the entropy and the `top` likeliest tokens of
+    each row (jules_hip_token_logprobs; no counterpart in the reference, whose
+    fusedCrossEntropyLoss is cross_entropy).  logits fp32 or bf16 [..., N], N up to
+    2^22, rows equally far apart (logits[..., :N] of a padded width); tokens
+    int32, one a row, a negative one for none (logp 0), or None; top at most 64.
+    Returns TokenLogprobs(logp, lse, entropy, top_ids, top_logp): fp32 of logits' leading shape, the last two
+    [..., top] int32 and fp32 (None where top is 0), by falling logit and rising index.  out: a
+    TokenLogprobs to write into, whose entries that are None are not wanted."""
+    stride = _row_stride(logits, "logits")
+    M, N = _rows(logits)
+    lead = logits.shape[:-1]
+    top = int(top)
+    if top < 0 or top > 64 or top > N:
+        raise ValueError(f"top {top} must be at most 64 and {N}")
+    if tokens is not None:
+        _need(tokens, "tokens", (torch.int32,), numel=M)
+    if out is not None:
+        if out.logp is not None and tokens is None:
+            raise ValueError("logp without tokens")
+        for name, t in (("logp", out.logp), ("lse", out.lse), ("entropy", out.entropy)):
+            if t is not None:
+                _need(t, name, (torch.float32,), numel=M)
+        if (out.top_ids is not None or out.top_logp is not None) and not top:
+            raise ValueError("top_ids or top_logp where top is 0")
+        if top:
+            _need(out.top_ids, "top_ids", (torch.int32,), numel=M * top)
+            _need(out.top_logp, "top_logp", (torch.float32,), numel=M * top)
+    ws_bytes = 0 if workspace is None else _workspace(workspace, "workspace")
+    _one_device(("logits", "tokens", "workspace", *TokenLogprobs._fields), logits, tokens, workspace,
+                *((None,) * 5 if out is None else out))
+    if out is None:
+        new = logits.new_empty
+        out = TokenLogprobs(None if tokens is None else new(lead, dtype=torch.float32), new(lead, dtype=torch.float32),
+                            new(lead, dtype=torch.float32), new((*lead, top), dtype=torch.int32) if top else None,
+                            new((*lead, top), dtype=torch.float32) if top else None)
+    if workspace is None:
+        ws_bytes = lib().jules_hip_token_logprobs_workspace_size(M, N, top)
+        if ws_bytes:
+            workspace = logits.new_empty((ws_bytes,), dtype=torch.uint8)
+    _call(logits, lib().jules_hip_token_logprobs, _DT[logits.dtype], logits.data_ptr(), stride, float(scale), _ptr(tokens),
+          _ptr(out.logp), _ptr(out.lse), _ptr(out.entropy), top, _ptr(out.top_ids), _ptr(out.top_logp), M, N, _ptr(workspace),
+          ws_bytes)
+    return out
+
+
+def token_logprobs_bwd(logits, tokens, lse, dlogp, entropy=None, dentropy=None, scale=1.0, out=None):
+    """The gradient of token_logprobs' logp and entropy with respect to the logits
+    (jules_hip_token_logprobs_bwd), in their dtype: logits, tokens and scale as they were, lse and
+    entropy as it returned them, dlogp and dentropy (or None) fp32, one a row.  out may be logits."""
+    stride = _row_stride(logits, "logits")
+    M, N = _rows(logits)
+    _need(tokens, "tokens", (torch.int32,), numel=M)
+    _need(lse, "lse", (torch.float32,), numel=M)
+    _need(dlogp, "dlogp", (torch.float32,), numel=M)
+    if dentropy is not None:
+        _need(dentropy, "dentropy", (torch.float32,), numel=M)
+        _need(entropy, "entropy", (torch.float32,), numel=M)
+    elif entropy is not None:
+        _need(entropy, "entropy", (torch.float32,), numel=M)
+    if out is not None:
+        out_stride = _row_stride(out, "out")
+        if out.shape != logits.shape or out.dtype != logits.dtype:
+            raise ValueError(f"out: {out.dtype} {tuple(out.shape)}, expected {logits.dtype} {tuple(logits.shape)}")
+    _one_device(("logits", "tokens", "lse", "dlogp", "entropy", "dentropy", "out"), logits, tokens, lse, dlogp, entropy, dentropy, out)
+    if out is None:
+        out, out_stride = torch.empty_like(logits, memory_format=torch.contiguous_format), N
+    _call(logits, lib().jules_hip_token_logprobs_bwd, _DT[logits.dtype], logits.data_ptr(), stride, float(scale), tokens.data_ptr(),
+          lse.data_ptr(), _ptr(entropy), dlogp.data_ptr(), _ptr(dentropy), out.data_ptr(), out_stride, M, N)
+    return out
 
 
 def rotary_frequencies(rotary_dim, sections=None, base=10000.0, device="cuda"):
