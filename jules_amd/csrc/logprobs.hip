@@ -11,15 +11,14 @@
 // block joins them at the end.
 //
 // The k alternatives are the first in the order (value falling, index rising).
-// Each thread also keeps the largest value of each of its pieces.  The k-th
-// largest pair (value, piece) among the threads' largest bounds what can be among
-// the first k, since k threads hold one at least as large; at most k threads reach
-// it, so at most 8 NP k elements do.  Those threads read their pieces that reach
-// it again and put the elements in LDS, where each counts those before it.
+// Each thread also keeps its largest value and the first of its pieces that has
+// it.  The k-th of these pairs (value, piece) bounds what can be among the first
+// k, since k threads hold an element at least as far in front; only those k
+// threads can hold more.  They read their pieces again and put the elements that
+// reach the bound in LDS, where each counts those before it.
 //
-// A row may be split over blocks (few rows, or more than 65536 elements); the
-// blocks' results, their k alternatives among them, are then joined by a second
-// kernel.
+// A row may be split over blocks, whose results, their k alternatives among them,
+// are then joined by a second kernel.
 //
 //   dx_j = scale (g ([j = t] - p_j) - gh p_j (ln p_j + entropy)),  p = e^(z - lse)
 #include <algorithm>
@@ -34,8 +33,9 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // where a distance from the maximum is -infinity: e^ of it is 0, and so is its product with that
 constexpr float FAR = -1e30f;
-constexpr int MAX_TOP = kMaxLogprobTop;
-constexpr int MAX_PARTS = kMaxLogprobVocab / 65536;
+constexpr int MAX_PARTS = 64;
+// keys in LDS, 64 KB of it less the other shared values
+constexpr int MAX_KEYS = 8064;
 
 // a float's place in an order of unsigned numbers, 0 where nothing is; -0 is +0
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -45,9 +45,17 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t o) {
     return __uint_as_float(o ^ ((int32_t)o < 0 ? 0x80000000u : 0xffffffffu));
 }
-// (value falling, place rising)
+// key of (value falling, place rising)
 __device__ __forceinline__ uint64_t key_of(float v, uint32_t place) { return (uint64_t)order_of(v) << 32 | (0xffffffffu - place); }
 __device__ __forceinline__ uint32_t place_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+
+// The largest of three, NaN where one is NaN.  As an instruction of its own: the
+// builtin's operands are first multiplied by 1 to quieten NaNs, an instruction an element.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float r;
+    asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 // maximum, and the sums relative to it: e^((x - m) scale), and that times its exponent in powers of 2
 struct Sums {
@@ -122,19 +130,69 @@ __device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, int
 // how many of n keys in LDS come before this one
 __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
     int rank = 0;
+#pragma unroll 4
     for (int i = 0; i < n; ++i) rank += keys[i] > key;
     return rank;
 }
 
-template <typename T, int BT, int NP, bool TOP>
-__global__ __launch_bounds__(BT) void logprobs_kernel(LogprobArgs a) {
-    constexpr int WAVES = BT / 64, B = NP < 4 ? NP : 4;
-    __shared__ Sums wave_sums[WAVES];
-    __shared__ uint64_t keys[TOP ? std::max(BT, MAX_TOP * 8 * NP + 8) : 1];
+// A part's alternatives, their keys in LDS, in any order: bound, see above.  `best` and
+// `best_piece` (-1: none) are the thread's.  Returns how many reached the bound, at least the `top` first
+// where there are as many; keys has room for the elements of `top` threads, and for one of each thread.
+template <typename T, int BT>
+__device__ __forceinline__ int find_top(uint64_t* keys, const T* x, int first, int len, int top, float best, int best_piece) {
     __shared__ uint32_t groups[64];
     __shared__ int found[2];
     __shared__ uint64_t threshold;
     __shared__ uint32_t group_threshold;
+    const int tid = threadIdx.x;
+    const uint64_t own = best_piece < 0 ? 0 : key_of(best, (uint32_t)best_piece);
+    // the top-th largest of 64 groups' largest values bounds the threads' from below
+    uint32_t g = (uint32_t)(own >> 32);
+#pragma unroll
+    for (int o = 1; o < BT / 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor((int)g, o));
+    if (tid % (BT / 64) == 0) groups[tid / (BT / 64)] = g;
+    if (tid < 2) found[tid] = 0;
+    if (tid == 0) threshold = 0;
+    __syncthreads();
+    if (tid < 64) {
+        g = groups[tid];
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)g, i);
+            rank += o > g || (o == g && i < tid);
+        }
+        if (rank == top - 1) group_threshold = g;
+    }
+    __syncthreads();
+    // the top-th of the threads'
+    if (own && (uint32_t)(own >> 32) >= group_threshold) keys[atomicAdd(&found[0], 1)] = own;
+    __syncthreads();
+    const int threads = found[0];
+    if (tid < threads && rank_of(keys[tid], keys, threads) == top - 1) threshold = keys[tid];
+    __syncthreads();
+    // those threads' elements that reach it
+    const uint64_t bound = threshold;
+    if (own && own >= bound) {
+        for (int piece = tid; 8 * piece < len; piece += BT) {
+            const int n = min(8, len - 8 * piece);
+            const f32x8_t v = load_piece(x + 8 * piece, n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n && key_of(v.v[i], (uint32_t)piece) >= bound)
+                    keys[atomicAdd(&found[1], 1)] = key_of(v.v[i], (uint32_t)(first + 8 * piece + i));
+        }
+    }
+    __syncthreads();
+    return found[1];
+}
+
+// BT threads for a part of a row, in turns of B pieces each.  Dynamic LDS with TOP: key_bytes()
+template <typename T, int BT, bool TOP>
+__global__ __launch_bounds__(BT, 8) void logprobs_kernel(LogprobArgs a) {
+    constexpr int WAVES = BT / 64, B = TOP ? 2 : 4;  // 64 registers: two blocks of 1024 a CU
+    __shared__ Sums wave_sums[WAVES];
+    extern __shared__ uint64_t keys[];
     const int tid = threadIdx.x;
     for (int64_t item = blockIdx.x; item < (int64_t)a.M * a.parts; item += gridDim.x) {
         const int64_t row = item / a.parts;
@@ -142,35 +200,29 @@ __global__ __launch_bounds__(BT) void logprobs_kernel(LogprobArgs a) {
         const int first = part * a.width, len = min(a.width, a.N - first);
         const T* x = static_cast<const T*>(a.logits) + row * a.stride + first;
         Sums mine = no_sums();
-        float u[TOP ? NP : 1];
         float best = -INFINITY;
         int best_piece = -1;
-#pragma unroll
-        for (int b = 0; b < NP; b += B) {
+        for (int b = tid; 8 * b < len; b += B * BT) {
             f32x8_t v[B];
 #pragma unroll
             for (int t = 0; t < B; ++t) {
-                const int j = 8 * (tid + BT * (b + t)), n = min(8, len - j);
+                const int j = 8 * (b + BT * t), n = min(8, len - j);
                 if (n > 0) v[t] = load_piece(x + j, n, -INFINITY);
             }
             float m = mine.m;
 #pragma unroll
             for (int t = 0; t < B; ++t) {
-                const int piece = tid + BT * (b + t);
+                const int piece = b + BT * t;
                 if (8 * piece >= len) continue;
-                float top = v[t].v[0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) top = larger(top, v[t].v[i]);
+                const float* e = v[t].v;
+                const float top = largest(largest(e[0], e[1], e[2]), largest(e[3], e[4], e[5]), largest(e[6], e[7], e[7]));
                 m = larger(m, top);
-                if constexpr (TOP) {
-                    u[b + t] = top;
-                    if (top > best || best_piece < 0) best = top, best_piece = piece;
-                }
+                if (TOP && (top > best || best_piece < 0)) best = top, best_piece = piece;
             }
             raise(&mine, m, a.c2);
 #pragma unroll
             for (int t = 0; t < B; ++t) {
-                if (8 * (tid + BT * (b + t)) >= len) continue;
+                if (8 * (b + BT * t) >= len) continue;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float d = larger((v[t].v[i] - m) * a.c2, FAR), e = __builtin_amdgcn_exp2f(d);
@@ -183,18 +235,11 @@ __global__ __launch_bounds__(BT) void logprobs_kernel(LogprobArgs a) {
         for (int o = 32; o > 0; o >>= 1)
             mine = join(mine, Sums{__shfl_xor(mine.m, o), __shfl_xor(mine.s, o), __shfl_xor(mine.w, o)}, a.c2);
         if ((tid & 63) == 0) wave_sums[tid >> 6] = mine;
-        if constexpr (TOP) {
-            uint32_t g = best_piece < 0 ? 0 : order_of(best);
-#pragma unroll
-            for (int o = 1; o < BT / 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor((int)g, o));
-            if (tid % (BT / 64) == 0) groups[tid / (BT / 64)] = g;
-            if (tid < 2) found[tid] = 0;
-            if (tid == 0) threshold = 0;
-        }
         __syncthreads();
-        Sums all = wave_sums[0];
+        Sums all = wave_sums[tid % WAVES];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) all = join(all, wave_sums[w], a.c2);
+        for (int o = 1; o < WAVES; o <<= 1)
+            all = join(all, Sums{__shfl_xor(all.m, o), __shfl_xor(all.s, o), __shfl_xor(all.w, o)}, a.c2);
         const RowNumbers r = row_numbers(all);
         if (a.parts > 1) {
             if (tid == 0) a.sums[item] = all;
@@ -203,128 +248,102 @@ __global__ __launch_bounds__(BT) void logprobs_kernel(LogprobArgs a) {
         }
         if constexpr (TOP) {
             uint64_t* part_keys = a.parts > 1 ? a.keys + item * a.top : nullptr;
-            if (r.bad) {  // no order among these
-                for (int i = tid; i < a.top; i += BT) {
-                    if (part_keys)
-                        part_keys[i] = 0;
-                    else
-                        write_top(a, row, i, 0, r);
-                }
-            } else {
-                // the top-th largest of 64 groups' largest values: a bound from below
-                if (tid < 64) {
-                    const uint32_t g = groups[tid];
-                    int rank = 0;
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)g, i);
-                        rank += o > g || (o == g && i < tid);
-                    }
-                    if (rank == a.top - 1) group_threshold = g;
-                }
-                __syncthreads();
-                // the top-th largest of the threads'
-                const uint64_t own = best_piece < 0 ? 0 : key_of(best, (uint32_t)best_piece);
-                if (own && (uint32_t)(own >> 32) >= group_threshold) keys[atomicAdd(&found[0], 1)] = own;
-                __syncthreads();
-                const int threads = found[0];
-                if (tid < threads && rank_of(keys[tid], keys, threads) == a.top - 1) threshold = keys[tid];
-                __syncthreads();
-                // their elements that reach it
-                const uint64_t bound = threshold;
-                if (own && own >= bound) {
-#pragma unroll
-                    for (int t = 0; t < NP; ++t) {
-                        const int piece = tid + BT * t, n = min(8, len - 8 * piece);
-                        if (n <= 0 || key_of(u[t], (uint32_t)piece) < bound) continue;
-                        const f32x8_t v = load_piece(x + 8 * piece, n);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i < n && key_of(v.v[i], (uint32_t)piece) >= bound)
-                                keys[atomicAdd(&found[1], 1)] = key_of(v.v[i], (uint32_t)(first + 8 * piece + i));
-                    }
-                }
-                __syncthreads();
-                const int n = found[1];
-                if (part_keys && tid >= n && tid < a.top) part_keys[tid] = 0;  // a part shorter than that
-                for (int i = tid; i < n; i += BT) {
-                    const uint64_t key = keys[i];
-                    const int rank = rank_of(key, keys, n);
-                    if (rank >= a.top) continue;
-                    if (part_keys)
-                        part_keys[rank] = key;
-                    else
-                        write_top(a, row, rank, key, r);
-                }
+            // no order where there is a NaN or +infinity
+            const int n = r.bad ? 0 : find_top<T, BT>(keys, x, first, len, a.top, best, best_piece);
+            if (tid < a.top && (r.bad || tid >= n)) {  // a part may be shorter than `top`, a row not
+                if (part_keys)
+                    part_keys[tid] = 0;
+                else
+                    write_top(a, row, tid, 0, r);
+            }
+            for (int i = tid; i < n; i += BT) {
+                const uint64_t key = keys[i];
+                const int rank = rank_of(key, keys, n);
+                if (rank >= a.top) continue;
+                if (part_keys)
+                    part_keys[rank] = key;
+                else
+                    write_top(a, row, rank, key, r);
             }
         }
         __syncthreads();  // the shared values are the next item's
     }
 }
 
-// rows that were split: a block each
+// Rows that were split: a block each.  Every part's keys are sorted, so the smallest of
+// the parts' k/parts-th bounds the row's k-th from below: few keys reach it.
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
-    __shared__ uint64_t keys[MAX_PARTS * MAX_TOP];
+    extern __shared__ uint64_t keys[];
+    __shared__ int found;
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        Sums all = no_sums();
-        for (int p = 0; p < a.parts; ++p) all = join(all, a.sums[row * a.parts + p], a.c2);
+        const int n = a.parts * a.top, lane = threadIdx.x & 63;
+        const uint64_t* row_keys = a.keys + row * n;
+        uint64_t bound = ~(uint64_t)0;
+        if (lane < a.parts && a.top) bound = row_keys[lane * a.top + (a.top - 1) / a.parts];
+        Sums all = lane < a.parts ? a.sums[row * a.parts + lane] : no_sums();
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            all = join(all, Sums{__shfl_xor(all.m, o), __shfl_xor(all.s, o), __shfl_xor(all.w, o)}, a.c2);
+            const uint64_t other = __shfl_xor(bound, o);
+            bound = other < bound ? other : bound;
+        }
         const RowNumbers r = row_numbers(all);
         if (threadIdx.x == 0) write_row<T>(a, row, r);
         if (!a.top) continue;
-        const int n = a.parts * a.top;
-        for (int i = threadIdx.x; i < n; i += 256) keys[i] = a.keys[row * n + i];
+        if (r.bad) {
+            if (threadIdx.x < a.top) write_top(a, row, threadIdx.x, 0, r);
+            continue;
+        }
+        if (threadIdx.x == 0) found = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += 256) {
-            const uint64_t key = keys[i];
-            if (r.bad) {
-                if (i < a.top) write_top(a, row, i, 0, r);
-            } else if (key) {
-                const int rank = rank_of(key, keys, n);
-                if (rank < a.top) write_top(a, row, rank, key, r);
-            }
+            const uint64_t key = row_keys[i];
+            if (key && key >= bound) keys[atomicAdd(&found, 1)] = key;
+        }
+        __syncthreads();
+        const int reached = found;
+        for (int i = threadIdx.x; i < reached; i += 256) {
+            const int rank = rank_of(keys[i], keys, reached);
+            if (rank < a.top) write_top(a, row, rank, keys[i], r);
         }
         __syncthreads();
     }
 }
 
 struct Split {
-    int parts, width;
+    int parts, width, threads;
 };
-Split split_of(int M, int N) {
-    int parts = N / 65536 + (N % 65536 != 0);
-    if (M < 256) parts = std::max(parts, std::min((512 + M - 1) / M, N / 2048));
+Split split_of(int M, int N, int top) {
+    // what the keys in LDS allow: `top` threads' elements
+    const int most = top ? MAX_KEYS / (8 * top) * (8 * 1024) : N;
+    int parts = N / most + (N % most != 0);
+    if (M < 192) parts = std::max(parts, std::min((256 + M - 1) / M, N / 4096));
     parts = std::min(std::max(parts, 1), MAX_PARTS);
     const int width = (N / parts + (N % parts != 0) + 7) / 8 * 8;
-    return Split{N / width + (N % width != 0), width};
+    return Split{N / width + (N % width != 0), width, width <= 8192 ? 256 : 1024};
 }
 
-template <typename T, int BT, int NP>
-void launch_part(const LogprobArgs& a, hipStream_t s) {
+template <typename T, int BT>
+void launch_parts(const LogprobArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)std::min((int64_t)a.M * a.parts, (int64_t)1 << 20);
-    if (a.top)
-        logprobs_kernel<T, BT, NP, true><<<grid, BT, 0, s>>>(a);
-    else
-        logprobs_kernel<T, BT, NP, false><<<grid, BT, 0, s>>>(a);
+    if (a.top) {
+        const int turns = a.width / (8 * BT) + (a.width % (8 * BT) != 0);
+        logprobs_kernel<T, BT, true><<<grid, BT, sizeof(uint64_t) * std::max(BT, 8 * turns * a.top), s>>>(a);
+    } else {
+        logprobs_kernel<T, BT, false><<<grid, BT, 0, s>>>(a);
+    }
 }
 
 template <typename T>
-hipError_t launch(const LogprobArgs& a, hipStream_t s) {
-    if (a.width <= 2048)
-        launch_part<T, 256, 1>(a, s);
-    else if (a.width <= 4096)
-        launch_part<T, 256, 2>(a, s);
-    else if (a.width <= 8192)
-        launch_part<T, 256, 4>(a, s);
-    else if (a.width <= 16384)
-        launch_part<T, 256, 8>(a, s);
-    else if (a.width <= 32768)
-        launch_part<T, 1024, 4>(a, s);
+hipError_t launch(const LogprobArgs& a, int threads, hipStream_t s) {
+    if (threads == 256)
+        launch_parts<T, 256>(a, s);
     else
-        launch_part<T, 1024, 8>(a, s);
+        launch_parts<T, 1024>(a, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
-    logprobs_join_kernel<T><<<(unsigned)std::min(a.M, 1 << 20), 256, 0, s>>>(a);
+    logprobs_join_kernel<T><<<(unsigned)std::min(a.M, 1 << 20), 256, sizeof(uint64_t) * a.parts * a.top, s>>>(a);
     return hipGetLastError();
 }
 
@@ -383,21 +402,21 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(GradArgs a) {
 }  // namespace
 
 size_t token_logprobs_workspace_size(int M, int N, int top) {
-    const Split p = split_of(M, N);
+    const Split p = split_of(M, N, top);
     return p.parts == 1 ? 0 : (size_t)M * p.parts * (sizeof(uint64_t) * top + 16);
 }
 
 hipError_t launch_token_logprobs(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens, float* logp,
                                  float* lse, float* entropy, int top, int32_t* top_ids, float* top_logp, int M, int N, void* ws,
                                  hipStream_t s) {
-    const Split p = split_of(M, N);
+    const Split p = split_of(M, N, top);
     LogprobArgs a{logits, tokens, logp, lse, entropy, top_ids, top_logp, stride, scale, scale * LOG2E,
                   M, N, top, p.parts, p.width, nullptr, nullptr};
     if (p.parts > 1) {
         a.keys = static_cast<uint64_t*>(ws);
         a.sums = reinterpret_cast<Sums*>(a.keys + (size_t)M * p.parts * top);
     }
-    return dtype == JH_F32 ? launch<float>(a, s) : launch<uint16_t>(a, s);
+    return dtype == JH_F32 ? launch<float>(a, p.threads, s) : launch<uint16_t>(a, p.threads, s);
 }
 
 hipError_t launch_token_logprobs_bwd(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens,

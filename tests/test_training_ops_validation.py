@@ -114,7 +114,8 @@ def test_token_logprobs_bwd_statuses(change, status):
 def test_logprobs_workspace_size():
     f = _lib.lib().jules_hip_token_logprobs_workspace_size
     assert f(4096, 50257, 20) == 0            # a block a row
-    assert f(1, 128256, 20) > 0 and f(4096, 128256, 0) > 0
+    assert f(4096, 128256, 0) == 0 and f(4096, 128256, 20) == 0
+    assert f(1, 128256, 20) > 0 and f(8, 128256, 0) > 0 and f(4096, 400000, 64) > 0
     assert f(8, 1000, 5) == 0
     for bad in ((0, 100, 1), (1, 0, 1), (1, (1 << 22) + 1, 1), (1, 100000, 65), (1, 100000, -1), (-1, 100000, 1)):
         assert f(*bad) == 0
