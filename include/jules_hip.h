@@ -438,7 +438,7 @@ int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t
 /* ---- log probabilities of tokens, and their gradient ------------------------------
  * z = scale * logits, row by row of [M, N] (rows row_stride elements apart, row_stride
  * >= N: an output layer padded to a round width needs no copy), logits JH_F32 or JH_BF16,
- * 1 <= N <= 2^22, scale between 1e-30 and 1e30.  No counterpart in the reference: jules_hip_cross_entropy gives one mean loss.
+ * 1 <= N <= 2^21, scale between 1e-30 and 1e30.  No counterpart in the reference: jules_hip_cross_entropy gives one mean loss.
  *   lse     = log(sum(exp(z)))               logp = z[token] - lse
  *   entropy = -sum(p log p), p = exp(z - lse)
  *   top_ids, top_logp [M, top]: the indices of the `top` largest logits, falling, equal

@@ -25,11 +25,14 @@ __global__ __launch_bounds__(256) void dropout_kernel(Dropout d, const XT* x, co
     while (row < M) {
         const int n = min(8, N - 8 * piece);
         const int64_t at = row * N + 8 * (int64_t)piece;
-        f32x8_t y = drop8(load_piece(x + at, n), key, d, (uint32_t)row, (uint32_t)piece);
+        const Raw8<XT> raw = load_raw(x + at, n);
+        Raw8<OT> old;
+        if constexpr (RES) old = load_raw(r + at, n);
+        f32x8_t y = drop8(values(raw), key, d, (uint32_t)row, (uint32_t)piece);
         if constexpr (RES) {
-            const f32x8_t old = load_piece(r + at, n);
+            const f32x8_t v = values(old);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y.v[i] += old.v[i];
+            for (int i = 0; i < 8; ++i) y.v[i] += v.v[i];
         }
         store_piece(out + at, y, n);
         row += rows_on;

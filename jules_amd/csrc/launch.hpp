@@ -203,7 +203,7 @@ hipError_t launch_add_layernorm_bwd(int x_dtype, int h_dtype, const Dropout& dro
 // log probabilities of tokens, entropy, alternatives, and the logits' gradient
 // (logprobs.hip); ws: token_logprobs_workspace_size bytes
 constexpr int kMaxLogprobTop = 64;
-constexpr int kMaxLogprobVocab = 1 << 22;
+constexpr int kMaxLogprobVocab = 1 << 21;
 size_t token_logprobs_workspace_size(int M, int N, int top);
 hipError_t launch_token_logprobs(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens,
                                  float* logp, float* lse, float* entropy, int top, int32_t* top_ids, float* top_logp,

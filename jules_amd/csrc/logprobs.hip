@@ -135,18 +135,24 @@ __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n
     return rank;
 }
 
-// A part's alternatives, their keys in LDS, in any order: bound, see above.  `best` and
-// `best_piece` (-1: none) are the thread's.  Returns how many reached the bound, at least the `top` first
-// where there are as many; keys has room for the elements of `top` threads, and for one of each thread.
+// A thread's largest value, the first of its pieces that has it (-1: no pieces), and the
+// largest of its other pieces' largest values
+struct Likeliest {
+    float best, next;
+    int piece;
+};
+
+// A part's alternatives, their keys in LDS, in any order.  Returns how many reached the
+// bound (see above), the `top` first among them.  keys has room for the elements of
+// `top` threads, and for one of each thread.
 template <typename T, int BT>
-__device__ __forceinline__ int find_top(uint64_t* keys, const T* x, int first, int len, int top, float best, int best_piece) {
+__device__ __forceinline__ int find_top(uint64_t* keys, const T* x, int first, int len, int top, const Likeliest& l) {
     __shared__ uint32_t groups[64];
     __shared__ int found[2];
     __shared__ uint64_t threshold;
     __shared__ uint32_t group_threshold;
     const int tid = threadIdx.x;
-    const uint64_t own = best_piece < 0 ? 0 : key_of(best, (uint32_t)best_piece);
-    // the top-th largest of 64 groups' largest values bounds the threads' from below
+    const uint64_t own = l.piece < 0 ? 0 : key_of(l.best, (uint32_t)l.piece);
     uint32_t g = (uint32_t)(own >> 32);
 #pragma unroll
     for (int o = 1; o < BT / 64; o <<= 1) g = max(g, (uint32_t)__shfl_xor((int)g, o));
@@ -155,118 +161,146 @@ __device__ __forceinline__ int find_top(uint64_t* keys, const T* x, int first, i
     if (tid == 0) threshold = 0;
     __syncthreads();
     if (tid < 64) {
+        // a number that at least `top` of 64 groups reach, so at least as many threads: the
+        // largest with its first bits, until no more than that reach it
         g = groups[tid];
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) {
-            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)g, i);
-            rank += o > g || (o == g && i < tid);
+        uint32_t at = 0;
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+            const int reach = __popcll(__ballot(g >= (at | bit)));
+            if (reach >= top) at |= bit;
+            if (reach == top) break;
         }
-        if (rank == top - 1) group_threshold = g;
+        if (tid == 0) group_threshold = at;
     }
     __syncthreads();
-    // the top-th of the threads'
+    // the top-th of the threads' best
     if (own && (uint32_t)(own >> 32) >= group_threshold) keys[atomicAdd(&found[0], 1)] = own;
     __syncthreads();
     const int threads = found[0];
     if (tid < threads && rank_of(keys[tid], keys, threads) == top - 1) threshold = keys[tid];
     __syncthreads();
-    // those threads' elements that reach it
+    // those threads' elements that reach it, mostly of one piece each
     const uint64_t bound = threshold;
     if (own && own >= bound) {
-        for (int piece = tid; 8 * piece < len; piece += BT) {
+        const auto take = [&](int piece) {
             const int n = min(8, len - 8 * piece);
-            const f32x8_t v = load_piece(x + 8 * piece, n);
+            const f32x8_t v = values(load_raw(x + 8 * piece, n));
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (i < n && key_of(v.v[i], (uint32_t)piece) >= bound)
                     keys[atomicAdd(&found[1], 1)] = key_of(v.v[i], (uint32_t)(first + 8 * piece + i));
-        }
+        };
+        take(l.piece);
+        if (order_of(l.next) >= (uint32_t)(bound >> 32))
+            for (int piece = tid; 8 * piece < len; piece += BT)
+                if (piece != l.piece) take(piece);
     }
     __syncthreads();
     return found[1];
 }
 
-// BT threads for a part of a row, in turns of B pieces each.  Dynamic LDS with TOP: key_bytes()
+// -infinity as an element's bits
+template <typename T>
+constexpr uint32_t kNothing = sizeof(T) == 4 ? 0xff800000u : 0xff80u;
+
+// pieces b, b + BT, .. of the thread's part
+template <int BT, bool TOP, typename T, int B>
+__device__ __forceinline__ void add_pieces(const Raw8<T> (&raw)[B], int b, float c2, Sums* mine, Likeliest* l) {
+    f32x8_t v[B];
+    float m = mine->m;
+#pragma unroll
+    for (int t = 0; t < B; ++t) {
+        v[t] = values(raw[t]);
+        const float* e = v[t].v;
+        const float top = largest(largest(e[0], e[1], e[2]), largest(e[3], e[4], e[5]), largest(e[6], e[7], e[7]));
+        m = larger(m, top);
+        if constexpr (TOP) {
+            l->next = __builtin_amdgcn_fmed3f(l->next, l->best, top);  // next <= best: the second of the three
+            if (top > l->best || l->piece < 0) l->best = top, l->piece = b + BT * t;
+        }
+    }
+    raise(mine, m, c2);
+#pragma unroll
+    for (int t = 0; t < B; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = larger((v[t].v[i] - m) * c2, FAR), e = __builtin_amdgcn_exp2f(d);
+            mine->s += e;
+            mine->w = __builtin_fmaf(e, d, mine->w);
+        }
+}
+
+// BT threads for a part of a row, in turns of B pieces each.  Dynamic LDS with TOP: launch_parts()
 template <typename T, int BT, bool TOP>
 __global__ __launch_bounds__(BT, 8) void logprobs_kernel(LogprobArgs a) {
-    constexpr int WAVES = BT / 64, B = TOP ? 2 : 4;  // 64 registers: two blocks of 1024 a CU
+    constexpr int WAVES = BT / 64, B = 4;
     __shared__ Sums wave_sums[WAVES];
     extern __shared__ uint64_t keys[];
-    const int tid = threadIdx.x;
-    for (int64_t item = blockIdx.x; item < (int64_t)a.M * a.parts; item += gridDim.x) {
-        const int64_t row = item / a.parts;
-        const int part = (int)(item % a.parts);
-        const int first = part * a.width, len = min(a.width, a.N - first);
+    const int tid = threadIdx.x, part = blockIdx.y;
+    const int first = part * a.width, len = min(a.width, a.N - first);
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const T* x = static_cast<const T*>(a.logits) + row * a.stride + first;
         Sums mine = no_sums();
-        float best = -INFINITY;
-        int best_piece = -1;
-        for (int b = tid; 8 * b < len; b += B * BT) {
-            f32x8_t v[B];
+        Likeliest l{-INFINITY, -INFINITY, -1};
+        int b = tid;
+        for (; 8 * (b + BT * (B - 1)) + 8 <= len; b += B * BT) {
+            Raw8<T> raw[B];
 #pragma unroll
-            for (int t = 0; t < B; ++t) {
-                const int j = 8 * (b + BT * t), n = min(8, len - j);
-                if (n > 0) v[t] = load_piece(x + j, n, -INFINITY);
-            }
-            float m = mine.m;
-#pragma unroll
-            for (int t = 0; t < B; ++t) {
-                const int piece = b + BT * t;
-                if (8 * piece >= len) continue;
-                const float* e = v[t].v;
-                const float top = largest(largest(e[0], e[1], e[2]), largest(e[3], e[4], e[5]), largest(e[6], e[7], e[7]));
-                m = larger(m, top);
-                if (TOP && (top > best || best_piece < 0)) best = top, best_piece = piece;
-            }
-            raise(&mine, m, a.c2);
-#pragma unroll
-            for (int t = 0; t < B; ++t) {
-                if (8 * (b + BT * t) >= len) continue;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float d = larger((v[t].v[i] - m) * a.c2, FAR), e = __builtin_amdgcn_exp2f(d);
-                    mine.s += e;
-                    mine.w = __builtin_fmaf(e, d, mine.w);
-                }
-            }
+            for (int t = 0; t < B; ++t) raw[t] = load_raw(x + 8 * (b + BT * t), 8);
+            add_pieces<BT, TOP>(raw, b, a.c2, &mine, &l);
         }
+#pragma unroll 1
+        for (; 8 * b < len; b += BT) {
+            const Raw8<T> raw[1] = {load_raw(x + 8 * b, min(8, len - 8 * b), kNothing<T>)};
+            add_pieces<BT, TOP>(raw, b, a.c2, &mine, &l);
+        }
+        // the wave's, relative to its maximum, then the block's
+        float m = mine.m;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            mine = join(mine, Sums{__shfl_xor(mine.m, o), __shfl_xor(mine.s, o), __shfl_xor(mine.w, o)}, a.c2);
+        for (int o = 32; o > 0; o >>= 1) m = larger(m, __shfl_xor(m, o));
+        raise(&mine, m, a.c2);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            mine.s += __shfl_xor(mine.s, o);
+            mine.w += __shfl_xor(mine.w, o);
+        }
         if ((tid & 63) == 0) wave_sums[tid >> 6] = mine;
         __syncthreads();
         Sums all = wave_sums[tid % WAVES];
 #pragma unroll
         for (int o = 1; o < WAVES; o <<= 1)
             all = join(all, Sums{__shfl_xor(all.m, o), __shfl_xor(all.s, o), __shfl_xor(all.w, o)}, a.c2);
-        const RowNumbers r = row_numbers(all);
-        if (a.parts > 1) {
-            if (tid == 0) a.sums[item] = all;
-        } else if (tid == 0) {
-            write_row<T>(a, row, r);
-        }
-        if constexpr (TOP) {
-            uint64_t* part_keys = a.parts > 1 ? a.keys + item * a.top : nullptr;
-            // no order where there is a NaN or +infinity
-            const int n = r.bad ? 0 : find_top<T, BT>(keys, x, first, len, a.top, best, best_piece);
-            if (tid < a.top && (r.bad || tid >= n)) {  // a part may be shorter than `top`, a row not
-                if (part_keys)
-                    part_keys[tid] = 0;
+        const int64_t item = row * a.parts + part;
+        if (TOP || tid == 0) {
+            const RowNumbers r = row_numbers(all);
+            if (tid == 0) {
+                if (a.parts > 1)
+                    a.sums[item] = all;
                 else
-                    write_top(a, row, tid, 0, r);
+                    write_row<T>(a, row, r);
             }
-            for (int i = tid; i < n; i += BT) {
-                const uint64_t key = keys[i];
-                const int rank = rank_of(key, keys, n);
-                if (rank >= a.top) continue;
-                if (part_keys)
-                    part_keys[rank] = key;
-                else
-                    write_top(a, row, rank, key, r);
+            if constexpr (TOP) {
+                uint64_t* part_keys = a.parts > 1 ? a.keys + item * a.top : nullptr;
+                // no order where there is a NaN or +infinity
+                const int n = r.bad ? 0 : find_top<T, BT>(keys, x, first, len, a.top, l);
+                if (tid < a.top && (r.bad || tid >= n)) {  // a part may be shorter than `top`, a row not
+                    if (part_keys)
+                        part_keys[tid] = 0;
+                    else
+                        write_top(a, row, tid, 0, r);
+                }
+                for (int i = tid; i < n; i += BT) {
+                    const uint64_t key = keys[i];
+                    const int rank = rank_of(key, keys, n);
+                    if (rank >= a.top) continue;
+                    if (part_keys)
+                        part_keys[rank] = key;
+                    else
+                        write_top(a, row, rank, key, r);
+                }
             }
         }
-        __syncthreads();  // the shared values are the next item's
+        __syncthreads();  // the shared values are the next row's
     }
 }
 
@@ -316,17 +350,17 @@ struct Split {
 };
 Split split_of(int M, int N, int top) {
     // what the keys in LDS allow: `top` threads' elements
-    const int most = top ? MAX_KEYS / (8 * top) * (8 * 1024) : N;
+    const int most = top ? MAX_KEYS / (8 * top) * (8 * 512) : N;
     int parts = N / most + (N % most != 0);
     if (M < 192) parts = std::max(parts, std::min((256 + M - 1) / M, N / 4096));
     parts = std::min(std::max(parts, 1), MAX_PARTS);
     const int width = (N / parts + (N % parts != 0) + 7) / 8 * 8;
-    return Split{N / width + (N % width != 0), width, width <= 8192 ? 256 : 1024};
+    return Split{N / width + (N % width != 0), width, width <= 8192 ? 256 : 512};
 }
 
 template <typename T, int BT>
 void launch_parts(const LogprobArgs& a, hipStream_t s) {
-    const unsigned grid = (unsigned)std::min((int64_t)a.M * a.parts, (int64_t)1 << 20);
+    const dim3 grid((unsigned)std::min(a.M, 1 << 20), (unsigned)a.parts);
     if (a.top) {
         const int turns = a.width / (8 * BT) + (a.width % (8 * BT) != 0);
         logprobs_kernel<T, BT, true><<<grid, BT, sizeof(uint64_t) * std::max(BT, 8 * turns * a.top), s>>>(a);
@@ -340,7 +374,7 @@ hipError_t launch(const LogprobArgs& a, int threads, hipStream_t s) {
     if (threads == 256)
         launch_parts<T, 256>(a, s);
     else
-        launch_parts<T, 1024>(a, s);
+        launch_parts<T, 512>(a, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
     logprobs_join_kernel<T><<<(unsigned)std::min(a.M, 1 << 20), 256, sizeof(uint64_t) * a.parts * a.top, s>>>(a);
@@ -376,20 +410,21 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(GradArgs a) {
         float g = token < 0 || none ? 0.0f : a.dlogp[row] * a.scale;
         const float gh = !a.dentropy || none ? 0.0f : a.dentropy[row] * a.scale;
         if (token >= a.N) g = __builtin_nanf("");
-        f32x8_t v[GRAD_PIECES];
+        Raw8<T> raw[GRAD_PIECES];
 #pragma unroll
         for (int t = 0; t < GRAD_PIECES; ++t) {
             const int j = first + 8 * ((int)threadIdx.x + 256 * t), n = min(8, a.N - j);
-            if (n > 0) v[t] = load_piece(x + j, n);
+            if (n > 0) raw[t] = load_raw(x + j, n);
         }
 #pragma unroll
         for (int t = 0; t < GRAD_PIECES; ++t) {
             const int j = first + 8 * ((int)threadIdx.x + 256 * t), n = min(8, a.N - j);
             if (n <= 0) continue;
+            const f32x8_t v = values(raw[t]);
             f32x8_t y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float log = none ? FAR : larger(__builtin_fmaf(v[t].v[i], a.scale, -lse), FAR);
+                const float log = none ? FAR : larger(__builtin_fmaf(v.v[i], a.scale, -lse), FAR);
                 const float p = __builtin_amdgcn_exp2f(log * LOG2E);
                 y.v[i] = -p * __builtin_fmaf(gh, log + entropy, g);
                 if (j + i == token) y.v[i] += g;

@@ -59,6 +59,48 @@ __device__ __forceinline__ void store_piece(T* p, const f32x8_t& r, int n) {
     }
 }
 
+// A piece as it lies in memory.  Loads that are to be under way together are written
+// as load_raw, their values taken afterwards: a conversion beside the load, in the branch
+// of whole pieces, makes the compiler wait for each before the next.
+template <typename T>
+struct Raw8 {
+    u32x4_t v[sizeof(T) / 2];
+};
+__device__ __forceinline__ uint32_t bits1(const float* p) { return __float_as_uint(*p); }
+__device__ __forceinline__ uint32_t bits1(const uint16_t* p) { return *p; }
+// the first n of 8 elements, n = 1 .. 8; those behind have the bits `rest`
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw(const T* p, int n, uint32_t rest = 0) {
+    Raw8<T> r;
+    if (n == 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const u32x4_any2_t*>(p)[i].v;
+    } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i < n ? bits1(p + i) : rest;
+        if constexpr (sizeof(T) == 4) {
+            r.v[0] = u32x4_t{e[0], e[1], e[2], e[3]};
+            r.v[1] = u32x4_t{e[4], e[5], e[6], e[7]};
+        } else {
+            r.v[0] = u32x4_t{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+        }
+    }
+    return r;
+}
+__device__ __forceinline__ f32x8_t values(const Raw8<float>& r) {
+    f32x8_t x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.v[i] = __uint_as_float(r.v[i / 4][i % 4]);
+    return x;
+}
+__device__ __forceinline__ f32x8_t values(const Raw8<uint16_t>& r) {
+    f32x8_t x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[2 * i] = bf16_lo(r.v[0][i]), x.v[2 * i + 1] = bf16_hi(r.v[0][i]);
+    return x;
+}
+
 // the larger of two, NaN where one is NaN (fmaxf drops it): one instruction on gfx950
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 

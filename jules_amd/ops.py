@@ -593,7 +593,7 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
     dimension, with the log-sum-exp, the entropy and the `top` likeliest tokens of
     each row (jules_hip_token_logprobs; no counterpart in the reference, whose
     fusedCrossEntropyLoss is cross_entropy).  logits fp32 or bf16 [..., N], N up to
-    2^22, rows equally far apart (logits[..., :N] of a padded width); tokens
+    2^21, rows equally far apart (logits[..., :N] of a padded width); tokens
     int32, one a row, a negative one for none (logp 0), or None; top at most 64.
     Returns TokenLogprobs(logp, lse, entropy, top_ids, top_logp): fp32 of logits' leading shape, the last two
     [..., top] int32 and fp32 (None where top is 0), by falling logit and rising index.  out: a

@@ -82,7 +82,7 @@ def test_layernorm_workspace_size():
     assert f(0, 8) == 0 and f(8, 0) == 0 and f(-1, 8) == 0 and f(1 << 21, 1 << 21) == 0
 
 
-_LOGPROB = [(dict(dtype=2), DTYPE), (dict(M=-1), SHAPE), (dict(N=0), SHAPE), (dict(N=(1 << 22) + 1, stride=1 << 23), SHAPE),
+_LOGPROB = [(dict(dtype=2), DTYPE), (dict(M=-1), SHAPE), (dict(N=0), SHAPE), (dict(N=(1 << 21) + 1, stride=1 << 23), SHAPE),
             (dict(M=1 << 30, N=1 << 20, stride=1 << 20), SHAPE), (dict(stride=99), ARG), (dict(stride=1 << 41), ARG), (dict(stride=-100), ARG),
             (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=NAN), ARG), (dict(scale=INF), ARG), (dict(logits=None), NULL),
             (dict(tokens=None), NULL), (dict(logits=P + 1), ALIGN), (dict(tokens=P + 2), ALIGN), (dict(lse=P + 2), ALIGN),
@@ -117,7 +117,7 @@ def test_logprobs_workspace_size():
     assert f(4096, 128256, 0) == 0 and f(4096, 128256, 20) == 0
     assert f(1, 128256, 20) > 0 and f(8, 128256, 0) > 0 and f(4096, 400000, 64) > 0
     assert f(8, 1000, 5) == 0
-    for bad in ((0, 100, 1), (1, 0, 1), (1, (1 << 22) + 1, 1), (1, 100000, 65), (1, 100000, -1), (-1, 100000, 1)):
+    for bad in ((0, 100, 1), (1, 0, 1), (1, (1 << 21) + 1, 1), (1, 100000, 65), (1, 100000, -1), (-1, 100000, 1)):
         assert f(*bad) == 0
 
 
