@@ -12,7 +12,7 @@
 //
 // A row is read once, held in registers, and written once.  The mean is summed in
 // 64 bits and the squares are those of the distances from it, also in 64 bits: no
-// row that fp32 holds overflows or cancels in them.
+// row overflows or cancels in them.
 //
 // Backward: a group of threads goes over many rows with its columns' two sums in
 // registers, so dy and h are read once for the row's gradient and the columns'; a
@@ -71,33 +71,41 @@ __device__ __forceinline__ f32x8_t load_vector(const float* v, int j, int n, flo
     return r;
 }
 
-template <typename XT>
-__device__ __forceinline__ f32x8_t read_h(const ForwardArgs& a, const DropKey& key, int64_t row, int j, int n) {
-    const int64_t at = row * a.N + j;
-    f32x8_t h = load_piece(static_cast<const XT*>(a.x) + at, n);
-    if (a.drop.t) h = drop8(h, key, a.drop, (uint32_t)row, (uint32_t)j / 8);
-    if (a.r) {
-        const f32x8_t r = a.h_dtype == JH_F32 ? load_piece(static_cast<const float*>(a.r) + at, n)
-                                              : load_piece(static_cast<const uint16_t*>(a.r) + at, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h.v[i] += r.v[i];
+// x and r of a piece as they lie in memory, and h of them
+template <typename XT, typename RT, bool RES>
+struct RawH {
+    Raw8<XT> x;
+    Raw8<RT> r;
+    __device__ __forceinline__ void load(const ForwardArgs& a, int64_t row, int j, int n) {
+        x = load_raw(static_cast<const XT*>(a.x) + row * a.N + j, n);
+        if constexpr (RES) r = load_raw(static_cast<const RT*>(a.r) + row * a.N + j, n);
     }
-    return h;
-}
+    __device__ __forceinline__ f32x8_t h(const ForwardArgs& a, const DropKey& key, int64_t row, int j) const {
+        f32x8_t h = values(x);
+        if (a.drop.t) h = drop8(h, key, a.drop, (uint32_t)row, (uint32_t)j / 8);
+        if constexpr (RES) {
+            const f32x8_t v = values(r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h.v[i] += v.v[i];
+        }
+        return h;
+    }
+};
 __device__ __forceinline__ void store_any(void* p, int dtype, int64_t at, const f32x8_t& v, int n) {
     if (dtype == JH_F32)
         store_piece(static_cast<float*>(p) + at, v, n);
     else
         store_piece(static_cast<uint16_t*>(p) + at, v, n);
 }
-__device__ __forceinline__ void write_y(const ForwardArgs& a, int64_t row, int j, int n, const f32x8_t& h, float mean,
-                                        float rstd) {
+// h and y of a piece.  The weight and the bias are loaded before the piece's stores: a load
+// behind stores waits for them too, the counter of both being one.
+__device__ __forceinline__ void write_y(const ForwardArgs& a, int64_t row, int j, int n, const f32x8_t& h, float mean, float rstd) {
     const int64_t at = row * a.N + j;
-    if (a.h_out) store_any(a.h_out, a.h_dtype, at, h, n);
     const f32x8_t g = load_vector(a.gamma, j, n, 1.0f), b = load_vector(a.beta, j, n, 0.0f);
     f32x8_t y;
 #pragma unroll
     for (int i = 0; i < 8; ++i) y.v[i] = __builtin_fmaf((h.v[i] - mean) * rstd, g.v[i], b.v[i]);
+    if (a.h_out) store_any(a.h_out, a.h_dtype, at, h, n);
     store_any(a.out, a.out_dtype, at, y, n);
 }
 
@@ -107,21 +115,24 @@ __device__ __forceinline__ double sum8(const f32x8_t& h, int n) {
     for (int i = 0; i < 8; ++i) s += i < n ? (double)h.v[i] : 0.0;
     return s;
 }
-__device__ __forceinline__ double squares8(const f32x8_t& h, double mean, int n) {
+// of the distances from the mean in fp32, which are exact where that is far from zero
+__device__ __forceinline__ double squares8(const f32x8_t& h, float mean, int n) {
     double s = 0.0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const double d = i < n ? (double)h.v[i] - mean : 0.0;
+        const double d = i < n ? (double)(h.v[i] - mean) : 0.0;
         s = __builtin_fma(d, d, s);
     }
     return s;
 }
-__device__ __forceinline__ float row_rstd(double squares, int N, float eps) {
-    return (float)(1.0 / sqrt(squares / (double)N + (double)eps));
+// squares about `mean`, which is `center` rounded
+__device__ __forceinline__ float row_rstd(double squares, double center, float mean, int N, float eps) {
+    const double e = center - (double)mean, var = squares / (double)N - e * e;
+    return (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)eps));
 }
 
 // G threads a row, NP pieces of 8 neighbouring elements a thread
-template <typename XT, int G, int NP>
+template <typename XT, typename RT, bool RES, int G, int NP>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_kernel(ForwardArgs a) {
     constexpr int ROWS = G < 256 ? 256 / G : 1;
     const int tid = G < 256 ? threadIdx.x % G : threadIdx.x;
@@ -129,17 +140,20 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_kernel(Forwar
     int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + (G < 256 ? threadIdx.x / G : 0); row < a.M;
          row += (int64_t)gridDim.x * ROWS) {
+        RawH<XT, RT, RES> raw[NP];
         f32x8_t h[NP];
         double s[1] = {0.0};
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
             const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n > 0) h[t] = read_h<XT>(a, key, row, j, n);
+            if (n > 0) raw[t].load(a, row, j, n);
         }
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
-            const int n = min(8, a.N - 8 * (tid + G * t));
-            if (n > 0) s[0] += sum8(h[t], n);
+            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+            if (n <= 0) continue;
+            h[t] = raw[t].h(a, key, row, j);
+            s[0] += sum8(h[t], n);
         }
         reduce_group<G>(s, turn);
         const double center = s[0] / (double)a.N;
@@ -148,73 +162,89 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_kernel(Forwar
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
             const int n = min(8, a.N - 8 * (tid + G * t));
-            if (n > 0) s[0] += squares8(h[t], center, n);
+            if (n > 0) s[0] += squares8(h[t], mean, n);
         }
         reduce_group<G>(s, turn);
-        const float rstd = row_rstd(s[0], a.N, a.eps);
+        const float rstd = row_rstd(s[0], center, mean, a.N, a.eps);
         if (tid == 0) {
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
         }
+        float center32 = mean;  // the distances are formed again, rather than kept in registers
+        asm volatile("" : "+v"(center32));
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
             const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n > 0) write_y(a, row, j, n, h[t], mean, rstd);
+            if (n > 0) write_y(a, row, j, n, h[t], center32, rstd);
         }
     }
 }
 
 // rows longer than a block holds: read three times.  An element of x and r is last
 // read by the thread that then writes it, so the outputs may be the inputs here too.
-template <typename XT>
+template <typename XT, typename RT, bool RES>
 __global__ __launch_bounds__(1024) void add_layernorm_long_kernel(ForwardArgs a) {
     const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
     int turn = 0;
-    const auto pieces = [&](auto&& f) {
-        for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) f((int)j, (int)min((int64_t)8, a.N - j));
-    };
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const auto pieces = [&](auto&& f) {
+            for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) {
+                const int n = (int)min((int64_t)8, a.N - j);
+                RawH<XT, RT, RES> raw;
+                raw.load(a, row, (int)j, n);
+                f((int)j, n, raw.h(a, key, row, (int)j));
+            }
+        };
         double s[1] = {0.0};
-        pieces([&](int j, int n) { s[0] += sum8(read_h<XT>(a, key, row, j, n), n); });
+        pieces([&](int, int n, const f32x8_t& h) { s[0] += sum8(h, n); });
         reduce_group<1024>(s, turn);
         const double center = s[0] / (double)a.N;
         const float mean = (float)center;
         s[0] = 0.0;
-        pieces([&](int j, int n) { s[0] += squares8(read_h<XT>(a, key, row, j, n), center, n); });
+        pieces([&](int, int n, const f32x8_t& h) { s[0] += squares8(h, mean, n); });
         reduce_group<1024>(s, turn);
-        const float rstd = row_rstd(s[0], a.N, a.eps);
+        const float rstd = row_rstd(s[0], center, mean, a.N, a.eps);
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
         }
-        pieces([&](int j, int n) { write_y(a, row, j, n, read_h<XT>(a, key, row, j, n), mean, rstd); });
+        pieces([&](int j, int n, const f32x8_t& h) {
+            write_y(a, row, j, n, h, mean, rstd);
+        });
     }
 }
 
-template <typename XT, int G, int NP>
-void launch_forward(const ForwardArgs& a, int blocks, hipStream_t s) {
+template <typename XT, typename RT, bool RES, int G, int NP>
+void launch_forward(const ForwardArgs& a, hipStream_t s) {
     constexpr int ROWS = G < 256 ? 256 / G : 1;
     const int64_t rows = ((int64_t)a.M + ROWS - 1) / ROWS;
-    add_layernorm_kernel<XT, G, NP><<<(unsigned)std::min((int64_t)blocks, rows), G < 256 ? 256 : G, 0, s>>>(a);
+    add_layernorm_kernel<XT, RT, RES, G, NP><<<(unsigned)std::min((int64_t)1 << 20, rows), G < 256 ? 256 : G, 0, s>>>(a);
 }
 
-template <typename XT>
+template <typename XT, typename RT, bool RES>
 hipError_t launch_forward(const ForwardArgs& a, hipStream_t s) {
     if (a.N <= 128)
-        launch_forward<XT, 16, 1>(a, 8192, s);
+        launch_forward<XT, RT, RES, 16, 1>(a, s);
     else if (a.N <= 512)
-        launch_forward<XT, 64, 1>(a, 8192, s);
+        launch_forward<XT, RT, RES, 64, 1>(a, s);
+    else if (a.N <= 1024)
+        launch_forward<XT, RT, RES, 64, 2>(a, s);
     else if (a.N <= 2048)
-        launch_forward<XT, 256, 1>(a, 2048, s);
+        launch_forward<XT, RT, RES, 256, 1>(a, s);
     else if (a.N <= 4096)
-        launch_forward<XT, 256, 2>(a, 2048, s);
+        launch_forward<XT, RT, RES, 256, 2>(a, s);
     else if (a.N <= 8192)
-        launch_forward<XT, 256, 4>(a, 1024, s);
+        launch_forward<XT, RT, RES, 256, 4>(a, s);
     else if (a.N <= 16384)
-        launch_forward<XT, 512, 4>(a, 512, s);
+        launch_forward<XT, RT, RES, 1024, 2>(a, s);
     else
-        add_layernorm_long_kernel<XT><<<(unsigned)std::min(a.M, 2048), 1024, 0, s>>>(a);
+        add_layernorm_long_kernel<XT, RT, RES><<<(unsigned)std::min(a.M, 2048), 1024, 0, s>>>(a);
     return hipGetLastError();
+}
+template <typename XT>
+hipError_t launch_forward(const ForwardArgs& a, hipStream_t s) {
+    if (!a.r) return launch_forward<XT, XT, false>(a, s);
+    return a.h_dtype == JH_F32 ? launch_forward<XT, float, true>(a, s) : launch_forward<XT, uint16_t, true>(a, s);
 }
 
 // ---- backward -----------------------------------------------------------------
@@ -225,92 +255,114 @@ struct BackwardArgs {
     void *dx, *dr;   // either may be null: not wanted
     float* partial;  // [blocks][2][N]: sums of dy n and of dy over the block's rows; null: not wanted
     Dropout drop;
-    int M, N, x_dtype, h_dtype;  // dy and dx, h, dh and dr
+    int M, N;
 };
 
-__device__ __forceinline__ f32x8_t load_any(const void* p, int dtype, int64_t at, int n) {
-    return dtype == JH_F32 ? load_piece(static_cast<const float*>(p) + at, n)
-                           : load_piece(static_cast<const uint16_t*>(p) + at, n);
-}
-// dr and dx of a piece
-__device__ __forceinline__ void write_gradient(const BackwardArgs& a, const DropKey& key, int64_t row, int j, int n,
-                                               const f32x8_t& dy, const f32x8_t& norm, const f32x8_t& gamma, float rstd, float c1,
-                                               float c2) {
-    const int64_t at = row * a.N + j;
-    f32x8_t g;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) g.v[i] = rstd * (__builtin_fmaf(dy.v[i], gamma.v[i], -c1) - norm.v[i] * c2);
-    if (a.dh) {
-        const f32x8_t dh = load_any(a.dh, a.h_dtype, at, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g.v[i] += dh.v[i];
+// dy, h and dh of a piece as they lie in memory
+template <typename XT, typename HT>
+struct RawGrad {
+    Raw8<XT> dy;
+    Raw8<HT> h, dh;
+    __device__ __forceinline__ void load(const BackwardArgs& a, int64_t row, int j, int n, bool with_dh) {
+        const int64_t at = row * a.N + j;
+        dy = load_raw(static_cast<const XT*>(a.dy) + at, n);
+        h = load_raw(static_cast<const HT*>(a.h) + at, n);
+        if (with_dh && a.dh) dh = load_raw(static_cast<const HT*>(a.dh) + at, n);
     }
-    if (a.dr) store_any(a.dr, a.h_dtype, at, g, n);
-    if (a.dx) {
-        if (a.drop.t) g = drop8(g, key, a.drop, (uint32_t)row, (uint32_t)j / 8);
-        store_any(a.dx, a.x_dtype, at, g, n);
+    __device__ __forceinline__ f32x8_t norm(float mean, float rstd) const {
+        f32x8_t r = values(h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = (r.v[i] - mean) * rstd;
+        return r;
     }
-}
+    // dr and dx of the piece
+    __device__ __forceinline__ void write(const BackwardArgs& a, const DropKey& key, int64_t row, int j, int n, const f32x8_t& norm,
+                                          const f32x8_t& gamma, float rstd, float c1, float c2) const {
+        const int64_t at = row * a.N + j;
+        const f32x8_t y = values(dy);
+        f32x8_t g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g.v[i] = rstd * (__builtin_fmaf(y.v[i], gamma.v[i], -c1) - norm.v[i] * c2);
+        if (a.dh) {
+            const f32x8_t more = values(dh);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g.v[i] += more.v[i];
+        }
+        if (a.dr) store_piece(static_cast<HT*>(a.dr) + at, g, n);
+        if (a.dx) {
+            if (a.drop.t) g = drop8(g, key, a.drop, (uint32_t)row, (uint32_t)j / 8);
+            store_piece(static_cast<XT*>(a.dx) + at, g, n);
+        }
+    }
+};
 
-template <int G, int NP>
+template <typename XT, typename HT, int G, int NP>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(BackwardArgs a) {
     constexpr int ROWS = G < 256 ? 256 / G : 1;
     const int tid = G < 256 ? threadIdx.x % G : threadIdx.x, group = G < 256 ? threadIdx.x / G : 0;
     const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
     int turn = 0;
-    f32x8_t gamma[NP], sum_n[NP], sum_y[NP];
+    constexpr bool KEEP = NP == 1;  // more pieces: no registers to spare for the weight
+    f32x8_t gamma[KEEP ? NP : 1], sum_n[NP], sum_y[NP];
+    const auto weight = [&](int t) {
+        const int j = 8 * (tid + G * t), n = min(8, a.N - j);
+        return n > 0 ? load_vector(a.gamma, j, n, 1.0f) : f32x8_t{};
+    };
 #pragma unroll
     for (int t = 0; t < NP; ++t) {
-        const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-        if (n > 0) gamma[t] = load_vector(a.gamma, j, n, 1.0f);
+        if constexpr (KEEP) gamma[t] = weight(t);
         sum_n[t] = sum_y[t] = f32x8_t{};
     }
     for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.M; row += (int64_t)gridDim.x * ROWS) {
-        f32x8_t dy[NP], norm[NP];
+        RawGrad<XT, HT> raw[NP];
         const float mean = a.mean[row], rstd = a.rstd[row];
         float c[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
             const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n <= 0) continue;
-            dy[t] = load_any(a.dy, a.x_dtype, row * a.N + j, n);
-            norm[t] = load_any(a.h, a.h_dtype, row * a.N + j, n);
+            if (n > 0) raw[t].load(a, row, j, n, true);
         }
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
-            const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n <= 0) continue;
+            if (8 * (tid + G * t) >= a.N) continue;
+            const f32x8_t dy = values(raw[t].dy), norm = raw[t].norm(mean, rstd), w = KEEP ? gamma[KEEP ? t : 0] : weight(t);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                norm[t].v[i] = (norm[t].v[i] - mean) * rstd;
-                const float g = dy[t].v[i] * gamma[t].v[i];  // 0 behind the row's end
+                const float g = dy.v[i] * w.v[i];  // 0 behind the row's end
                 c[0] += g;
-                c[1] = __builtin_fmaf(g, norm[t].v[i], c[1]);
-                sum_n[t].v[i] = __builtin_fmaf(dy[t].v[i], norm[t].v[i], sum_n[t].v[i]);
-                sum_y[t].v[i] += dy[t].v[i];
+                c[1] = __builtin_fmaf(g, norm.v[i], c[1]);
+                sum_n[t].v[i] = __builtin_fmaf(dy.v[i], norm.v[i], sum_n[t].v[i]);
+                sum_y[t].v[i] += dy.v[i];
             }
         }
         reduce_group<G>(c, turn);
         const float c1 = c[0] / (float)a.N, c2 = c[1] / (float)a.N;
+        f32x8_t w = KEEP ? gamma[0] : weight(0);  // before the stores of the piece before, see write_y
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
             const int j = 8 * (tid + G * t), n = min(8, a.N - j);
-            if (n > 0) write_gradient(a, key, row, j, n, dy[t], norm[t], gamma[t], rstd, c1, c2);
+            if (n <= 0) continue;
+            const f32x8_t now = w;
+            if (t + 1 < NP) w = KEEP ? gamma[KEEP ? t + 1 : 0] : weight(t + 1);
+            raw[t].write(a, key, row, j, n, raw[t].norm(mean, rstd), now, rstd, c1, c2);
         }
     }
     if (!a.partial) return;
     float* out = a.partial + (int64_t)blockIdx.x * 2 * a.N;
     if constexpr (ROWS > 1) {
         // the block's groups, in order
-        __shared__ float sums[ROWS][2][8 * G];
+        constexpr int W = 8 * G * NP;
+        __shared__ float sums[ROWS][2][W];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            sums[group][0][8 * tid + i] = sum_n[0].v[i];
-            sums[group][1][8 * tid + i] = sum_y[0].v[i];
-        }
+        for (int t = 0; t < NP; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sums[group][0][8 * (tid + G * t) + i] = sum_n[t].v[i];
+                sums[group][1][8 * (tid + G * t) + i] = sum_y[t].v[i];
+            }
         __syncthreads();
-        for (int k = threadIdx.x; k < 16 * G; k += 256) {
-            const int which = k / (8 * G), j = k % (8 * G);
+        for (int k = threadIdx.x; k < 2 * W; k += 256) {
+            const int which = k / W, j = k % W;
             if (j >= a.N) continue;
             float s = 0.0f;
             for (int g = 0; g < ROWS; ++g) s += sums[g][which][j];
@@ -328,23 +380,23 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(Ba
 }
 
 // rows longer than a block holds: dy, h are read twice, and once more for the columns
+template <typename XT, typename HT>
 __global__ __launch_bounds__(1024) void add_layernorm_bwd_long_kernel(BackwardArgs a) {
     const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const float mean = a.mean[row], rstd = a.rstd[row];
-        const auto pieces = [&](auto&& f) {
+        const auto pieces = [&](bool with_dh, auto&& f) {
             for (int64_t j = 8 * (int64_t)threadIdx.x; j < a.N; j += 8 * 1024) {
                 const int n = (int)min((int64_t)8, a.N - j);
-                const f32x8_t dy = load_any(a.dy, a.x_dtype, row * a.N + j, n);
-                f32x8_t norm = load_any(a.h, a.h_dtype, row * a.N + j, n);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) norm.v[i] = (norm.v[i] - mean) * rstd;
-                f((int)j, n, dy, norm, load_vector(a.gamma, (int)j, n, 1.0f));
+                RawGrad<XT, HT> raw;
+                raw.load(a, row, (int)j, n, with_dh);
+                f((int)j, n, raw, raw.norm(mean, rstd), load_vector(a.gamma, (int)j, n, 1.0f));
             }
         };
         float c[2] = {0.0f, 0.0f};
-        pieces([&](int, int, const f32x8_t& dy, const f32x8_t& norm, const f32x8_t& gamma) {
+        pieces(false, [&](int, int, const RawGrad<XT, HT>& raw, const f32x8_t& norm, const f32x8_t& gamma) {
+            const f32x8_t dy = values(raw.dy);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float g = dy.v[i] * gamma.v[i];
@@ -354,22 +406,24 @@ __global__ __launch_bounds__(1024) void add_layernorm_bwd_long_kernel(BackwardAr
         });
         reduce_group<1024>(c, turn);
         const float c1 = c[0] / (float)a.N, c2 = c[1] / (float)a.N;
-        pieces([&](int j, int n, const f32x8_t& dy, const f32x8_t& norm, const f32x8_t& gamma) {
-            write_gradient(a, key, row, j, n, dy, norm, gamma, rstd, c1, c2);
+        pieces(true, [&](int j, int n, const RawGrad<XT, HT>& raw, const f32x8_t& norm, const f32x8_t& gamma) {
+            raw.write(a, key, row, j, n, norm, gamma, rstd, c1, c2);
         });
     }
 }
 // the columns' sums of rows blockIdx.y, blockIdx.y + gridDim.y, .. of long rows
+template <typename XT, typename HT>
 __global__ __launch_bounds__(256) void layernorm_columns_kernel(BackwardArgs a) {
     for (int64_t j = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x); j < a.N; j += 8 * 256 * (int64_t)gridDim.x) {
         const int n = (int)min((int64_t)8, a.N - j);
         f32x8_t sum_n{}, sum_y{};
         for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
-            const f32x8_t dy = load_any(a.dy, a.x_dtype, row * a.N + j, n), h = load_any(a.h, a.h_dtype, row * a.N + j, n);
-            const float mean = a.mean[row], rstd = a.rstd[row];
+            RawGrad<XT, HT> raw;
+            raw.load(a, row, (int)j, n, false);
+            const f32x8_t dy = values(raw.dy), norm = raw.norm(a.mean[row], a.rstd[row]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sum_n.v[i] = __builtin_fmaf(dy.v[i], (h.v[i] - mean) * rstd, sum_n.v[i]);
+                sum_n.v[i] = __builtin_fmaf(dy.v[i], norm.v[i], sum_n.v[i]);
                 sum_y.v[i] += dy.v[i];
             }
         }
@@ -379,20 +433,25 @@ __global__ __launch_bounds__(256) void layernorm_columns_kernel(BackwardArgs a) 
     }
 }
 
-// dgamma, dbeta = the partial rows' sums: 32 columns a block, 8 threads a column
-__global__ __launch_bounds__(256) void layernorm_fold_kernel(const float* partial, int parts, float* dgamma, float* dbeta,
-                                                             int N) {
-    __shared__ float sums[8][32];
-    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-    for (int64_t j0 = 32 * (int64_t)blockIdx.x; j0 < 2 * (int64_t)N; j0 += 32 * (int64_t)gridDim.x) {
+// dgamma, dbeta = the partial rows' sums: a wave adds every 16th row of 64 columns,
+// 8 loads under way together
+__global__ __launch_bounds__(1024) void layernorm_fold_kernel(const float* partial, int parts, float* dgamma, float* dbeta,
+                                                              int N) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int64_t width = 2 * (int64_t)N;
+    for (int64_t j0 = 64 * (int64_t)blockIdx.x; j0 < width; j0 += 64 * (int64_t)gridDim.x) {
         const int64_t j = j0 + lane;
         float s = 0.0f;
-        if (j < 2 * (int64_t)N)
-            for (int p = group; p < parts; p += 8) s += partial[p * 2 * (int64_t)N + j];
-        sums[group][lane] = s;
+        if (j < width) {
+#pragma unroll 8
+            for (int p = wave; p < parts; p += 16) s += partial[p * width + j];
+        }
+        sums[wave][lane] = s;
         __syncthreads();
-        if (group == 0 && j < 2 * (int64_t)N) {
-            for (int g = 1; g < 8; ++g) s += sums[g][lane];
+        if (wave == 0 && j < width) {
+#pragma unroll
+            for (int w = 1; w < 16; ++w) s += sums[w][lane];
             float* out = j < N ? dgamma : dbeta;
             if (out) out[j < N ? j : j - N] = s;
         }
@@ -402,16 +461,43 @@ __global__ __launch_bounds__(256) void layernorm_fold_kernel(const float* partia
 
 // how many blocks, and with them partial rows, the backward pass has
 int backward_blocks(int M, int N) {
-    if (N <= 512) {
+    if (N <= 1024) {
         const int rows = N <= 128 ? 16 : 4;
         return std::min(M / rows + (M % rows != 0), 1024);
     }
-    return std::min(M, N <= 2048 ? 1024 : N <= 16384 ? 512 : 64);
+    return std::min(M, N <= 2048 ? 1024 : N <= 4096 ? 512 : N <= 16384 ? 256 : 64);
 }
 
-template <int G, int NP>
+template <typename XT, typename HT, int G, int NP>
 void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
-    add_layernorm_bwd_kernel<G, NP><<<(unsigned)blocks, G < 256 ? 256 : G, 0, s>>>(a);
+    add_layernorm_bwd_kernel<XT, HT, G, NP><<<(unsigned)blocks, G < 256 ? 256 : G, 0, s>>>(a);
+}
+template <typename XT, typename HT>
+void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
+    if (a.N <= 128) {
+        launch_backward<XT, HT, 16, 1>(a, blocks, s);
+    } else if (a.N <= 512) {
+        launch_backward<XT, HT, 64, 1>(a, blocks, s);
+    } else if (a.N <= 1024) {
+        launch_backward<XT, HT, 64, 2>(a, blocks, s);
+    } else if (a.N <= 2048) {
+        launch_backward<XT, HT, 256, 1>(a, blocks, s);
+    } else if (a.N <= 4096) {
+        launch_backward<XT, HT, 512, 1>(a, blocks, s);
+    } else if (a.N <= 8192) {
+        launch_backward<XT, HT, 1024, 1>(a, blocks, s);
+    } else if (a.N <= 16384) {
+        // 1024 threads have the registers for 2 pieces in bf16 alone
+        if constexpr (sizeof(XT) + sizeof(HT) == 4)
+            launch_backward<XT, HT, 1024, 2>(a, blocks, s);
+        else
+            launch_backward<XT, HT, 512, 4>(a, blocks, s);
+    } else {
+        // the columns first: dx and dr may be dy and dh
+        if (a.partial)
+            layernorm_columns_kernel<XT, HT><<<dim3((unsigned)std::min((a.N + 2047) / 2048, 65535), blocks), 256, 0, s>>>(a);
+        if (a.dx || a.dr) add_layernorm_bwd_long_kernel<XT, HT><<<(unsigned)std::min(a.M, 2048), 1024, 0, s>>>(a);
+    }
 }
 
 }  // namespace
@@ -429,31 +515,17 @@ hipError_t launch_add_layernorm_bwd(int x_dtype, int h_dtype, const Dropout& dro
                                     const float* mean, const float* rstd, const float* gamma, void* dx, void* dr, float* dgamma,
                                     float* dbeta, int M, int N, void* ws, hipStream_t s) {
     const bool columns = dgamma || dbeta;
-    const BackwardArgs a{dy, h, dh, mean, rstd, gamma, dx, dr, columns ? static_cast<float*>(ws) : nullptr, drop, M, N, x_dtype,
-                         h_dtype};
+    const BackwardArgs a{dy, h, dh, mean, rstd, gamma, dx, dr, columns ? static_cast<float*>(ws) : nullptr, drop, M, N};
     const int blocks = backward_blocks(M, N);
-    if (M == 0) {
-        // no rows: the columns' sums are 0
-    } else if (N <= 128) {
-        launch_backward<16, 1>(a, blocks, s);
-    } else if (N <= 512) {
-        launch_backward<64, 1>(a, blocks, s);
-    } else if (N <= 2048) {
-        launch_backward<256, 1>(a, blocks, s);
-    } else if (N <= 4096) {
-        launch_backward<256, 2>(a, blocks, s);
-    } else if (N <= 8192) {
-        launch_backward<512, 2>(a, blocks, s);
-    } else if (N <= 16384) {
-        launch_backward<512, 4>(a, blocks, s);
-    } else {
-        // the columns first: dx and dr may be dy and dh
-        if (columns) layernorm_columns_kernel<<<dim3((unsigned)std::min((N + 2047) / 2048, 65535), blocks), 256, 0, s>>>(a);
-        if (dx || dr) add_layernorm_bwd_long_kernel<<<(unsigned)std::min(M, 2048), 1024, 0, s>>>(a);
+    if (M > 0) {  // no rows: the columns' sums are 0
+        if (x_dtype == JH_F32)
+            h_dtype == JH_F32 ? launch_backward<float, float>(a, blocks, s) : launch_backward<float, uint16_t>(a, blocks, s);
+        else
+            h_dtype == JH_F32 ? launch_backward<uint16_t, float>(a, blocks, s) : launch_backward<uint16_t, uint16_t>(a, blocks, s);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !columns) return e;
-    layernorm_fold_kernel<<<(unsigned)std::min((2 * (int64_t)N + 31) / 32, (int64_t)2048), 256, 0, s>>>(a.partial, blocks, dgamma,
+    layernorm_fold_kernel<<<(unsigned)std::min((2 * (int64_t)N + 63) / 64, (int64_t)2048), 1024, 0, s>>>(a.partial, blocks, dgamma,
                                                                                                   dbeta, N);
     return hipGetLastError();
 }
