@@ -567,9 +567,9 @@ int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t
             return fail(JH_ERR_ALIGN, "add_layernorm_bwd: pointers must be aligned to their elements");
         if (dgamma || dbeta) {
             const size_t need = jh::add_layernorm_bwd_workspace_size(M, N);
-            if (!workspace || workspace_bytes < need)
+            if (need && (!workspace || workspace_bytes < need))
                 return fail(JH_ERR_WORKSPACE, "add_layernorm_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-            if (!aligned(workspace, 4)) return fail(JH_ERR_ALIGN, "add_layernorm_bwd: workspace must be 4-byte aligned");
+            if (need && !aligned(workspace, 4)) return fail(JH_ERR_ALIGN, "add_layernorm_bwd: workspace must be 4-byte aligned");
         }
     }
     return check_hip(jh::launch_add_layernorm_bwd(x_dtype, h_dtype, d, dy, h, dh, mean, rstd, gamma, dx, dresidual, dgamma, dbeta,

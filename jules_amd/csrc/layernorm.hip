@@ -296,8 +296,9 @@ struct RawGrad {
     }
 };
 
-template <typename XT, typename HT, int G, int NP>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(BackwardArgs a) {
+// SUMS: the columns' sums of the block's rows go to a.partial
+template <typename XT, typename HT, int G, int NP, bool SUMS>
+__device__ __forceinline__ void backward_rows(const BackwardArgs& a, int block, int blocks) {
     constexpr int ROWS = G < 256 ? 256 / G : 1;
     const int tid = G < 256 ? threadIdx.x % G : threadIdx.x, group = G < 256 ? threadIdx.x / G : 0;
     const DropKey key = a.drop.t ? drop_key(a.drop) : DropKey{};
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(Ba
         if constexpr (KEEP) gamma[t] = weight(t);
         sum_n[t] = sum_y[t] = f32x8_t{};
     }
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.M; row += (int64_t)gridDim.x * ROWS) {
+    for (int64_t row = (int64_t)block * ROWS + group; row < a.M; row += (int64_t)blocks * ROWS) {
         RawGrad<XT, HT> raw[NP];
         const float mean = a.mean[row], rstd = a.rstd[row];
         float c[2] = {0.0f, 0.0f};
@@ -331,8 +332,10 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(Ba
                 const float g = dy.v[i] * w.v[i];  // 0 behind the row's end
                 c[0] += g;
                 c[1] = __builtin_fmaf(g, norm.v[i], c[1]);
-                sum_n[t].v[i] = __builtin_fmaf(dy.v[i], norm.v[i], sum_n[t].v[i]);
-                sum_y[t].v[i] += dy.v[i];
+                if constexpr (SUMS) {
+                    sum_n[t].v[i] = __builtin_fmaf(dy.v[i], norm.v[i], sum_n[t].v[i]);
+                    sum_y[t].v[i] += dy.v[i];
+                }
             }
         }
         reduce_group<G>(c, turn);
@@ -347,8 +350,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(Ba
             raw[t].write(a, key, row, j, n, raw[t].norm(mean, rstd), now, rstd, c1, c2);
         }
     }
-    if (!a.partial) return;
-    float* out = a.partial + (int64_t)blockIdx.x * 2 * a.N;
+    if (!SUMS || !a.partial) return;
+    float* out = a.partial + (int64_t)block * 2 * a.N;
     if constexpr (ROWS > 1) {
         // the block's groups, in order
         constexpr int W = 8 * G * NP;
@@ -377,6 +380,63 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(Ba
             store_piece(out + a.N + j, sum_y[t], n);
         }
     }
+}
+
+template <typename XT, typename HT, int G, int NP>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_kernel(BackwardArgs a) {
+    backward_rows<XT, HT, G, NP, true>(a, blockIdx.x, gridDim.x);
+}
+
+// Few rows: blocks from a.first on; the first row_blocks take a row each (256 / G rows),
+// the others all rows of 64 columns, whose sums they leave in dgamma and dbeta: dy and h are read twice,
+// out of the caches, and there is one launch and no workspace.
+template <typename XT, typename HT, int G, int NP>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void add_layernorm_bwd_few_kernel(BackwardArgs a, int first, int row_blocks,
+                                                                                 float* dgamma, float* dbeta) {
+    constexpr int WAVES = G < 256 ? 4 : G / 64;
+    const int block = first + blockIdx.x;
+    if (block < row_blocks) {
+        backward_rows<XT, HT, G, NP, false>(a, block, row_blocks);
+        return;
+    }
+    // 8 pieces a wave, 8 rows: lane = 8 row + piece
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int j0 = 64 * (block - row_blocks), j = j0 + 8 * (lane & 7), n = min(8, a.N - j);
+    f32x8_t sum_n{}, sum_y{};
+    if (n > 0) {
+#pragma unroll 2
+        for (int row = 8 * wave + (lane >> 3); row < a.M; row += 8 * WAVES) {
+            RawGrad<XT, HT> raw;
+            raw.load(a, row, j, n, false);
+            const f32x8_t dy = values(raw.dy), norm = raw.norm(a.mean[row], a.rstd[row]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum_n.v[i] = __builtin_fmaf(dy.v[i], norm.v[i], sum_n.v[i]);
+                sum_y.v[i] += dy.v[i];
+            }
+        }
+    }
+    __shared__ float sums[WAVES][2][64];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) {
+            sum_n.v[i] += __shfl_xor(sum_n.v[i], o);
+            sum_y.v[i] += __shfl_xor(sum_y.v[i], o);
+        }
+        if (lane < 8) {
+            sums[wave][0][8 * lane + i] = sum_n.v[i];
+            sums[wave][1][8 * lane + i] = sum_y.v[i];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= 128) return;
+    float* out = threadIdx.x < 64 ? dgamma : dbeta;
+    if (!out || j0 + lane >= a.N) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += sums[w][threadIdx.x >> 6][lane];
+    out[j0 + lane] = s;
 }
 
 // rows longer than a block holds: dy, h are read twice, and once more for the columns
@@ -500,6 +560,45 @@ void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
     }
 }
 
+// Where the columns' sums read dy and h again rather than leave partial sums: the second
+// launch and the workspace cost the caller 4.5 us (64 x 1024: 14.5 us against 18.9), reading
+// again costs more than that from some thousand rows on (512 x 8192 bf16: 15.9 us against 18.9,
+// fp32 26 against 24; 2000 x 1024: 25 against 18.7).
+bool backward_few(int M, int N) { return N <= 16384 && (M <= 512 || (M <= 2048 && M * N <= 1 << 20)); }
+
+template <typename XT, typename HT, int G, int NP>
+void launch_few(const BackwardArgs& a, float* dgamma, float* dbeta, hipStream_t s) {
+    constexpr int ROWS = G < 256 ? 256 / G : 1, BT = G < 256 ? 256 : G;
+    const int rows = a.dx || a.dr ? (a.M + ROWS - 1) / ROWS : 0;
+    const int columns = dgamma || dbeta ? (a.N + 63) / 64 : 0;
+    if (rows && columns && a.dx == a.dy) {  // the columns have to have read dy
+        add_layernorm_bwd_few_kernel<XT, HT, G, NP><<<columns, BT, 0, s>>>(a, rows, rows, dgamma, dbeta);
+        add_layernorm_bwd_few_kernel<XT, HT, G, NP><<<rows, BT, 0, s>>>(a, 0, rows, dgamma, dbeta);
+    } else if (rows + columns) {
+        add_layernorm_bwd_few_kernel<XT, HT, G, NP><<<rows + columns, BT, 0, s>>>(a, 0, rows, dgamma, dbeta);
+    }
+}
+template <typename XT, typename HT>
+void launch_few(const BackwardArgs& a, float* dgamma, float* dbeta, hipStream_t s) {
+    if (a.N <= 512)
+        launch_few<XT, HT, 64, 1>(a, dgamma, dbeta, s);
+    else if (a.N <= 2048)
+        launch_few<XT, HT, 256, 1>(a, dgamma, dbeta, s);
+    else if (a.N <= 8192)
+        launch_few<XT, HT, 1024, 1>(a, dgamma, dbeta, s);
+    else
+        launch_few<XT, HT, 1024, 2>(a, dgamma, dbeta, s);
+}
+
+// f<XT, HT>() by the types
+template <typename F>
+void by_types(int x_dtype, int h_dtype, F&& f) {
+    if (x_dtype == JH_F32)
+        h_dtype == JH_F32 ? f(0.0f, 0.0f) : f(0.0f, (uint16_t)0);
+    else
+        h_dtype == JH_F32 ? f((uint16_t)0, 0.0f) : f((uint16_t)0, (uint16_t)0);
+}
+
 }  // namespace
 
 hipError_t launch_add_layernorm(int x_dtype, int h_dtype, int out_dtype, const Dropout& drop, const void* x, const void* r,
@@ -509,20 +608,22 @@ hipError_t launch_add_layernorm(int x_dtype, int h_dtype, int out_dtype, const D
     return x_dtype == JH_F32 ? launch_forward<float>(a, s) : launch_forward<uint16_t>(a, s);
 }
 
-size_t add_layernorm_bwd_workspace_size(int M, int N) { return (size_t)backward_blocks(M, N) * 2 * (size_t)N * sizeof(float); }
+size_t add_layernorm_bwd_workspace_size(int M, int N) {
+    return backward_few(M, N) ? 0 : (size_t)backward_blocks(M, N) * 2 * (size_t)N * sizeof(float);
+}
 
 hipError_t launch_add_layernorm_bwd(int x_dtype, int h_dtype, const Dropout& drop, const void* dy, const void* h, const void* dh,
                                     const float* mean, const float* rstd, const float* gamma, void* dx, void* dr, float* dgamma,
                                     float* dbeta, int M, int N, void* ws, hipStream_t s) {
     const bool columns = dgamma || dbeta;
     const BackwardArgs a{dy, h, dh, mean, rstd, gamma, dx, dr, columns ? static_cast<float*>(ws) : nullptr, drop, M, N};
-    const int blocks = backward_blocks(M, N);
-    if (M > 0) {  // no rows: the columns' sums are 0
-        if (x_dtype == JH_F32)
-            h_dtype == JH_F32 ? launch_backward<float, float>(a, blocks, s) : launch_backward<float, uint16_t>(a, blocks, s);
-        else
-            h_dtype == JH_F32 ? launch_backward<uint16_t, float>(a, blocks, s) : launch_backward<uint16_t, uint16_t>(a, blocks, s);
+    if (M > 0 && backward_few(M, N)) {
+        by_types(x_dtype, h_dtype, [&](auto x, auto g) { launch_few<decltype(x), decltype(g)>(a, dgamma, dbeta, s); });
+        return hipGetLastError();
     }
+    const int blocks = backward_blocks(M, N);
+    if (M > 0)  // no rows: the columns' sums are 0
+        by_types(x_dtype, h_dtype, [&](auto x, auto g) { launch_backward<decltype(x), decltype(g)>(a, blocks, s); });
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !columns) return e;
     layernorm_fold_kernel<<<(unsigned)std::min((2 * (int64_t)N + 63) / 64, (int64_t)2048), 1024, 0, s>>>(a.partial, blocks, dgamma,

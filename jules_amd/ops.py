@@ -483,7 +483,7 @@ def add_layernorm(x, residual=None, gamma=None, beta=None, eps=1e-5, p=0.0, rng=
     if mean is None:
         mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     if rstd is None:
-        rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     _call(x, lib().jules_hip_add_layernorm, _DT[x.dtype], F32 if h is None else _DT[h.dtype], _DT[out.dtype], p, rng_ptr, offset,
           x.data_ptr(), _ptr(residual), _ptr(gamma), _ptr(beta), _ptr(h), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), M, N,
           float(eps))
@@ -536,10 +536,11 @@ def add_layernorm_bwd(dy, h, mean, rstd, gamma=None, dh=None, p=0.0, rng=None, o
         if dgamma is None:
             dgamma = dy.new_empty((N,), dtype=torch.float32)
         if dbeta is None:
-            dbeta = dy.new_empty((N,), dtype=torch.float32)
+            dbeta = torch.empty_like(dgamma)
         if workspace is None:
-            workspace = add_layernorm_bwd_workspace(M, N, dy.device)
-            ws_bytes = workspace.numel() * 4
+            ws_bytes = lib().jules_hip_add_layernorm_bwd_workspace_size(M, N)
+            if ws_bytes:
+                workspace = dy.new_empty((ws_bytes,), dtype=torch.uint8)
     _call(dy, lib().jules_hip_add_layernorm_bwd, _DT[dy.dtype], _DT[h.dtype], p, rng_ptr, offset, dy.data_ptr(), h.data_ptr(), _ptr(dh),
           mean.data_ptr(), rstd.data_ptr(), _ptr(gamma), _ptr(dx), dresidual.data_ptr(), _ptr(dgamma), _ptr(dbeta), M, N,
           _ptr(workspace), ws_bytes)
@@ -621,10 +622,10 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
     _one_device(("logits", "tokens", "workspace", *TokenLogprobs._fields), logits, tokens, workspace,
                 *((None,) * 5 if out is None else out))
     if out is None:
-        new = logits.new_empty
-        out = TokenLogprobs(None if tokens is None else new(lead, dtype=torch.float32), new(lead, dtype=torch.float32),
-                            new(lead, dtype=torch.float32), new((*lead, top), dtype=torch.int32) if top else None,
-                            new((*lead, top), dtype=torch.float32) if top else None)
+        lse = logits.new_empty(lead, dtype=torch.float32)
+        top_logp = logits.new_empty((*lead, top), dtype=torch.float32) if top else None
+        out = TokenLogprobs(None if tokens is None else torch.empty_like(lse), lse, torch.empty_like(lse),
+                            torch.empty_like(top_logp, dtype=torch.int32) if top else None, top_logp)
     if workspace is None:
         ws_bytes = lib().jules_hip_token_logprobs_workspace_size(M, N, top)
         if ws_bytes:

@@ -68,7 +68,7 @@ def test_add_layernorm_statuses(change, status):
 ])
 def test_add_layernorm_bwd_statuses(change, status):
     a = dict(x_dtype=F32, h_dtype=BF16, p=0.1, rng=P, offset=0, dy=P, h=P, dh=P, mean=P, rstd=P, gamma=P, dx=P, dr=P, dgamma=P, dbeta=P,
-             M=40, N=8, ws=P, ws_bytes=1 << 20)
+             M=4000, N=8, ws=P, ws_bytes=1 << 20)
     a.update(change)
     if "ws_bytes" in change:
         a["ws_bytes"] = _lib.lib().jules_hip_add_layernorm_bwd_workspace_size(a["M"], a["N"]) - 1
@@ -77,7 +77,9 @@ def test_add_layernorm_bwd_statuses(change, status):
 
 def test_layernorm_workspace_size():
     f = _lib.lib().jules_hip_add_layernorm_bwd_workspace_size
-    for M, N in ((1, 1), (7, 64), (64, 1024), (32768, 4096), (1 << 20, 128), (5000, 16384), (5000, 100000)):
+    for M, N in ((1, 1), (7, 64), (64, 1024), (512, 16384), (2048, 512)):  # few rows
+        assert f(M, N) == 0
+    for M, N in ((513, 2048), (2049, 1), (64, 16385), (32768, 4096), (1 << 20, 128), (5000, 16384), (5000, 100000)):
         assert 8 * N <= f(M, N) <= 8 * 1024 * N
     assert f(0, 8) == 0 and f(8, 0) == 0 and f(-1, 8) == 0 and f(1 << 21, 1 << 21) == 0
 
