@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(Dropout d, const XT* x, co
 template <typename XT, typename OT>
 hipError_t launch(const Dropout& d, const void* x, const void* r, void* out, int M, int N, hipStream_t s) {
     const int64_t blocks = ((int64_t)M * (N / 8 + (N % 8 != 0)) + 255) / 256;
-    const unsigned grid = (unsigned)std::min(blocks, (int64_t)2048);
+    const unsigned grid = (unsigned)std::min(blocks, (int64_t)1 << 20);
     if (r)
         dropout_kernel<XT, OT, true><<<grid, 256, 0, s>>>(d, static_cast<const XT*>(x), static_cast<const OT*>(r),
                                                           static_cast<OT*>(out), M, N);

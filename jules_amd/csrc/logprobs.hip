@@ -179,21 +179,23 @@ __device__ __forceinline__ int find_top(uint64_t* keys, const T* x, int first, i
     const int threads = found[0];
     if (tid < threads && rank_of(keys[tid], keys, threads) == top - 1) threshold = keys[tid];
     __syncthreads();
-    // those threads' elements that reach it, mostly of one piece each
+    // those threads' elements that reach it, mostly of one piece each; where a thread may have
+    // more, its wave reads all of its pieces together
     const uint64_t bound = threshold;
-    if (own && own >= bound) {
-        const auto take = [&](int piece) {
-            const int n = min(8, len - 8 * piece);
-            const f32x8_t v = values(load_raw(x + 8 * piece, n));
+    const auto take = [&](int piece) {
+        const int n = min(8, len - 8 * piece);
+        const f32x8_t v = values(load_raw(x + 8 * piece, n));
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n && key_of(v.v[i], (uint32_t)piece) >= bound)
-                    keys[atomicAdd(&found[1], 1)] = key_of(v.v[i], (uint32_t)(first + 8 * piece + i));
-        };
-        take(l.piece);
-        if (order_of(l.next) >= (uint32_t)(bound >> 32))
-            for (int piece = tid; 8 * piece < len; piece += BT)
-                if (piece != l.piece) take(piece);
+        for (int i = 0; i < 8; ++i)
+            if (i < n && key_of(v.v[i], (uint32_t)piece) >= bound)
+                keys[atomicAdd(&found[1], 1)] = key_of(v.v[i], (uint32_t)(first + 8 * piece + i));
+    };
+    const bool reaches = own && own >= bound;
+    const bool more = reaches && order_of(l.next) >= (uint32_t)(bound >> 32);
+    if (reaches && !more) take(l.piece);
+    for (uint64_t left = __ballot(more); left; left &= left - 1) {
+        const int thread = (tid & ~63) + __builtin_ctzll(left);
+        for (int piece = thread + BT * (tid & 63); 8 * piece < len; piece += BT * 64) take(piece);
     }
     __syncthreads();
     return found[1];
@@ -248,6 +250,11 @@ __global__ __launch_bounds__(BT, 8) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
             for (int t = 0; t < B; ++t) raw[t] = load_raw(x + 8 * (b + BT * t), 8);
             add_pieces<BT, TOP>(raw, b, a.c2, &mine, &l);
+        }
+        if (8 * (b + BT) + 8 <= len) {
+            const Raw8<T> raw[2] = {load_raw(x + 8 * b, 8), load_raw(x + 8 * (b + BT), 8)};
+            add_pieces<BT, TOP>(raw, b, a.c2, &mine, &l);
+            b += 2 * BT;
         }
 #pragma unroll 1
         for (; 8 * b < len; b += BT) {
@@ -345,6 +352,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
     }
 }
 
+// how rows are split, and the threads of a block
 struct Split {
     int parts, width, threads;
 };
@@ -352,10 +360,11 @@ Split split_of(int M, int N, int top) {
     // what the keys in LDS allow: `top` threads' elements
     const int most = top ? MAX_KEYS / (8 * top) * (8 * 512) : N;
     int parts = N / most + (N % most != 0);
-    if (M < 192) parts = std::max(parts, std::min((256 + M - 1) / M, N / 4096));
+    if (M < 1024 && N >= 65536) parts = std::max(parts, std::min(1024 / M, N / 8192));
     parts = std::min(std::max(parts, 1), MAX_PARTS);
     const int width = (N / parts + (N % parts != 0) + 7) / 8 * 8;
-    return Split{N / width + (N % width != 0), width, width <= 8192 ? 256 : 512};
+    const int threads = width <= 8192 && top <= 8 ? 64 : width <= 8192 ? 256 : M * parts > 256 || width <= 16384 ? 512 : 1024;
+    return Split{N / width + (N % width != 0), width, threads};
 }
 
 template <typename T, int BT>
@@ -371,10 +380,14 @@ void launch_parts(const LogprobArgs& a, hipStream_t s) {
 
 template <typename T>
 hipError_t launch(const LogprobArgs& a, int threads, hipStream_t s) {
-    if (threads == 256)
+    if (threads == 64)
+        launch_parts<T, 64>(a, s);
+    else if (threads == 256)
         launch_parts<T, 256>(a, s);
-    else
+    else if (threads == 512)
         launch_parts<T, 512>(a, s);
+    else
+        launch_parts<T, 1024>(a, s);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.parts == 1) return e;
     logprobs_join_kernel<T><<<(unsigned)std::min(a.M, 1 << 20), 256, sizeof(uint64_t) * a.parts * a.top, s>>>(a);
@@ -390,19 +403,27 @@ struct GradArgs {
     void* dlogits;
     int64_t stride, out_stride;
     float scale;
-    int M, N, chunks;
+    int M, N;
 };
 
-constexpr int GRAD_PIECES = 2;
-constexpr int GRAD_CHUNK = 256 * 8 * GRAD_PIECES;
-
+// BT threads for 32 bytes each of a row; a row's blocks side by side (rows side by side: 177 us
+// for 4096 x 50257 bf16 instead of 148)
 template <typename T>
-__global__ __launch_bounds__(256) void logprobs_bwd_kernel(GradArgs a) {
-    for (int64_t item = blockIdx.x; item < (int64_t)a.M * a.chunks; item += gridDim.x) {
-        const int64_t row = item / a.chunks;
-        const int first = (int)(item % a.chunks) * GRAD_CHUNK;
+constexpr int kGradPieces = 4 / (int)sizeof(T);
+
+template <typename T, int BT>
+__global__ __launch_bounds__(BT) void logprobs_bwd_kernel(GradArgs a) {
+    constexpr int PIECES = kGradPieces<T>;
+    const int first = 8 * ((int)blockIdx.x * BT * PIECES + (int)threadIdx.x);
+    for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
         const T* x = static_cast<const T*>(a.logits) + row * a.stride;
         T* out = static_cast<T*>(a.dlogits) + row * a.out_stride;
+        Raw8<T> raw[PIECES];
+#pragma unroll
+        for (int t = 0; t < PIECES; ++t) {
+            const int j = first + 8 * BT * t, n = min(8, a.N - j);
+            if (n > 0) raw[t] = load_raw(x + j, n);
+        }
         const int token = a.tokens[row];
         const float lse = a.lse[row], entropy = a.entropy ? a.entropy[row] : 0.0f;
         // a row of nothing but -infinity has no gradient, whatever reaches it
@@ -410,15 +431,9 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(GradArgs a) {
         float g = token < 0 || none ? 0.0f : a.dlogp[row] * a.scale;
         const float gh = !a.dentropy || none ? 0.0f : a.dentropy[row] * a.scale;
         if (token >= a.N) g = __builtin_nanf("");
-        Raw8<T> raw[GRAD_PIECES];
 #pragma unroll
-        for (int t = 0; t < GRAD_PIECES; ++t) {
-            const int j = first + 8 * ((int)threadIdx.x + 256 * t), n = min(8, a.N - j);
-            if (n > 0) raw[t] = load_raw(x + j, n);
-        }
-#pragma unroll
-        for (int t = 0; t < GRAD_PIECES; ++t) {
-            const int j = first + 8 * ((int)threadIdx.x + 256 * t), n = min(8, a.N - j);
+        for (int t = 0; t < PIECES; ++t) {
+            const int j = first + 8 * BT * t, n = min(8, a.N - j);
             if (n <= 0) continue;
             const f32x8_t v = values(raw[t]);
             f32x8_t y;
@@ -432,6 +447,18 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(GradArgs a) {
             store_piece(out + j, y, n);
         }
     }
+}
+
+template <typename T, int BT>
+hipError_t launch_grad(const GradArgs& a, hipStream_t s) {
+    constexpr int W = 8 * BT * kGradPieces<T>;
+    logprobs_bwd_kernel<T, BT><<<dim3((unsigned)((a.N + W - 1) / W), (unsigned)std::min(a.M, 65535)), BT, 0, s>>>(a);
+    return hipGetLastError();
+}
+// rows of one wave's width in waves of their own: 65536 x 1000 bf16 keep half of 256 threads idle
+template <typename T>
+hipError_t launch_grad(const GradArgs& a, hipStream_t s) {
+    return a.N <= 4096 ? launch_grad<T, 64>(a, s) : launch_grad<T, 256>(a, s);
 }
 
 }  // namespace
@@ -457,14 +484,8 @@ hipError_t launch_token_logprobs(int dtype, const void* logits, int64_t stride, 
 hipError_t launch_token_logprobs_bwd(int dtype, const void* logits, int64_t stride, float scale, const int32_t* tokens,
                                      const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
                                      void* dlogits, int64_t out_stride, int M, int N, hipStream_t s) {
-    const GradArgs a{logits, tokens, lse, entropy, dlogp, dentropy, dlogits, stride, out_stride, scale, M, N,
-                     N / GRAD_CHUNK + (N % GRAD_CHUNK != 0)};
-    const unsigned grid = (unsigned)std::min((int64_t)M * a.chunks, (int64_t)1 << 20);
-    if (dtype == JH_F32)
-        logprobs_bwd_kernel<float><<<grid, 256, 0, s>>>(a);
-    else
-        logprobs_bwd_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
-    return hipGetLastError();
+    const GradArgs a{logits, tokens, lse, entropy, dlogp, dentropy, dlogits, stride, out_stride, scale, M, N};
+    return dtype == JH_F32 ? launch_grad<float>(a, s) : launch_grad<uint16_t>(a, s);
 }
 
 }  // namespace jh

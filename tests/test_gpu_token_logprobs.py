@@ -32,6 +32,10 @@ def _tokens(dev, M, N, seed=0):
     return torch.randint(0, N, (M,), generator=torch.Generator().manual_seed(seed), dtype=i32).to(dev)
 
 
+def _normal(dev, M, seed=0):
+    return torch.randn(M, generator=torch.Generator().manual_seed(seed + 500)).to(dev)
+
+
 @np.errstate(invalid="ignore")  # -infinity less itself, in places that are compared apart
 def _check(x, tokens, scale, out, top):
     want = logprobs64(x, tokens, scale)
@@ -132,7 +136,7 @@ def test_masked(dev, N, dtype):
         _check(x, tokens, 1.0, out, top)
     assert out.lse[4] == -INF and out.logp[4] == -INF and out.entropy[4] == 0 and (out.top_logp[4] == -INF).all()
     assert out.entropy[3] == 0 and out.top_logp[3, 0] == 0 and out.entropy[6] == 0 and out.logp[7] == -INF
-    g = torch.randn(M, device=dev)
+    g = _normal(dev, M)
     g[4] = float("nan")  # what a loss makes of -infinity
     dx = ops.token_logprobs_bwd(x, tokens, out.lse, g, out.entropy, -g)
     assert torch.equal(dx[4], torch.zeros_like(dx[4]))
@@ -187,7 +191,7 @@ def test_backward_widths(dev, N):
                                           (2, f32, False, 1.3, 5, 3)):
         case(f"token_logprobs_bwd {M}x{N} {t} entropy {more} scale {scale} pad {pad} shift {shift}")
         x, tokens = _logits(dev, M, N, t, N, shift, pad), _tokens(dev, M, N)
-        g, h = torch.randn(M, device=dev), torch.randn(M, device=dev) if more else None
+        g, h = _normal(dev, M, N), _normal(dev, M, N + 1) if more else None
         out = ops.token_logprobs(x, tokens, scale=scale)
         dx = ops.token_logprobs_bwd(x, tokens, out.lse, g, out.entropy, h, scale=scale)
         torch.cuda.synchronize()
@@ -201,7 +205,7 @@ def test_in_place_and_padding(dev, N, pad):
     x, tokens = _logits(dev, 20, N, bf16, 4, 0, pad), _tokens(dev, 20, N)
     whole = x._base.view(20, N + pad) if pad else x
     out = ops.token_logprobs(x, tokens)
-    g = torch.randn(20, device=dev)
+    g = _normal(dev, 20)
     want = ops.token_logprobs_bwd(x, tokens, out.lse, g)
     behind = whole[:, N:].clone()
     assert ops.token_logprobs_bwd(x, tokens, out.lse, g, out=x) is x
@@ -238,7 +242,7 @@ def test_leading_dimensions_and_out(dev):
     assert none.logp is None and torch.equal(none.top_ids, a.top_ids[:, :2]) and torch.equal(none.entropy, a.entropy)
     row = ops.token_logprobs(x[0], tokens[:1], top=4)
     assert row.logp.shape == () and torch.equal(row.top_ids, a.top_ids[0])
-    g = torch.randn(12, device=dev)
+    g = _normal(dev, 12)
     assert torch.equal(ops.token_logprobs_bwd(x3, tokens, a.lse, g).view(12, 600), ops.token_logprobs_bwd(x, tokens, a.lse, g))
 
 
@@ -256,7 +260,7 @@ def test_differences(dev):
     outputs' bounds over the step."""
     M, N, e = 12, 40, 2.0**-5
     x, tokens = _logits(dev, M, N, f32, 6, scale=1.5), _tokens(dev, M, N)
-    g, h = torch.randn(M, generator=torch.Generator().manual_seed(1)).to(dev), torch.randn(M, generator=torch.Generator().manual_seed(2)).to(dev)
+    g, h = _normal(dev, M, 1), _normal(dev, M, 2)
 
     def loss(x):
         o = ops.token_logprobs(x, tokens, scale=0.8)

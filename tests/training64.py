@@ -100,8 +100,9 @@ def logprobs64(x, tokens, scale):
     """Of rows of numbers and -infinity: dict of lse, entropy, log [M, N] and logp in 64 bits, with
     bounds.  Distances z from the row's maximum carry 4 roundings into the exponents (the
     difference, the product, the factor's two), e^z 2 more, and the distance between two
-    maxima the same; 110 joins of 3 roundings and chains of 64 additions at most."""
-    x = f64(x)
+    maxima the same; 110 joins of 3 roundings and chains of 64 additions at most.  The
+    entry point takes scale as fp32."""
+    x, scale = f64(x), float(np.float32(scale))
     with np.errstate(divide="ignore", invalid="ignore"):
         z = (x - np.where(np.isfinite(x), x, -np.inf).max(-1, keepdims=True)) * scale
         none = ~np.isfinite(x).any(-1)
@@ -133,7 +134,9 @@ def top64(x, top):
 
 
 def logprobs_bwd64(x, tokens, lse, entropy, dlogp, dentropy, scale):
-    """The gradient in 64 bits from the kernel's inputs, lse and entropy among them, and its bound."""
+    """The gradient in 64 bits from the kernel's inputs, lse, entropy and scale as fp32 among
+    them, and its bound."""
+    scale = float(np.float32(scale))
     x, lse, g = f64(x), f64(lse)[:, None], f64(dlogp)[:, None]
     with np.errstate(invalid="ignore"):
         log = np.where(np.isfinite(lse), x * scale - lse, -np.inf)
