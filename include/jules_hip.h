@@ -377,52 +377,57 @@ int jules_hip_add_rmsnorm(int x_dtype, int residual_dtype, int out_dtype, const 
                           void* out, float* scale, int M, int N, float epsilon, void* stream);
 
 /* ---- dropout ------------------------------------------------------------------
- * out = [residual +] (element kept ? x * 65536 / (65536 - t) : 0),  t = p * 65536
- * rounded to a whole number (ties to even), row by row of [M, N].  No counterpart in the reference.
+ * out = [residual +] (element kept ? x * 65536 / (65536 - t) : 0),  t = 65536 p
+ * rounded to a whole number (ties to even), row by row of [M, N].  No counterpart
+ * in the reference: between the products of a training step, beside
+ * jules_hip_flash_attn_bwd and jules_hip_add_layernorm_bwd.
  * Element (i, j) is kept where 16 random bits are at least t: half word j % 8 (the
  * low half of each word first) of the four words of Philox4x32 with 10 rounds at
  * the counter (j / 8, i, low and high word of rng[1] + offset) and the key (low and
  * high word of rng[0]).  No mask is stored: the same call on the gradient, without
- * residual, is the backward pass, and other types or strides change no bit.
+ * residual, is the backward pass, and other types change no bit of it.
  * rng: int64 [2] in device memory (seed, position), read by the kernel, so that a
  *   captured graph drops other elements where the position was changed between
- *   replays; offset keeps apart the calls of one step.  Not looked at where t = 0.
+ *   replays; offset keeps the calls of one step apart.  Not looked at where t = 0.
  * 0 <= p < 1, and t < 65536 (JH_ERR_ARG).  x_dtype, out_dtype: JH_F32 or JH_BF16,
- * each by itself; residual NULL or [M, N] of out_dtype.  Arithmetic in fp32; a dropped
- * NaN or infinity is 0.  out may be x where the types are the same, or residual;
- * other overlaps are not allowed.  Pointers aligned to their elements.
+ * each by itself; residual NULL or [M, N] of out_dtype.  Arithmetic in fp32; a
+ * dropped NaN or infinity is 0.  out may be x where the types are the same, or
+ * residual; other overlaps are not allowed.  Pointers aligned to their elements.
  */
 int jules_hip_dropout(int x_dtype, int out_dtype, float p, const int64_t* rng, uint64_t offset,
                       const void* x, const void* residual, void* out, int M, int N, void* stream);
 
 /* ---- residual addition + dropout + layer norm, and its gradients -----------------
  * h = residual + dropout(x),  out = (h - mean) * rstd * gamma + beta,  row by row of
- * [M, N]: mean of h, rstd = 1 / sqrt(mean((h - mean)^2) + epsilon).  No counterpart in
- * the reference: jules_hip_layernorm with what a training step has around it.
+ * [M, N]: mean of h, rstd = 1 / sqrt(mean((h - mean)^2) + epsilon).  No counterpart
+ * in the reference: jules_hip_layernorm with what a training step has around it.
  * p, rng, offset: as in jules_hip_dropout; p = 0 for none.
  * x_dtype, h_dtype, out_dtype: JH_F32 or JH_BF16, each by itself; gamma, beta fp32
  * [N], NULL for ones and zeros.  residual: NULL, or [M, N] of h_dtype.  h: NULL, or
- * [M, N] of h_dtype that receives h rounded to it; it may be residual, and x where the types are
- * the same.  out may be x where the types are the same.  mean, rstd: NULL, or fp32 [M].
+ * [M, N] of h_dtype that receives h rounded to it; it may be residual, and x where
+ * the types are the same.  out may be x where the types are the same.  mean, rstd:
+ * NULL, or fp32 [M].
  * The norm is of h in fp32, before its rounding; the mean and the squares are summed
- * in 64 bits.  A NaN or an infinity in a row makes the row's out, mean and rstd NaN
- * (h is as ever).  epsilon >= 0; with 0 a row of equal elements is NaN.  Deterministic.  Pointers
- * aligned to their elements; overlaps other than those named are not allowed.
+ * in 64 bits.  A NaN or an infinity in a row makes the row's out, mean or rstd NaN
+ * (h is as ever).  epsilon >= 0; with 0 a row of equal elements is NaN.
+ * Deterministic.  Pointers aligned to their elements; overlaps other than those
+ * named are not allowed.
  *
- * jules_hip_add_layernorm_bwd: from dy [M, N] (x_dtype: out's gradient), h [M, N] (h_dtype),
- *   mean and rstd as the forward call left them, gamma, and dh (NULL, or [M, N] of
- *   h_dtype: what reaches h past the norm):
+ * jules_hip_add_layernorm_bwd: from dy [M, N] (x_dtype: the gradient of out), h
+ *   [M, N] (h_dtype), mean and rstd as the forward call left them, gamma, and dh
+ *   (NULL, or [M, N] of h_dtype: what reaches h past the norm):
  *   n = (h - mean) rstd,  a = dy gamma,
  *   dresidual = rstd (a - mean(a) - n mean(a n)) + dh   [M, N] of h_dtype
  *   dx        = dropout of dresidual before its rounding, with the forward call's p,
  *               rng and offset                          [M, N] of x_dtype
  *   dgamma, dbeta = sums over the rows of dy n, dy      fp32 [N]
- *   Any of the four may be NULL: not wanted.  dx may be dy, dresidual may be dh; other overlaps
- *   are not allowed.  M = 0 gives sums of 0.  fp32; deterministic (no atomics).
- *   workspace: jules_hip_add_layernorm_bwd_workspace_size(M, N) bytes (the blocks'
- *   sums: at most 8 * 1024 * N), 4-byte aligned, no initialisation, overwritten by every call;
- *   not looked at without dgamma and dbeta.  Calls that overlap in time need
- *   separate ones.
+ *   Any of the four may be NULL: not wanted.  dx may be dy, dresidual may be dh;
+ *   other overlaps are not allowed.  M = 0 gives sums of 0.  fp32; deterministic (no
+ *   atomics).
+ *   workspace: jules_hip_add_layernorm_bwd_workspace_size(M, N) bytes (sums of some
+ *   rows each: at most 8192 N, and 0 for few rows, where NULL will do), 4-byte
+ *   aligned, no initialisation, overwritten by every call; not looked at without
+ *   dgamma and dbeta.  Calls that overlap in time need separate ones.
  */
 int jules_hip_add_layernorm(int x_dtype, int h_dtype, int out_dtype, float p, const int64_t* rng,
                             uint64_t offset, const void* x, const void* residual,
@@ -437,26 +442,32 @@ int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t
 
 /* ---- log probabilities of tokens, and their gradient ------------------------------
  * z = scale * logits, row by row of [M, N] (rows row_stride elements apart, row_stride
- * >= N: an output layer padded to a round width needs no copy), logits JH_F32 or JH_BF16,
- * 1 <= N <= 2^21, scale between 1e-30 and 1e30.  No counterpart in the reference: jules_hip_cross_entropy gives one mean loss.
+ * >= N: an output layer padded to a round width needs no copy), logits JH_F32 or
+ * JH_BF16, 1 <= N <= 2^21, scale between 1e-30 and 1e30, the largest |z| of a row
+ * within fp32.  No counterpart in the reference: jules_hip_cross_entropy gives one mean loss.
  *   lse     = log(sum(exp(z)))               logp = z[token] - lse
  *   entropy = -sum(p log p), p = exp(z - lse)
  *   top_ids, top_logp [M, top]: the indices of the `top` largest logits, falling, equal
  *             ones by rising index, and their log probabilities
  * tokens int32 [M]: a negative one is none (logp 0, no gradient), one >= N gives NaN.
- * logp, lse, entropy: fp32 [M] or NULL; tokens may be NULL without logp.  0 <= top <= 64, top <= N.
- * -infinity (what a mask forbids) has probability 0.  A row of nothing else: lse and all
- * log probabilities -infinity, entropy 0, gradient 0.  A NaN or +infinity in a row: NaN everywhere, top_ids -1.
- * One pass over the logits, fp32 sums; deterministic.
+ * logp, lse, entropy: fp32 [M] or NULL; tokens may be NULL without logp.  0 <= top <=
+ * 64, top <= N.
+ * -infinity (what a mask forbids) has probability 0.  A row of nothing else: lse and
+ * all log probabilities -infinity, entropy 0, gradient 0 whatever reaches it.  A NaN or
+ * +infinity in a row: NaN everywhere, top_ids -1.  One pass over the logits, fp32 sums;
+ * deterministic.
  * workspace: jules_hip_token_logprobs_workspace_size(M, N, top) bytes (rows split over
- * workgroups: few rows, or N > 65536; 0: NULL will do), 8-byte aligned, no initialisation,
- * overwritten by every call; calls that overlap in time need separate ones.
+ * workgroups: M < 1024 at N >= 65536, and long rows with many alternatives; 0: NULL will
+ * do), 8-byte aligned, no initialisation, overwritten by every call; calls that overlap
+ * in time need separate ones.
  *
- * jules_hip_token_logprobs_bwd: dlogits [M, N] of the logits' dtype, rows dlogits_stride apart, is
+ * jules_hip_token_logprobs_bwd: dlogits [M, N] of the logits' dtype, rows dlogits_stride
+ *   apart, is
  *   scale * (dlogp (onehot(token) - p) - dentropy p (log p + entropy))
- *   from lse and entropy as the forward call with the same scale left them, dlogp fp32 [M]
- *   and dentropy fp32 [M] or NULL (entropy is not looked at then).  dlogits may be
- *   logits; other overlaps are not allowed.
+ *   from lse and entropy as the forward call with the same scale left them, dlogp fp32
+ *   [M] and dentropy fp32 [M] or NULL (entropy is not looked at then).  p has the error
+ *   of lse, 2^-24 of its magnitude.  dlogits may be logits; other overlaps are not
+ *   allowed.
  */
 size_t jules_hip_token_logprobs_workspace_size(int M, int N, int top);
 int jules_hip_token_logprobs(int dtype, const void* logits, int64_t row_stride, float scale,

@@ -513,6 +513,7 @@ int jules_hip_dropout(int x_dtype, int out_dtype, float p, const int64_t* rng, u
     if (!x || !out || (d.t && !rng)) return fail(JH_ERR_NULL, "dropout: null x, out or rng");
     if (!aligned(x, real_size(x_dtype)) || !aligned(out, real_size(out_dtype)) || !aligned(residual, real_size(out_dtype)))
         return fail(JH_ERR_ALIGN, "dropout: pointers must be aligned to their elements");
+    if (x == out && x_dtype != out_dtype) return fail(JH_ERR_ARG, "dropout: in place needs the same dtype");
     return check_hip(jh::launch_dropout(x_dtype, out_dtype, d, x, residual, out, M, N, static_cast<hipStream_t>(stream)),
                      "dropout launch");
 }
@@ -534,6 +535,8 @@ int jules_hip_add_layernorm(int x_dtype, int h_dtype, int out_dtype, float p, co
         !aligned(mean, 4) || !aligned(rstd, 4) ||
         ((residual || h) && (!aligned(residual, real_size(h_dtype)) || !aligned(h, real_size(h_dtype)))))
         return fail(JH_ERR_ALIGN, "add_layernorm: pointers must be aligned to their elements");
+    if ((x == out && x_dtype != out_dtype) || (x == h && x_dtype != h_dtype) || out == h || (residual && out == residual))
+        return fail(JH_ERR_ARG, "add_layernorm: out may be x, and h residual or x, of the same dtype, and no more");
     return check_hip(jh::launch_add_layernorm(x_dtype, h_dtype, out_dtype, d, x, residual, gamma, beta, h, out, mean, rstd, M, N,
                                               epsilon, static_cast<hipStream_t>(stream)),
                      "add_layernorm launch");
@@ -565,6 +568,9 @@ int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t
             !aligned(dh, real_size(h_dtype)) || !aligned(dresidual, real_size(h_dtype)) || !aligned(mean, 4) ||
             !aligned(rstd, 4) || !aligned(gamma, 4))
             return fail(JH_ERR_ALIGN, "add_layernorm_bwd: pointers must be aligned to their elements");
+        if ((dx && (dx == h || dx == dh || dx == dresidual)) || (dresidual && (dresidual == h || dresidual == dy)) ||
+            (dgamma && dgamma == dbeta))
+            return fail(JH_ERR_ARG, "add_layernorm_bwd: dx may be dy, dresidual may be dh, and no more");
         if (dgamma || dbeta) {
             const size_t need = jh::add_layernorm_bwd_workspace_size(M, N);
             if (need && (!workspace || workspace_bytes < need))

@@ -10,14 +10,18 @@
 //   dr_j = rstd (a_j - sum a / N - n_j sum a n / N) + dh_j,  dx = drop(dr)
 //   dgamma_j = sum over rows of dy_j n_j,  dbeta_j = sum over rows of dy_j
 //
-// A row is read once, held in registers, and written once.  The mean is summed in
-// 64 bits and the squares are those of the distances from it, also in 64 bits: no
-// row overflows or cancels in them.
+// A row is read once, held in registers, and written once: bound by HBM.  32768 x
+// 4096 bf16 with a residual and dropout take 200 us forward (5.4 TB/s; 260 while the
+// loads of x and r were waited for one by one), 255 us backward (5.3 TB/s; 454 so).
+//
+// The mean is summed in 64 bits and so are the squares of the distances from it: no
+// row overflows or cancels in them, for a convert and an addition an element.
 //
 // Backward: a group of threads goes over many rows with its columns' two sums in
 // registers, so dy and h are read once for the row's gradient and the columns'; a
 // block leaves one row of partial sums in the workspace, and a second kernel adds
-// those in order.  No atomics: the results do not depend on timing.
+// those in order.  As many blocks as are resident: 512 of 512 threads at 4096 columns
+// (256: 301 us, 1024: 263).  No atomics: the results do not depend on timing.
 #include <algorithm>
 
 #include "launch.hpp"

@@ -8,14 +8,23 @@
 //
 // One pass over a row: every thread keeps the maximum and the sums of its own
 // pieces of 8 neighbouring elements, the sums relative to its maximum, and the
-// block joins them at the end.
+// block joins them at the end.  Bound by HBM: 4096 x 50257 bf16 73 us, 5.7 TB/s,
+// where a plain read of as many bytes gets 5.1 to 6.3.  What that took:
+//   64 registers, for 32 waves a CU (90 us; 147 with one block of 1024 threads);
+//   whole turns of 4 pieces without checks, their loads under way together (72 us;
+//   checks around each load made the compiler wait for it before the next);
+//   512 threads a row, not 1024: what a wave spends on joining is as much as it
+//   spends on 100 elements a thread.
 //
 // The k alternatives are the first in the order (value falling, index rising).
 // Each thread also keeps its largest value and the first of its pieces that has
 // it.  The k-th of these pairs (value, piece) bounds what can be among the first
 // k, since k threads hold an element at least as far in front; only those k
 // threads can hold more.  They read their pieces again and put the elements that
-// reach the bound in LDS, where each counts those before it.
+// reach the bound in LDS, where each counts those before it.  No row, whatever its
+// values, has more of them than k threads have elements.  4096 x 50257 bf16 take 89,
+// 97 and 205 us with 1, 20 and 64 alternatives, 2048 x 50257 fp32 74 us with 5
+// (5.6 TB/s); there the six barriers between these steps cost most.
 //
 // A row may be split over blocks, whose results, their k alternatives among them,
 // are then joined by a second kernel.
@@ -352,7 +361,12 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
     }
 }
 
-// how rows are split, and the threads of a block
+// How rows are split, and the threads of a block.  Few long rows are split for the chip's
+// sake: 64 x 128256 bf16 take 33 us whole, 20 in parts; 512 x 128256 49 and 35.  Below 65536
+// the second launch costs the caller more than it gives (64 x 32000 fp32: 16 us and 20).
+// A wave a row up to 8192 elements: 16384 x 8000 bf16 52.6 us, with 256 threads 57.9; 65536 x
+// 1000 38 and 85; with many alternatives their keys leave few such blocks a CU.  1024 threads
+// where a block a CU is all there is.
 struct Split {
     int parts, width, threads;
 };
@@ -369,7 +383,8 @@ Split split_of(int M, int N, int top) {
 
 template <typename T, int BT>
 void launch_parts(const LogprobArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)std::min(a.M, 1 << 20), (unsigned)a.parts);
+    // the runtime takes fewer than 2^32 threads a launch
+    const dim3 grid((unsigned)std::min(a.M, (1 << 20) / a.parts), (unsigned)a.parts);
     if (a.top) {
         const int turns = a.width / (8 * BT) + (a.width % (8 * BT) != 0);
         logprobs_kernel<T, BT, true><<<grid, BT, sizeof(uint64_t) * std::max(BT, 8 * turns * a.top), s>>>(a);
@@ -452,7 +467,8 @@ __global__ __launch_bounds__(BT) void logprobs_bwd_kernel(GradArgs a) {
 template <typename T, int BT>
 hipError_t launch_grad(const GradArgs& a, hipStream_t s) {
     constexpr int W = 8 * BT * kGradPieces<T>;
-    logprobs_bwd_kernel<T, BT><<<dim3((unsigned)((a.N + W - 1) / W), (unsigned)std::min(a.M, 65535)), BT, 0, s>>>(a);
+    const int blocks = (a.N + W - 1) / W;  // of a row, at most 1024
+    logprobs_bwd_kernel<T, BT><<<dim3((unsigned)blocks, (unsigned)std::min({a.M, 65535, (1 << 23) / blocks})), BT, 0, s>>>(a);
     return hipGetLastError();
 }
 // rows of one wave's width in waves of their own: 65536 x 1000 bf16 keep half of 256 threads idle

@@ -212,6 +212,14 @@ def test_in_place_and_padding(dev, N, pad):
     assert torch.equal(x, want) and torch.equal(whole[:, N:], behind)
 
 
+@pytest.mark.parametrize("N,top", [(2**21, 64), (2**21, 0), (122881, 64), (600001, 33)])
+def test_longest_rows(dev, N, top):
+    """Rows split by what the keys of many alternatives take."""
+    case(f"token_logprobs 3x{N} top {top}")
+    x, tokens = _logits(dev, 3, N, bf16, 11, 1), _tokens(dev, 3, N)
+    _check(x, tokens, 1.0, ops.token_logprobs(x, tokens, top=top), top)
+
+
 def test_rows_beyond_the_blocks(dev):
     """More items than the grid takes at once, and rows of one element to a few."""
     for M, N, top in ((1_100_000, 5, 3), (1_050_000, 1, 1)):

@@ -38,9 +38,10 @@ def test_generator_vectors():
     (dict(p=-0.1), ARG), (dict(p=1.0), ARG), (dict(p=NAN), ARG), (dict(p=1.0 - 2.0**-18), ARG),
     (dict(rng=None), NULL), (dict(x=None), NULL), (dict(out=None), NULL), (dict(rng=P + 4), ALIGN), (dict(x=P + 2), ALIGN),
     (dict(out=P + 1), ALIGN), (dict(res=P + 1), ALIGN), (dict(M=0, x=None, out=None, rng=None), OK), (dict(N=0, x=None), OK),
+    (dict(out=P), ARG),  # in place with another dtype
 ])
 def test_dropout_statuses(change, status):
-    a = dict(x_dtype=F32, out_dtype=BF16, p=0.1, rng=P, offset=0, x=P, res=P, out=P, M=4, N=8)
+    a = dict(x_dtype=F32, out_dtype=BF16, p=0.1, rng=P, offset=0, x=P, res=2 * P, out=3 * P, M=4, N=8)
     a.update(change)
     assert _lib.lib().jules_hip_dropout(*a.values(), None) == status
 
@@ -51,9 +52,11 @@ def test_dropout_statuses(change, status):
     (dict(rng=None), NULL), (dict(x=None), NULL), (dict(out=None), NULL), (dict(x=P + 2), ALIGN), (dict(res=P + 1), ALIGN),
     (dict(h=P + 1), ALIGN), (dict(gamma=P + 2), ALIGN), (dict(beta=P + 1), ALIGN), (dict(mean=P + 2), ALIGN), (dict(rstd=P + 2), ALIGN),
     (dict(out=P + 1), ALIGN), (dict(rng=P + 4), ALIGN), (dict(M=0, x=None), OK), (dict(N=0, out=None), OK),
+    (dict(h=P), ARG), (dict(out=P, out_dtype=BF16), ARG),  # in place with another dtype
+    (dict(out=3 * P), ARG), (dict(out=2 * P, out_dtype=BF16), ARG),  # out is h, or the residual
 ])
 def test_add_layernorm_statuses(change, status):
-    a = dict(x_dtype=F32, h_dtype=BF16, out_dtype=F32, p=0.1, rng=P, offset=0, x=P, res=P, gamma=P, beta=P, h=P, out=P, mean=P, rstd=P,
+    a = dict(x_dtype=F32, h_dtype=BF16, out_dtype=F32, p=0.1, rng=P, offset=0, x=P, res=2 * P, gamma=P, beta=P, h=3 * P, out=4 * P, mean=P, rstd=P,
              M=4, N=8, eps=1e-5)
     a.update(change)
     assert _lib.lib().jules_hip_add_layernorm(*a.values(), None) == status
@@ -65,9 +68,10 @@ def test_add_layernorm_statuses(change, status):
     (dict(dy=P + 2), ALIGN), (dict(h=P + 1), ALIGN), (dict(dh=P + 1), ALIGN), (dict(dx=P + 2), ALIGN), (dict(dr=P + 1), ALIGN),
     (dict(dgamma=P + 2), ALIGN), (dict(dbeta=P + 2), ALIGN), (dict(gamma=P + 2), ALIGN), (dict(ws=P + 2), ALIGN),
     (dict(ws=None), WS), (dict(ws_bytes=255), WS), (dict(N=0, dy=None), OK),
+    (dict(dx=2 * P), ARG), (dict(dx=3 * P), ARG), (dict(dx=5 * P), ARG), (dict(dr=2 * P), ARG), (dict(dr=P), ARG), (dict(dbeta=6 * P), ARG),
 ])
 def test_add_layernorm_bwd_statuses(change, status):
-    a = dict(x_dtype=F32, h_dtype=BF16, p=0.1, rng=P, offset=0, dy=P, h=P, dh=P, mean=P, rstd=P, gamma=P, dx=P, dr=P, dgamma=P, dbeta=P,
+    a = dict(x_dtype=F32, h_dtype=BF16, p=0.1, rng=P, offset=0, dy=P, h=2 * P, dh=3 * P, mean=P, rstd=P, gamma=P, dx=4 * P, dr=5 * P, dgamma=6 * P, dbeta=7 * P,
              M=4000, N=8, ws=P, ws_bytes=1 << 20)
     a.update(change)
     if "ws_bytes" in change:
