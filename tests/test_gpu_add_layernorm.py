@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from jules_amd import ops
+from jules_amd import _lib, ops
 from tests.decoder64 import F32, f64
 from tests.helpers import case
 from tests.training64 import SLACK, drop32, kept, layernorm64, layernorm_bwd64, step, threshold
@@ -166,6 +166,72 @@ def test_in_place(dev, N):
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is dy2 and got[1] is dh2
 
 
+@pytest.mark.parametrize("M,N", [(5000, 300), (3000, 2000), (700, 3000), (1500, 8000), (600, 12000)])
+def test_in_place_of_many_rows(dev, M, N):
+    """Rows whose columns' sums are left in the workspace."""
+    dy, h, dh = (_rows(dev, M, N, bf16, i) for i in range(3))
+    gamma, _ = _weights(dev, N, 1)
+    rng = _rng(dev)
+    _, _, mean, rstd = ops.add_layernorm(h, None, gamma)
+    want = ops.add_layernorm_bwd(dy, h, mean, rstd, gamma, dh, p=0.1, rng=rng)
+    got = ops.add_layernorm_bwd(dy, h, mean, rstd, gamma, dh, p=0.1, rng=rng, dx=dy, dresidual=dh)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is dy and got[1] is dh
+
+
+@pytest.mark.parametrize("N", [100, 1000, 3000, 20001])
+def test_outputs_of_other_types(dev, N):
+    """y in fp32 of bf16 rows and the reverse; h of x where there is no residual, x's own place among them."""
+    x, r = _rows(dev, 5, N, bf16, 1), _rows(dev, 5, N, f32, 2)
+    gamma, beta = _weights(dev, N, 1)
+    for p in (0.0, 0.3):
+        out = ops.add_layernorm(x, r, gamma, beta, p=p, rng=_rng(dev), out=torch.empty(5, N, device=dev))
+        _check_forward(x, r, gamma, beta, p, *out)
+        out = ops.add_layernorm(r, x, gamma, beta, p=p, rng=_rng(dev), out=torch.empty(5, N, dtype=bf16, device=dev))
+        _check_forward(r, x, gamma, beta, p, *out)
+        out = ops.add_layernorm(x, None, gamma, beta, p=p, rng=_rng(dev), h=torch.empty(5, N, device=dev))
+        _check_forward(x, None, gamma, beta, p, *out)
+        want = ops.add_layernorm(x, None, gamma, beta, p=p, rng=_rng(dev))
+        mine = x.clone()
+        got = ops.add_layernorm(mine, None, gamma, beta, p=p, rng=_rng(dev), h=mine)
+        assert got[1] is mine and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("M,N", [(6, 100), (6, 5000), (900, 2000), (6, 20001)])
+def test_outputs_that_are_not_wanted(dev, M, N):
+    """Through the C ABI: each output alone has the bits that it has beside the others."""
+    dy, h = _rows(dev, M, N, bf16, 1), _rows(dev, M, N, bf16, 2)
+    gamma, _ = _weights(dev, N, 1)
+    _, _, mean, rstd = ops.add_layernorm(h, None, gamma)
+    want = ops.add_layernorm_bwd(dy, h, mean, rstd, gamma, p=0.2, rng=_rng(dev))
+    rng, ws = _rng(dev), ops.add_layernorm_bwd_workspace(M, N, dev)
+    for i in range(4):
+        out = [torch.zeros_like(t) if k == i else None for k, t in enumerate(want)]
+        st = _lib.lib().jules_hip_add_layernorm_bwd(
+            1, 1, 0.2, rng.data_ptr(), 0, dy.data_ptr(), h.data_ptr(), None, mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(),
+            *(None if t is None else t.data_ptr() for t in out), M, N, ws.data_ptr(), ws.numel() * 4,
+            torch.cuda.current_stream().cuda_stream)
+        assert st == 0 and torch.equal(out[i], want[i]), i
+
+
+def test_offsets_past_32_bits(dev):
+    """2.3 * 10^9 elements: the first and the last rows, and the columns' sums of rows that are 0 but for the last."""
+    M, N = 140000, 16384
+    case(f"add_layernorm {M}x{N}")
+    rows = torch.tensor([0, 1, M - 2, M - 1], device=dev)
+    x = torch.zeros(M, N, dtype=bf16, device=dev)
+    x[rows] = _rows(dev, 4, N, bf16, 1)
+    y, h, mean, rstd = ops.add_layernorm(x, None, p=0.3, rng=_rng(dev))
+    keep = kept(M, N, 0.3, RNG, 0, rows.cpu().numpy())
+    h32 = np.where(keep, x[rows].float().cpu().numpy() * np.float32(65536 / (65536 - threshold(0.3))), np.float32(0))
+    want, _, _, bound = layernorm64(h32, None, None, EPS)
+    assert torch.equal(h[rows].cpu(), torch.from_numpy(h32).to(bf16)) and not y[2:M - 2].any()
+    assert (np.abs(f64(y[rows]) - want) <= bound + SLACK * step(bf16) * np.abs(want) + TINY).all()
+    del y
+    dx, dr, dgamma, dbeta = ops.add_layernorm_bwd(x, h, mean, rstd, p=0.3, rng=_rng(dev))
+    _check_backward(x[rows], h[rows], mean[rows], rstd[rows], None, None, 0.0, (None, dr[rows], dgamma, dbeta), rows_added=M)
+    assert not dr[2:M - 2].any() and (dx[rows].cpu()[~torch.from_numpy(keep)] == 0).all()
+
+
 @pytest.mark.parametrize("N", [100, 500, 2000, 8000, 12000, 20001])
 def test_extreme_rows(dev, N):
     """Equal elements, NaN, infinities, tiny, huge and far-off values; rows beside them are theirs alone."""
@@ -266,10 +332,10 @@ def test_streams_and_workspaces(dev):
             assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
 
 
-def test_graph(dev):
+@pytest.mark.parametrize("M,N", [(300, 1500), (1200, 1500), (600, 5000)])
+def test_graph(dev, M, N):
     """Forward and backward in one graph, the position moved on between the replays, eager
     calls between them."""
-    M, N = 300, 1500
     x, r, dy = (_rows(dev, M, N, bf16, i) for i in range(3))
     gamma, beta = _weights(dev, N, 1)
     rng = _rng(dev)

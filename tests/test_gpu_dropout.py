@@ -61,6 +61,15 @@ def test_more_than_one_turn_of_the_blocks(dev, M, N):
     assert _same(y, _want(x, None, 0.2, bf16))
 
 
+def test_offsets_past_32_bits(dev):
+    """2.3 * 10^9 elements: the first and the last rows."""
+    M, N = 70001, 32767
+    case(f"dropout {M}x{N}")
+    rows = np.array([0, 1, M - 2, M - 1])
+    y = ops.dropout(torch.ones(M, N, dtype=bf16, device=dev), 0.5, _rng(dev))
+    assert torch.equal(y[torch.from_numpy(rows).to(dev)].cpu() != 0, torch.from_numpy(kept(M, N, 0.5, (SEED, AT), 0, rows)))
+
+
 @pytest.mark.parametrize("N", [37, 1024])
 def test_in_place(dev, N):
     x, r = _rows(dev, 50, N, f32, 1), _rows(dev, 50, N, f32, 2)

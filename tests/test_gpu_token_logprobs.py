@@ -237,6 +237,25 @@ def test_rows_beyond_the_blocks(dev):
         assert ((dx.double() - want).abs() <= 1000 * 2.0**-24).all()
 
 
+def test_offsets_past_32_bits(dev):
+    """2.3 * 10^9 elements: the first and the last rows; every other row of them."""
+    M, N = 45700, 50257
+    case(f"token_logprobs {M}x{N}")
+    x = torch.zeros(M, N, dtype=bf16, device=dev)
+    rows = torch.tensor([0, 2, M - 4, M - 2], device=dev)
+    x[rows] = _logits(dev, 4, N, bf16, 3)
+    tokens, g = _tokens(dev, M, N), _normal(dev, M)
+    out = ops.token_logprobs(x, tokens, top=5)
+    part = lambda o, r: ops.TokenLogprobs(*(v[r] for v in o))  # noqa: E731
+    _check(x[rows], tokens[rows], 1.0, part(out, rows), 5)
+    half = ops.token_logprobs(x[::2], tokens[::2].contiguous(), top=5)
+    assert all(torch.equal(a[::2], b) for a, b in zip(out, half))
+    dx = ops.token_logprobs_bwd(x, tokens, out.lse, g)
+    _check_bwd(x[rows], tokens[rows], out.lse[rows], None, g[rows], None, 1.0, dx[rows])
+    ops.token_logprobs_bwd(x[::2], tokens[::2].contiguous(), half.lse, g[::2].contiguous(), out=x[::2])
+    assert torch.equal(x[::2], dx[::2])
+
+
 def test_leading_dimensions_and_out(dev):
     x = _logits(dev, 12, 600, bf16, 1, 0, 8)
     x3 = x._base.view(3, 4, 608)[..., :600]
