@@ -622,9 +622,10 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
     _one_device(("logits", "tokens", "workspace", *TokenLogprobs._fields), logits, tokens, workspace,
                 *((None,) * 5 if out is None else out))
     if out is None:
-        lse = logits.new_empty(lead, dtype=torch.float32)
+        # one allocation: two more cost a call more than views of it do
+        lse, entropy, *logp = logits.new_empty((2 if tokens is None else 3, *lead), dtype=torch.float32).unbind()
         top_logp = logits.new_empty((*lead, top), dtype=torch.float32) if top else None
-        out = TokenLogprobs(None if tokens is None else torch.empty_like(lse), lse, torch.empty_like(lse),
+        out = TokenLogprobs(logp[0] if logp else None, lse, entropy,
                             torch.empty_like(top_logp, dtype=torch.int32) if top else None, top_logp)
     if workspace is None:
         ws_bytes = lib().jules_hip_token_logprobs_workspace_size(M, N, top)
