@@ -15,7 +15,8 @@
 // loads of x and r were waited for one by one), 255 us backward (5.3 TB/s; 454 so).
 //
 // The mean is summed in 64 bits and so are the squares of the distances from it: no
-// row overflows or cancels in them, for a convert and an addition an element.
+// row whose distances stay within fp32 overflows or cancels in them, for a convert and
+// an addition an element.
 //
 // Backward: a group of threads goes over many rows with its columns' two sums in
 // registers, so dy and h are read once for the row's gradient and the columns'; a
@@ -212,9 +213,7 @@ __global__ __launch_bounds__(1024) void add_layernorm_long_kernel(ForwardArgs a)
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
         }
-        pieces([&](int j, int n, const f32x8_t& h) {
-            write_y(a, row, j, n, h, mean, rstd);
-        });
+        pieces([&](int j, int n, const f32x8_t& h) { write_y(a, row, j, n, h, mean, rstd); });
     }
 }
 
@@ -225,6 +224,11 @@ void launch_forward(const ForwardArgs& a, hipStream_t s) {
     add_layernorm_kernel<XT, RT, RES, G, NP><<<(unsigned)std::min((int64_t)1 << 20, rows), G < 256 ? 256 : G, 0, s>>>(a);
 }
 
+// A block a row, none of its threads idle at the widths' upper ends, and as few of them as
+// the registers allow, for the most rows in flight (dropout and residual, bf16): 65536 x 1024
+// in waves of their own 104 us, 256 threads a row, half of them idle, 167; 32768 x 2048 with
+// 256 threads of 8 elements 114, waves of 32 126; x 4096 with 256 of 16 199, 512 of 8 236; 8192
+// x 8192 with 256 of 32 110, 512 of 16 126; 4096 x 16384 with 1024 of 16 133, 512 of 32 155.
 template <typename XT, typename RT, bool RES>
 hipError_t launch_forward(const ForwardArgs& a, hipStream_t s) {
     if (a.N <= 128)
@@ -544,7 +548,9 @@ __global__ __launch_bounds__(1024) void layernorm_fold_kernel(const float* parti
     }
 }
 
-// how many blocks, and with them partial rows, the backward pass has
+// How many blocks, and with them partial rows, the backward pass has: what is resident.
+// 65536 x 1024 bf16 in waves of their own: 1024 blocks 132 us, 512 144; with 256 threads a row,
+// as at 2048: 144 and 238; 32768 x 4096: 512 blocks 255, 256 301; 8192 x 8192: 256 127, 192 139.
 int backward_blocks(int M, int N) {
     if (N <= 1024) {
         const int rows = N <= 128 ? 16 : 4;
@@ -557,6 +563,9 @@ template <typename XT, typename HT, int G, int NP>
 void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
     add_layernorm_bwd_kernel<XT, HT, G, NP><<<(unsigned)blocks, G < 256 ? 256 : G, 0, s>>>(a);
 }
+// The columns' sums take 16 registers a piece, so the threads hold fewer than forward:
+// 32768 x 4096 bf16 with 512 of 8 elements 256 us, 256 of 16 275 at best; 8192 x 8192 with 1024
+// of 8 127, 512 of 16 136; 4096 x 16384 with 1024 of 16 151, 512 of 32 178.
 template <typename XT, typename HT>
 void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
     if (a.N <= 128) {
