@@ -19,7 +19,7 @@ namespace {
 template <typename XT, typename OT, bool RES>
 __global__ __launch_bounds__(256) void dropout_kernel(Dropout d, const XT* x, const OT* r, OT* out, int M, int N) {
     const int pieces = N / 8 + (N % 8 != 0);
-    const DropKey key = drop_key(d);
+    const DropKey key = d.t ? drop_key(d) : DropKey{};  // t = 0: rng may be null, and every element is kept
     // a thread's pieces lie `stride` apart, in rows and pieces: one division for all of them
     const uint32_t stride = gridDim.x * 256, first = blockIdx.x * 256 + threadIdx.x;
     const int rows_on = (int)(stride / (uint32_t)pieces), pieces_on = (int)(stride % (uint32_t)pieces);
@@ -31,7 +31,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(Dropout d, const XT* x, co
         const Raw8<XT> raw = load_raw(x + at, n);
         Raw8<OT> old;
         if constexpr (RES) old = load_raw(r + at, n);
-        f32x8_t y = drop8(values(raw), key, d, (uint32_t)row, (uint32_t)piece);
+        f32x8_t y = values(raw);
+        if (d.t) y = drop8(y, key, d, (uint32_t)row, (uint32_t)piece);
         if constexpr (RES) {
             const f32x8_t v = values(old);
 #pragma unroll

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from jules_amd import ops
+from jules_amd import _lib, ops
 from tests.helpers import case
 from tests.training64 import drop32, kept, threshold
 
@@ -51,6 +51,30 @@ def test_widths(dev, N):
         y = ops.dropout(x, p, _rng(dev), offset=11, residual=r, dtype=None if rt else ot)
         torch.cuda.synchronize()
         assert y.dtype == ot and _same(y, _want(x, r, p, ot, 11)), (M, N, p)
+
+
+@pytest.mark.parametrize("N", [1, 8, 13, 768, 5001])
+def test_nothing_dropped_without_rng(dev, N):
+    """p = 0, or one that rounds to it, takes no rng (evaluation): x, or its sum with the residual, in each
+    combination of types, through the front end and the C ABI."""
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for xt, rt, ot in ((f32, None, f32), (bf16, None, bf16), (f32, None, bf16), (bf16, None, f32), (f32, f32, f32), (bf16, bf16, bf16),
+                       (bf16, f32, f32), (f32, bf16, bf16)):
+        case(f"dropout 33x{N} {xt} {rt} {ot} p=0 without rng")
+        x = _rows(dev, 33, N, xt, N)
+        x[0, 0], x[32, N - 1] = float("nan"), float("inf")
+        r = None if rt is None else _rows(dev, 33, N, rt, N + 1)
+        want = _want(x, r, 0.0, ot)
+        y = ops.dropout(x, 0.0, residual=r, dtype=None if rt else ot)
+        torch.cuda.synchronize()
+        assert y.dtype == ot and _same(y, want), (xt, rt, ot)
+        for p in (0.0, 2.0**-18):
+            out = torch.empty_like(want, device=dev)
+            st = lib.jules_hip_dropout(int(xt == bf16), int(ot == bf16), p, None, 5, x.data_ptr(), None if r is None else r.data_ptr(),
+                                       out.data_ptr(), 33, N, stream)
+            torch.cuda.synchronize()
+            assert st == 0 and _same(out, want), (xt, rt, ot, p)
+    assert torch.equal(ops.dropout(x[1:3], 0.0, out=x[1:3]).cpu(), x[1:3].cpu())
 
 
 @pytest.mark.parametrize("M,N", [(70000, 40), (70000, 33), (9000, 520), (1, 3000001)])
