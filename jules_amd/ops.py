@@ -455,8 +455,8 @@ def add_layernorm(x, residual=None, gamma=None, beta=None, eps=1e-5, p=0.0, rng=
     reference, whose fusedLayerNorm is layernorm above).  x and residual fp32 or bf16, each by
     itself, residual or None; gamma, beta fp32 or None (ones, zeros); p, rng,
     offset: dropout's.  Returns (y, h, mean, rstd), what add_layernorm_bwd takes: y of x's dtype (or of
-    out's), h of residual's, or of x's without one (x itself where p is 0), mean and rstd
-    fp32.  out may be x, h may be residual."""
+    out's), h of residual's, or of x's without one (x itself where p is 0 and out is not
+    x), mean and rstd fp32.  out may be x, h may be residual."""
     _need(x, "x", _REAL)
     M, N = _rows(x)
     p, rng_ptr, offset = _drop_args(p, rng, offset)
@@ -476,7 +476,8 @@ def add_layernorm(x, residual=None, gamma=None, beta=None, eps=1e-5, p=0.0, rng=
         _need(rstd, "rstd", (torch.float32,), numel=M)
     _one_device(("x", "residual", "gamma", "beta", "rng", "out", "h", "mean", "rstd"), x, residual, gamma, beta, rng, out, h, mean,
                 rstd)
-    if h is None and (residual is not None or p > 0.0):
+    # without a residual and dropout h is x, unless y takes its place
+    if h is None and (residual is not None or p > 0.0 or (out is not None and out.data_ptr() == x.data_ptr())):
         h = torch.empty_like(x if residual is None else residual)
     if out is None:
         out = torch.empty_like(x)

@@ -166,6 +166,23 @@ def test_in_place(dev, N):
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is dy2 and got[1] is dh2
 
 
+@pytest.mark.parametrize("M,N", [(6, 100), (700, 2000), (6, 20001)])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_in_place_without_a_residual(dev, M, N, dtype):
+    """out = x where h would be x: h is what x was, and the gradients are those of the call beside it."""
+    x, dy = _rows(dev, M, N, dtype, 1), _rows(dev, M, N, dtype, 2)
+    gamma, beta = _weights(dev, N, 1)
+    want = ops.add_layernorm(x, None, gamma, beta)
+    assert want[1] is x
+    grads = ops.add_layernorm_bwd(dy, *want[1:], gamma)
+    for out in (lambda t: t, lambda t: t.view(M, N)):  # x itself, and another tensor of the same place
+        mine = x.clone()
+        got = ops.add_layernorm(mine, None, gamma, beta, out=out(mine))
+        assert torch.equal(mine, want[0]) and torch.equal(got[1], x)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(ops.add_layernorm_bwd(dy, *got[1:], gamma), grads))
+
+
 @pytest.mark.parametrize("M,N", [(5000, 300), (3000, 2000), (700, 3000), (1500, 8000), (600, 12000)])
 def test_in_place_of_many_rows(dev, M, N):
     """Rows whose columns' sums are left in the workspace."""
