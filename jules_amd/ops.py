@@ -303,9 +303,20 @@ def matmul_w8a8(A, B, scale_a, scale_b, bias=None, out=None):
     return out
 
 
+def _c_int(n, name):
+    """A count as the C ABI's int takes it: ctypes would cut a larger one off."""
+    n = int(n)
+    if not -2**31 <= n < 2**31:
+        raise ValueError(f"{name} {n} is not within 32 bits")
+    return n
+
+
 def _rows(x):
     N = x.shape[-1] if x.dim() > 0 else 1
-    return x.numel() // max(N, 1) if N else 0, N
+    M = x.numel() // max(N, 1) if N else 0
+    if M >= 2**31 or N >= 2**31:
+        raise ValueError(f"{M} rows of {N} elements: the number of each must be within 32 bits")
+    return M, N
 
 
 def softmax(x, out=None):
@@ -429,6 +440,7 @@ def dropout(x, p, rng=None, offset=0, residual=None, dtype=None, out=None):
     2^-16.  x fp32 or bf16; the result of `dtype` (x's), or of residual's and of
     its shape.  out may be x or residual."""
     _need(x, "x", _REAL)
+    M, N = _rows(x)
     p, rng_ptr, offset = _drop_args(p, rng, offset)
     if residual is not None:
         _need(residual, "residual", _REAL if dtype is None else (dtype,), shape=x.shape)
@@ -442,7 +454,6 @@ def dropout(x, p, rng=None, offset=0, residual=None, dtype=None, out=None):
     _one_device(("x", "rng", "residual", "out"), x, rng, residual, out)
     if out is None:
         out = torch.empty_like(x, dtype=dtype)
-    M, N = _rows(x)
     _call(x, lib().jules_hip_dropout, _DT[x.dtype], _DT[dtype], p, rng_ptr, offset, x.data_ptr(), _ptr(residual), out.data_ptr(),
           M, N)
     return out
@@ -492,7 +503,7 @@ def add_layernorm(x, residual=None, gamma=None, beta=None, eps=1e-5, p=0.0, rng=
 
 
 def add_layernorm_bwd_workspace(M, N, device):
-    nbytes = lib().jules_hip_add_layernorm_bwd_workspace_size(int(M), int(N))
+    nbytes = lib().jules_hip_add_layernorm_bwd_workspace_size(_c_int(M, "M"), _c_int(N, "N"))
     return torch.empty((max(nbytes, 4) // 4,), dtype=torch.float32, device=device)
 
 
@@ -586,7 +597,7 @@ def _row_stride(t, name):
 
 
 def token_logprobs_workspace(M, N, top, device):
-    nbytes = lib().jules_hip_token_logprobs_workspace_size(int(M), int(N), int(top))
+    nbytes = lib().jules_hip_token_logprobs_workspace_size(_c_int(M, "M"), _c_int(N, "N"), _c_int(top, "top"))
     return torch.empty((max(nbytes, 8) // 8 + 1,), dtype=torch.int64, device=device)
 
 

@@ -215,3 +215,20 @@ def test_row_strides():
     assert s(torch.zeros(4, 8), "x") == 8 and s(torch.zeros(4, 9)[:, :8], "x") == 9 and s(torch.zeros(2, 3, 9)[..., :8], "x") == 9
     assert s(torch.zeros(2, 1, 9)[..., :8], "x") == 9 and s(torch.zeros(1, 9)[:, :8], "x") == 8 and s(torch.zeros(6, 8)[::2], "x") == 16
     assert s(torch.zeros(8), "x") == 8 and s(torch.zeros(5, 1), "x") == 1 and s(torch.zeros(4, 2)[:, :1], "x") == 2
+
+
+@pytest.mark.parametrize("shape", [(2**32 + 8,), (2**31,), (2**31, 1), (2**32 + 5, 2)])
+def test_sizes_past_32_bits(shape):
+    """More rows, or elements a row, than the C ABI's int holds are refused, not cut off."""
+    x, rng = torch.empty(shape, dtype=bf16, device="meta"), torch.empty(2, dtype=i64, device="meta")
+    rows = torch.empty(shape[:-1], device="meta")
+    _raises(ops.dropout, x, 0.5, rng, match="32 bits")
+    _raises(ops.dropout, x, 0.0, match="32 bits")
+    _raises(ops.add_layernorm, x, match="32 bits")
+    _raises(ops.add_layernorm_bwd, x, x, rows, rows, match="32 bits")
+    _raises(ops.token_logprobs, x, match="32 bits")
+    _raises(ops.token_logprobs_bwd, x, rows, rows, rows, match="32 bits")
+    _raises(ops.add_rmsnorm, x, None, rows, match="32 bits")
+    M, N = (1, *shape) if len(shape) == 1 else shape
+    _raises(ops.add_layernorm_bwd_workspace, M, N, "cpu", match="32 bits")
+    _raises(ops.token_logprobs_workspace, M, N, 0, "cpu", match="32 bits")
