@@ -589,7 +589,7 @@ void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
     } else {
         // the columns first: dx and dr may be dy and dh
         if (a.partial)
-            layernorm_columns_kernel<XT, HT><<<dim3((unsigned)std::min((a.N + 2047) / 2048, 65535), blocks), 256, 0, s>>>(a);
+            layernorm_columns_kernel<XT, HT><<<dim3((unsigned)std::min(a.N / 2048 + (a.N % 2048 != 0), 65535), blocks), 256, 0, s>>>(a);
         if (a.dx || a.dr) add_layernorm_bwd_long_kernel<XT, HT><<<(unsigned)std::min(a.M, 2048), 1024, 0, s>>>(a);
     }
 }

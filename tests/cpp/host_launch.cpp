@@ -340,6 +340,47 @@ static void tiles() {
     }
 }
 
+// A training step's row operators at every size that their entry points take: what they
+// launch is within the runtime's limits, and sizes are formed without overflow.
+static void row_operators() {
+    int launches = 0;
+    stub::on_launch = [&](const stub::Launch& l) {
+        ++launches;
+        EXPECT(l.grid.x >= 1 && l.grid.x <= 1u << 31 && l.grid.y >= 1 && l.grid.y <= 65535, "%s: grid %u x %u", l.kernel.c_str(), l.grid.x,
+               l.grid.y);
+    };
+    const int kTop = INT32_MAX;
+    for (int N : {1, 7, 8, 500, 1024, 4096, 5001, 16384, 16385, 1 << 21, 1 << 27, (1 << 28) + 1, kTop - 4096, kTop - 2047, kTop - 2046, kTop - 1, kTop})
+        for (int M : {1, 2, 16, 65, 300, 512, 513, 2049, 70000, 1 << 22, 1 << 30, kTop}) {
+            if ((int64_t)M * N > int64_t(1) << 40) continue;
+            for (int t : {JH_F32, JH_BF16}) {
+                const int64_t* rng = fake<int64_t>(9);
+                EXPECT(jules_hip_dropout(t, t, 0.1f, rng, 0, fake(0), fake(1), fake(2), M, N, nullptr) == JH_OK, "dropout %d x %d: %s", M, N,
+                       jules_hip_last_error());
+                EXPECT(jules_hip_add_layernorm(t, t, t, 0.1f, rng, 0, fake(0), fake(1), fake(3), fake(4), fake(2), fake(5), fake(6), fake(7), M, N,
+                                               1e-5f, nullptr) == JH_OK,
+                       "add_layernorm %d x %d: %s", M, N, jules_hip_last_error());
+                const size_t bytes = jules_hip_add_layernorm_bwd_workspace_size(M, N);
+                EXPECT(bytes <= 8192 * (size_t)N, "%d x %d: workspace of %zu bytes", M, N, bytes);
+                launches = 0;
+                EXPECT(jules_hip_add_layernorm_bwd(t, t, 0.1f, rng, 0, fake(0), fake(1), fake(2), fake(3), fake(4), fake(5), fake(6), fake(7), fake(8),
+                                                   fake(10), M, N, fake(11), bytes, nullptr) == JH_OK,
+                       "add_layernorm_bwd %d x %d: %s", M, N, jules_hip_last_error());
+                EXPECT(launches >= 1, "add_layernorm_bwd %d x %d", M, N);
+                for (int top : {0, 1, 20, 64}) {
+                    if (N > 1 << 21 || top > N) continue;
+                    const size_t need = jules_hip_token_logprobs_workspace_size(M, N, top);
+                    EXPECT(jules_hip_token_logprobs(t, fake(0), N, 1.0f, fake<int32_t>(1), fake(2), fake(3), fake(4), top, fake<int32_t>(5), fake(6), M, N,
+                                                    fake(7), need, nullptr) == JH_OK,
+                           "token_logprobs %d x %d top %d: %s", M, N, top, jules_hip_last_error());
+                }
+                if (N <= 1 << 21)
+                    EXPECT(jules_hip_token_logprobs_bwd(t, fake(0), N, 1.0f, fake<int32_t>(1), fake(2), fake(3), fake(4), fake(5), fake(6), N, M, N, nullptr) == JH_OK,
+                           "token_logprobs_bwd %d x %d: %s", M, N, jules_hip_last_error());
+            }
+        }
+}
+
 static const struct {
     const char* name;
     void (*run)();
@@ -351,6 +392,7 @@ static const struct {
     {"overlapping_outputs", overlapping_outputs},
     {"mlp_wrappers", mlp_wrappers},
     {"tiles", tiles},
+    {"row_operators", row_operators},
 };
 
 int main(int argc, char** argv) {

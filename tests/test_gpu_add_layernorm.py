@@ -249,6 +249,40 @@ def test_offsets_past_32_bits(dev):
     assert not dr[2:M - 2].any() and (dx[rows].cpu()[~torch.from_numpy(keep)] == 0).all()
 
 
+def test_longest_row(dev):
+    """A row of 2^31 - 1 elements: grids formed near the end of 32 bits, every column's own sums,
+    and the rest at the row's ends and in its middle."""
+    N = 2**31 - 1
+    case(f"add_layernorm 1x{N}")
+    g = torch.Generator(dev).manual_seed(4)
+    h, dy = (torch.empty(1, N, dtype=bf16, device=dev).normal_(generator=g) for _ in range(2))
+    y, _, mean, rstd = ops.add_layernorm(h)
+    dx, dr, dgamma, dbeta = ops.add_layernorm_bwd(dy, h, mean, rstd)
+    torch.cuda.synchronize()
+    total, square, c1, c2, size1, size2 = (0.0,) * 6
+    for i in range(0, N, 1 << 28):
+        part, grad = h[0, i:i + (1 << 28)].double(), dy[0, i:i + (1 << 28)].double()
+        total, square = total + part.sum().item(), square + part.square().sum().item()
+        n = (part - mean.double()) * rstd.double()
+        c1, size1 = c1 + grad.sum().item(), size1 + grad.abs().sum().item()
+        c2, size2 = c2 + (grad * n).sum().item(), size2 + (grad * n).abs().sum().item()
+    assert abs(mean.item() - total / N) <= F32 * abs(total / N) + 2.0**-45
+    var = square / N - (total / N) ** 2
+    assert abs(rstd.item() - (var + EPS) ** -0.5) <= 2 * F32 * (var + EPS) ** -0.5
+    # one row: the columns' sums are its products, rounded as often
+    for i in range(0, N, 1 << 28):
+        at = slice(i, min(i + (1 << 28), N))
+        assert torch.equal(dbeta[at], dy[0, at].float()), i
+        assert torch.equal(dgamma[at], dy[0, at].float() * ((h[0, at].float() - mean) * rstd)), i
+    chain = (N / 1024 + 30) * F32  # as in layernorm_bwd64
+    for at in (slice(0, 5000), slice(2**30 - 2500, 2**30 + 2500), slice(N - 5000, N)):
+        n, grad = (h[0, at].double() - mean.double()) * rstd.double(), dy[0, at].double()
+        assert ((y[0, at].double() - n).abs() <= step(bf16) * SLACK * n.abs() + 4 * F32 * (1 + n.abs())).all()
+        want = rstd.double() * (grad - c1 / N - n * c2 / N)
+        bound = rstd.double() * (chain * size1 / N + n.abs() * chain * size2 / N) + SLACK * step(bf16) * want.abs() + 8 * F32 * (1 + want.abs() + n.abs())
+        assert ((dr[0, at].double() - want).abs() <= bound).all() and dx is dr
+
+
 @pytest.mark.parametrize("N", [100, 500, 2000, 8000, 12000, 20001])
 def test_extreme_rows(dev, N):
     """Equal elements, NaN, infinities, tiny, huge and far-off values; rows beside them are theirs alone."""
