@@ -421,6 +421,10 @@ struct GradArgs {
     int M, N;
 };
 
+// the log of a probability below all fp32 numbers: e^ of it is 0, and its product with what
+// reaches the entropy stays within fp32, so that the two are 0 together
+constexpr float GONE = -150.0f;
+
 // BT threads for 32 bytes each of a row; a row's blocks side by side (rows side by side: 177 us
 // for 4096 x 50257 bf16 instead of 148)
 template <typename T>
@@ -454,7 +458,7 @@ __global__ __launch_bounds__(BT) void logprobs_bwd_kernel(GradArgs a) {
             f32x8_t y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float log = none ? FAR : larger(__builtin_fmaf(v.v[i], a.scale, -lse), FAR);
+                const float log = none ? GONE : larger(__builtin_fmaf(v.v[i], a.scale, -lse), GONE);
                 const float p = __builtin_amdgcn_exp2f(log * LOG2E);
                 y.v[i] = -p * __builtin_fmaf(gh, log + entropy, g);
                 if (j + i == token) y.v[i] += g;

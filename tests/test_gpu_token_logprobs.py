@@ -144,6 +144,24 @@ def test_masked(dev, N, dtype):
     _check_bwd(x[keep], tokens[keep], out.lse[keep], out.entropy[keep], g[keep], -g[keep], 1.0, dx[keep])
 
 
+@pytest.mark.parametrize("N", [9, 1000, 9000, 50257])
+def test_masked_with_large_gradients(dev, N):
+    """What a scaled loss makes of the entropy's gradient: a masked place has none, however large it is."""
+    M = 6
+    x, tokens = _logits(dev, M, N, f32, 13), _tokens(dev, M, N)
+    keep = x[torch.arange(M, device=dev), tokens.long()]
+    for low in (-INF, torch.finfo(f32).min, -1e30):
+        x[:, N // 2:] = low
+        x[torch.arange(M, device=dev), tokens.long()] = keep
+        x[5] = -INF
+        out = ops.token_logprobs(x, tokens)
+        for size in (1e6, 1e9, 1e20, 1e30):
+            g, h = size * _normal(dev, M, 1), size * _normal(dev, M, 2)
+            dx = ops.token_logprobs_bwd(x, tokens, out.lse, g, out.entropy, h)
+            assert torch.isfinite(dx).all() and (dx[x <= -1e30] == 0).all(), (low, size)
+            _check_bwd(x, tokens, out.lse, out.entropy, g, h, 1.0, dx)
+
+
 @pytest.mark.parametrize("N", [9, 1000, 9000, 50257, 128256])
 def test_nan_and_infinity(dev, N):
     """A row with one is NaN everywhere, and no other row."""
