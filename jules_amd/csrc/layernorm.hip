@@ -283,6 +283,12 @@ struct RawGrad {
         for (int i = 0; i < 8; ++i) r.v[i] = (r.v[i] - mean) * rstd;
         return r;
     }
+    // sums of a = dy gamma and of a n; dy is 0 behind the row's end, where the mean alone times
+    // rstd may be past fp32: 0 times that is left out
+    __device__ __forceinline__ static void add(float (&c)[2], float a, float norm) {
+        c[0] += a;
+        c[1] = a == 0.0f ? c[1] : __builtin_fmaf(a, norm, c[1]);
+    }
     // dr and dx of the piece
     __device__ __forceinline__ void write(const BackwardArgs& a, const DropKey& key, int64_t row, int j, int n, const f32x8_t& norm,
                                           const f32x8_t& gamma, float rstd, float c1, float c2) const {
@@ -356,9 +362,7 @@ __device__ __forceinline__ void backward_rows(const BackwardArgs& a, int block, 
             const f32x8_t dy = values(raw[t].dy), norm = raw[t].norm(mean, rstd), w = KEEP ? gamma[KEEP ? t : 0] : weight(t);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float g = dy.v[i] * w.v[i];  // 0 behind the row's end
-                c[0] += g;
-                c[1] = __builtin_fmaf(g, norm.v[i], c[1]);
+                RawGrad<XT, HT>::add(c, dy.v[i] * w.v[i], norm.v[i]);
                 if constexpr (SUMS) {
                     sum_n[t].v[i] = __builtin_fmaf(dy.v[i], norm.v[i], sum_n[t].v[i]);
                     sum_y[t].v[i] += dy.v[i];
@@ -487,11 +491,7 @@ __global__ __launch_bounds__(1024) void add_layernorm_bwd_long_kernel(BackwardAr
         pieces(false, [&](int, int, const RawGrad<XT, HT>& raw, const f32x8_t& norm, const f32x8_t& gamma) {
             const f32x8_t dy = values(raw.dy);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float g = dy.v[i] * gamma.v[i];
-                c[0] += g;
-                c[1] = __builtin_fmaf(g, norm.v[i], c[1]);
-            }
+            for (int i = 0; i < 8; ++i) RawGrad<XT, HT>::add(c, dy.v[i] * gamma.v[i], norm.v[i]);
         });
         reduce_group<1024>(c, turn);
         const float c1 = c[0] / (float)a.N, c2 = c[1] / (float)a.N;

@@ -283,6 +283,23 @@ def test_longest_row(dev):
         assert ((dr[0, at].double() - want).abs() <= bound).all() and dx is dr
 
 
+@pytest.mark.parametrize("M,N", [(3, 1), (3, 100), (3, 513), (3, 2047), (3, 5001), (3, 12001), (3, 16387), (20, 40001), (2100, 100),
+                                 (2100, 1001), (600, 2047), (600, 3001), (600, 5001), (600, 12001)])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_equal_elements_far_from_zero(dev, M, N, dtype):
+    """Rows of 1e37 everywhere: a distance of 0 from the mean, where 0 less the mean times rstd is
+    past fp32's range, as it would be for elements behind the row's end."""
+    h = torch.full((M, N), 1e37, device=dev).to(dtype)
+    h[1] = -h[1]
+    dy, dh = _rows(dev, M, N, dtype, 1), _rows(dev, M, N, dtype, 2)
+    gamma, _ = _weights(dev, N, 1)
+    y, _, mean, rstd = ops.add_layernorm(h, None, gamma)
+    assert not y.any()
+    grads = ops.add_layernorm_bwd(dy, h, mean, rstd, gamma, dh)
+    assert all(torch.isfinite(t).all() for t in grads) and not grads[2].any()
+    _check_backward(dy, h, mean, rstd, gamma, dh, 0.0, grads)
+
+
 @pytest.mark.parametrize("N", [100, 500, 2000, 8000, 12000, 20001])
 def test_extreme_rows(dev, N):
     """Equal elements, NaN, infinities, tiny, huge and far-off values; rows beside them are theirs alone."""
