@@ -312,8 +312,9 @@ def _c_int(n, name):
 
 
 def _rows(x):
-    N = x.shape[-1] if x.dim() > 0 else 1
-    M = x.numel() // max(N, 1) if N else 0
+    shape = x.shape
+    N = shape[-1] if shape else 1
+    M = x.numel() // N if N else 0
     if M >= 2**31 or N >= 2**31:
         raise ValueError(f"{M} rows of {N} elements: the number of each must be within 32 bits")
     return M, N
@@ -568,14 +569,18 @@ class TokenLogprobs(NamedTuple):
     top_logp: Optional[torch.Tensor] = None
 
 
+_LOGPROBS_NAMES = ("logits", "tokens", "workspace", *TokenLogprobs._fields)
+
+
 def _row_stride(t, name):
     """Elements between two rows of a tensor whose last dimension is dense and whose
     others lie as those of a dense one would, rows of a padded width among them."""
     if not isinstance(t, torch.Tensor) or t.dtype not in _DT:
         raise ValueError(f"{name}: fp32 or bf16 tensor expected")
-    if t.dim() < 1:
+    shape = t.shape
+    if not shape:
         raise ValueError(f"{name} must have at least one dimension")
-    N = t.shape[-1]
+    N = shape[-1]
     if t.is_contiguous():
         return N
     if N > 1 and t.stride(-1) != 1:
@@ -613,7 +618,6 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
     TokenLogprobs to write into, whose entries that are None are not wanted."""
     stride = _row_stride(logits, "logits")
     M, N = _rows(logits)
-    lead = logits.shape[:-1]
     top = int(top)
     if top < 0 or top > 64 or top > N:
         raise ValueError(f"top {top} must be at most 64 and {N}")
@@ -631,13 +635,13 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
             _need(out.top_ids, "top_ids", (torch.int32,), numel=M * top)
             _need(out.top_logp, "top_logp", (torch.float32,), numel=M * top)
     ws_bytes = 0 if workspace is None else _workspace(workspace, "workspace")
-    _one_device(("logits", "tokens", "workspace", *TokenLogprobs._fields), logits, tokens, workspace,
-                *((None,) * 5 if out is None else out))
+    _one_device(_LOGPROBS_NAMES, logits, tokens, workspace, *(out or ()))
     if out is None:
-        # one allocation: two more cost a call more than views of it do
-        lse, entropy, *logp = logits.new_empty((2 if tokens is None else 3, *lead), dtype=torch.float32).unbind()
+        lead = logits.shape[:-1]
+        # tensors of their own: views of one would count each other's changes in place, which autograd looks at
+        lse = logits.new_empty(lead, dtype=torch.float32)
         top_logp = logits.new_empty((*lead, top), dtype=torch.float32) if top else None
-        out = TokenLogprobs(logp[0] if logp else None, lse, entropy,
+        out = TokenLogprobs(None if tokens is None else torch.empty_like(lse), lse, torch.empty_like(lse),
                             torch.empty_like(top_logp, dtype=torch.int32) if top else None, top_logp)
     if workspace is None:
         ws_bytes = lib().jules_hip_token_logprobs_workspace_size(M, N, top)

@@ -291,6 +291,37 @@ def test_leading_dimensions_and_out(dev):
     assert torch.equal(ops.token_logprobs_bwd(x3, tokens, a.lse, g).view(12, 600), ops.token_logprobs_bwd(x, tokens, a.lse, g))
 
 
+def test_outputs_are_tensors_of_their_own(dev):
+    """What an autograd function returns of them can be changed in place, and a change of one leaves
+    what was saved of another."""
+    x, tokens = _logits(dev, 6, 600, f32, 1).requires_grad_(), _tokens(dev, 6, 600)
+
+    class Logprob(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            out = ops.token_logprobs(x, tokens, top=2)
+            ctx.save_for_backward(x, out.lse, out.entropy)
+            return out.logp, out.entropy
+
+        @staticmethod
+        def backward(ctx, g, h):
+            x, lse, entropy = ctx.saved_tensors
+            return ops.token_logprobs_bwd(x, tokens, lse, g.contiguous(), entropy, h.contiguous())
+
+    logp, entropy = Logprob.apply(x)
+    logp.mul_(0.5)  # a mask, say
+    (logp.sum() + 2.0 * entropy.sum()).backward()
+    o = ops.token_logprobs(x.detach(), tokens)
+    assert torch.equal(logp, 0.5 * o.logp)
+    want = ops.token_logprobs_bwd(x.detach(), tokens, o.lse, torch.full((6,), 0.5, device=dev), o.entropy, torch.full((6,), 2.0, device=dev))
+    assert torch.equal(x.grad, want)
+    for out in (ops.token_logprobs(x.detach(), tokens, top=2), ops.token_logprobs(x.detach(), top=2)):
+        versions = [t._version for t in out if t is not None]
+        out.lse.zero_()
+        assert [t._version for t in out if t is not None] == [v + (t is out.lse) for v, t in zip(versions, (t for t in out if t is not None))]
+        assert all(t._base is None for t in out if t is not None)
+
+
 def test_empty(dev):
     out = ops.token_logprobs(torch.empty(0, 9, device=dev), torch.empty(0, dtype=i32, device=dev), top=2)
     assert out.logp.shape == (0,) and out.top_ids.shape == (0, 2)
