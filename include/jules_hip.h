@@ -449,12 +449,14 @@ int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t
  *   entropy = -sum(p log p), p = exp(z - lse)
  *   top_ids, top_logp [M, top]: the indices of the `top` largest logits, falling, equal
  *             ones by rising index, and their log probabilities
- * tokens int32 [M]: a negative one is none (logp 0, no gradient), one >= N gives NaN.
+ * tokens int32 [M]: a negative one is none: its logp is 0 and dlogp is not looked at. The
+ * row's entropy is as ever, and dentropy reaches the logits: 0 there keeps a padding row's
+ * gradient 0.  One >= N gives NaN.
  * logp, lse, entropy: fp32 [M] or NULL; tokens may be NULL without logp.  0 <= top <=
  * 64, top <= N.
  * -infinity (what a mask forbids) has probability 0.  A row of nothing else: lse and
  * all log probabilities -infinity, entropy 0, gradient 0 whatever reaches it.  A NaN or
- * +infinity in a row: NaN everywhere, top_ids -1.  One pass over the logits, fp32 sums;
+ * +infinity in a row: NaN everywhere but in a negative token's logp, top_ids -1.  One pass over the logits, fp32 sums;
  * deterministic.
  * workspace: jules_hip_token_logprobs_workspace_size(M, N, top) bytes (rows split over
  * workgroups: M < 1024 at N >= 65536, and long rows with many alternatives; 0: NULL will

@@ -612,7 +612,7 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
     each row (jules_hip_token_logprobs; no counterpart in the reference, whose
     fusedCrossEntropyLoss is cross_entropy).  logits fp32 or bf16 [..., N], N up to
     2^21, rows equally far apart (logits[..., :N] of a padded width); tokens
-    int32, one a row, a negative one for none (logp 0), or None; top at most 64.
+    int32, one a row, a negative one for none (logp 0, the rest as ever), or None; top at most 64.
     Returns TokenLogprobs(logp, lse, entropy, top_ids, top_logp): fp32 of logits' leading shape, the last two
     [..., top] int32 and fp32 (None where top is 0), by falling logit and rising index.  out: a
     TokenLogprobs to write into, whose entries that are None are not wanted."""
@@ -656,7 +656,8 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, out=None, workspace=No
 def token_logprobs_bwd(logits, tokens, lse, dlogp, entropy=None, dentropy=None, scale=1.0, out=None):
     """The gradient of token_logprobs' logp and entropy with respect to the logits
     (jules_hip_token_logprobs_bwd), in their dtype: logits, tokens and scale as they were, lse and
-    entropy as it returned them, dlogp and dentropy (or None) fp32, one a row.  out may be logits."""
+    entropy as it returned them, dlogp and dentropy (or None) fp32, one a row.  dlogp is not looked at
+    where the token is negative; dentropy is, so that it has to be 0 in a padding row.  out may be logits."""
     stride = _row_stride(logits, "logits")
     M, N = _rows(logits)
     _need(tokens, "tokens", (torch.int32,), numel=M)

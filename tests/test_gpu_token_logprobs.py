@@ -198,6 +198,23 @@ def test_tokens_that_are_none(dev, N):
     _check_bwd(x[rows], tokens[rows], out.lse[rows], out.entropy[rows], torch.nan_to_num(g[rows]), h[rows], 1.0, dx[rows])
 
 
+@pytest.mark.parametrize("N", [50, 5000, 50257])
+def test_padding_rows(dev, N):
+    """A negative token takes the log probability's gradient away, whatever it holds, and leaves the
+    entropy's: 0 where that is 0, and else what the row has with a dlogp of 0."""
+    x = _logits(dev, 4, N, f32, 2)
+    x[3, 1] = float("nan")
+    tokens = torch.tensor([-1, -7, -(2**31), -1], dtype=i32, device=dev)
+    out = ops.token_logprobs(x, tokens, top=2)
+    assert (out.logp == 0).all() and (out.top_ids[3] == -1).all() and torch.isnan(out.lse[3]) and torch.isnan(out.entropy[3])
+    g = torch.tensor([float("nan"), INF, 3.0, 1.0], device=dev)
+    h = torch.tensor([0.0, 0.5, -0.25, 0.0], device=dev)
+    dx = ops.token_logprobs_bwd(x, tokens, out.lse, g, out.entropy, h)
+    zero = ops.token_logprobs_bwd(x, _tokens(dev, 4, N), out.lse, torch.zeros(4, device=dev), out.entropy, h)
+    assert not dx[0].any() and dx[1:3].any() and torch.equal(dx[:3], zero[:3]) and torch.isnan(dx[3]).all()
+    assert not ops.token_logprobs_bwd(x, tokens, out.lse, g)[:3].any()
+
+
 def _check_bwd(x, tokens, lse, entropy, g, h, scale, dx):
     want, bound = logprobs_bwd64(x, tokens, lse, entropy, g, h, scale)
     assert (np.abs(f64(dx) - want) <= bound + SLACK * step(dx.dtype) * np.abs(want) + 2.0**-120).all()
