@@ -411,7 +411,7 @@ int jules_hip_dropout(int x_dtype, int out_dtype, float p, const int64_t* rng, u
  * in 64 bits.  A NaN or an infinity in a row makes the row's out, mean or rstd NaN
  * (h is as ever).  epsilon >= 0; with 0 a row of equal elements is NaN.
  * Deterministic.  Pointers aligned to their elements; overlaps other than those
- * named are not allowed.
+ * named are not allowed.  M = 0 or N = 0: nothing is written.
  *
  * jules_hip_add_layernorm_bwd: from dy [M, N] (x_dtype: the gradient of out), h
  *   [M, N] (h_dtype), mean and rstd as the forward call left them, gamma, and dh

@@ -471,6 +471,8 @@ def add_layernorm(x, residual=None, gamma=None, beta=None, eps=1e-5, p=0.0, rng=
     x), mean and rstd fp32.  out may be x, h may be residual."""
     _need(x, "x", _REAL)
     M, N = _rows(x)
+    if not N:
+        raise ValueError("x: rows of no elements have no mean")
     p, rng_ptr, offset = _drop_args(p, rng, offset)
     if gamma is not None:
         _need(gamma, "gamma", (torch.float32,), numel=N)

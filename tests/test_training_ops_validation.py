@@ -232,3 +232,11 @@ def test_sizes_past_32_bits(shape):
     M, N = (1, *shape) if len(shape) == 1 else shape
     _raises(ops.add_layernorm_bwd_workspace, M, N, "cpu", match="32 bits")
     _raises(ops.token_logprobs_workspace, M, N, 0, "cpu", match="32 bits")
+
+
+def test_rows_of_no_elements():
+    """They have no mean to return; without rows there is nothing to return."""
+    for x in (torch.zeros(3, 0), torch.zeros(2, 3, 0, dtype=bf16)):
+        _raises(ops.add_layernorm, x, match="no elements")
+        _raises(ops.add_layernorm, x, x, match="no elements")
+    _raises(ops.add_layernorm, torch.zeros(0, 8), match="GPU tensor")
