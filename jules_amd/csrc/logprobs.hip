@@ -374,7 +374,7 @@ Split split_of(int M, int N, int top) {
     // what the keys in LDS allow: `top` threads' elements
     const int most = top ? MAX_KEYS / (8 * top) * (8 * 512) : N;
     int parts = N / most + (N % most != 0);
-    if (M < 1024 && N >= 65536) parts = std::max(parts, std::min(1024 / M, N / 8192));
+    if (M <= 512 && N >= 65536) parts = std::max(parts, std::min(1024 / M, N / 8192));
     parts = std::min(std::max(parts, 1), MAX_PARTS);
     const int width = (N / parts + (N % parts != 0) + 7) / 8 * 8;
     const int threads = width <= 8192 && top <= 8 ? 64 : width <= 8192 ? 256 : M * parts > 256 || width <= 16384 ? 512 : 1024;

@@ -240,3 +240,14 @@ def test_rows_of_no_elements():
         _raises(ops.add_layernorm, x, match="no elements")
         _raises(ops.add_layernorm, x, x, match="no elements")
     _raises(ops.add_layernorm, torch.zeros(0, 8), match="GPU tensor")
+
+
+@pytest.mark.parametrize("N", [65536, 128256, 1 << 20])
+def test_which_rows_are_split(N):
+    """For the chip's sake, up to 512 of 65536 elements and more."""
+    f = _lib.lib().jules_hip_token_logprobs_workspace_size
+    for M in (1, 64, 511, 512):
+        assert f(M, N, 0) > 0, M
+    for M in (513, 768, 1023, 1024, 5000):
+        assert f(M, N, 0) == 0, M
+    assert f(512, 65535, 0) == 0 and f(1, 65535, 1) == 0
