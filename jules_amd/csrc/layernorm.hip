@@ -10,9 +10,12 @@
 //   dr_j = rstd (a_j - sum a / N - n_j sum a n / N) + dh_j,  dx = drop(dr)
 //   dgamma_j = sum over rows of dy_j n_j,  dbeta_j = sum over rows of dy_j
 //
-// A row is read once, held in registers, and written once: bound by HBM.  32768 x
-// 4096 bf16 with a residual and dropout take 200 us forward (5.4 TB/s; 260 while the
-// loads of x and r were waited for one by one), 255 us backward (5.3 TB/s; 454 so).
+// A row is read once, held in registers, and written once: bound by HBM.  A call of
+// 32768 x 4096 bf16 with a residual and dropout takes 203 us forward (5.3 TB/s; 260 while
+// the loads of x and r were waited for one by one), 259 us backward (5.2 TB/s; 454 so).
+// Rows over 16384 elements, which no block holds, are read again after each sum, and for
+// the columns: 2048 x 32768 bf16 184 us forward (2.9 TB/s of the bytes needed), 235
+// backward, fp32 320 and 439.
 //
 // The mean is summed in 64 bits and so are the squares of the distances from it: no
 // row whose distances stay within fp32 overflows or cancels in them, for a convert and
@@ -229,6 +232,9 @@ void launch_forward(const ForwardArgs& a, hipStream_t s) {
 // in waves of their own 104 us, 256 threads a row, half of them idle, 167; 32768 x 2048 with
 // 256 threads of 8 elements 114, waves of 32 126; x 4096 with 256 of 16 199, 512 of 8 236; 8192
 // x 8192 with 256 of 32 110, 512 of 16 126; 4096 x 16384 with 1024 of 16 133, 512 of 32 155.
+// One rule for both types; in fp32 16384 x 4096 take 198 us (5.4 TB/s), 4096 x 16384 251 (4.3),
+// and 8192 x 8192 217 (4.9) with 256 of 32, whose 182 registers leave two blocks a CU, where 512 of 16
+// take 207, 1024 of 8 232 (bf16 118, 125 and 157 in those runs).
 template <typename XT, typename RT, bool RES>
 hipError_t launch_forward(const ForwardArgs& a, hipStream_t s) {
     if (a.N <= 128)
@@ -565,7 +571,8 @@ void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
 }
 // The columns' sums take 16 registers a piece, so the threads hold fewer than forward:
 // 32768 x 4096 bf16 with 512 of 8 elements 256 us, 256 of 16 275 at best; 8192 x 8192 with 1024
-// of 8 127, 512 of 16 136; 4096 x 16384 with 1024 of 16 151, 512 of 32 178.
+// of 8 127, 512 of 16 136; 4096 x 16384 with 1024 of 16 151, 512 of 32 178.  fp32: 16384 x 4096 251 us
+// (5.3 TB/s), 8192 x 8192 255 (5.3), 4096 x 16384 294 (4.6).
 template <typename XT, typename HT>
 void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
     if (a.N <= 128) {
@@ -596,8 +603,9 @@ void launch_backward(const BackwardArgs& a, int blocks, hipStream_t s) {
 
 // Where the columns' sums read dy and h again rather than leave partial sums: the second
 // launch and the workspace cost the caller 4.5 us (64 x 1024: 14.5 us against 18.9), reading
-// again costs more than that from some thousand rows on (512 x 8192 bf16: 15.9 us against 18.9,
-// fp32 26 against 24; 2000 x 1024: 25 against 18.7).
+// again costs more than that from some thousand rows on (2000 x 1024: 25 against 18.7).  One
+// rule for both types: 512 x 8192 bf16 18.4 us against 20.7, fp32 28.0 against 25.5, where it loses;
+// 400 x 16384 24.7 against 29.4, fp32 37.4 against 45.3.
 bool backward_few(int M, int N) { return N <= 16384 && (M <= 512 || (M <= 2048 && M * N <= 1 << 20)); }
 
 template <typename XT, typename HT, int G, int NP>
