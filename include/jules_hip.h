@@ -456,8 +456,8 @@ int jules_hip_add_layernorm_bwd(int x_dtype, int h_dtype, float p, const int64_t
  * 64, top <= N.
  * -infinity (what a mask forbids) has probability 0.  A row of nothing else: lse and
  * all log probabilities -infinity, entropy 0, gradient 0 whatever reaches it.  A NaN or
- * +infinity in a row: NaN everywhere but in a negative token's logp, top_ids -1.  One pass over the logits, fp32 sums;
- * deterministic.
+ * +infinity in a row: NaN everywhere but in a negative token's logp, top_ids -1.
+ * One pass over the logits, fp32 sums; deterministic.
  * workspace: jules_hip_token_logprobs_workspace_size(M, N, top) bytes (rows split over
  * workgroups: M <= 512 at N >= 65536, and long rows with many alternatives; 0: NULL will
  * do), 8-byte aligned, no initialisation, overwritten by every call; calls that overlap

@@ -2,7 +2,7 @@
 // with the workspaces they hold, checked without a GPU: the library's host code,
 // launchers included, built with AddressSanitizer and UndefinedBehaviorSanitizer
 // and linked against hip_stub.cpp.  `host_launch <check>` runs one check and prints
-// "<check> ok"; run by tests/test_host_launch.py.
+// "<check> ok"; run by tests/test_host_launch.py and tests/test_training_host_launch.py.
 #include <algorithm>
 #include <chrono>
 #include <cstdint>
